@@ -1,0 +1,234 @@
+// Keys and values held in 8 bits: a step's new ones into the cache, and a sequence's read back as pages.
+//
+// Blocks of KV8_BLOCK = 16 tokens of a sequence and kv head have one scale each for keys and for values:
+// x ~ q * s with s = max|x| / 127 and q = rint(127 x / max|x|) a whole number (stored as q + 128), or
+// s = max|x| / 448 and q the nearest e4m3 number. The quotient is taken of 127 x (448 x), which is a float32 number whatever the
+// bfloat16 x, so a value halfway between two steps is seen as that and goes to the even one. A block of zeros has the scale
+// zero; a block with a value that is not finite reads back as NaN.
+// A block is put into 8 bits when its last token comes; until then its tokens lie as they came in the slot's open block,
+// so that no value is ever rounded twice and a token's place in the 8-bit pages is written once.
+#define ABK_DEFINE_ERROR
+#include "common.cuh"
+#include "kv8.cuh"
+
+#define KV8_WARPS 4
+
+struct Kv8Write {
+    const __nv_bfloat16 *qkv;  // k head h of row r at qkv + r * row + (n_heads + h) * head_dim, v n_kv_heads heads further
+    long long row;
+    int n_heads, n_kv_heads, n_seqs, one_each;
+    const int *seq_start, *seq_pos0, *seq_len_after, *seq_slot;
+    PagedCache cache;
+    uint8_t *k, *v;
+    float *scales;
+    __nv_bfloat16 *open;
+    int n_pages, *status;
+};
+
+// One block of one head's keys or values, held by a warp: token t of the block, elements 8 c .., in piece i of a lane with
+// 32 i + lane = t * HD / 8 + c.
+template <int HD> struct Kv8Block {
+    static constexpr int PIECES = KV8_BLOCK * HD / 256;
+    uint4 x[PIECES];
+};
+
+template <int HD, int FORM>
+__global__ void __launch_bounds__(32 * KV8_WARPS) kv8_write_kernel(Kv8Write p) {
+    constexpr int LPR = HD / 8, PIECES = Kv8Block<HD>::PIECES;  // lanes to a row of 16-byte pieces
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int which = blockIdx.y * KV8_WARPS + warp;  // keys of the heads, then values of the heads
+    if (which >= 2 * p.n_kv_heads) return;
+    const int j = which / p.n_kv_heads, head = which - j * p.n_kv_heads;
+    // the sequence and its block: block k of a sequence that brings n tokens from row a on has its first row at f_k; unit
+    // a / 16 + 2 s is block 0 and unit f_k / 16 + 2 s + 1 block k > 0 of sequence s, so units of different blocks differ
+    int s = blockIdx.x, first = 0, unit = blockIdx.x;
+    if (!p.one_each) {
+        s = last_not_above(p.seq_start, p.n_seqs, lane, [&](int start, int i) { return start / KV8_BLOCK + 2 * i <= unit; });
+        if (s < 0) return;
+    }
+    const int a = p.seq_start[s], n = p.seq_start[s + 1] - a;
+    if (n <= 0) return;
+    const int start = p.seq_pos0[s], after = p.seq_len_after[s], o = start % KV8_BLOCK;
+    if (!p.one_each && unit != a / KV8_BLOCK + 2 * s) {
+        const int q = unit - 2 * s - 1;
+        if (q * KV8_BLOCK + KV8_BLOCK <= a) return;
+        first = max(1, (q * KV8_BLOCK - a + o + KV8_BLOCK - 1) / KV8_BLOCK);
+        const int row = a + first * KV8_BLOCK - o;
+        if (row / KV8_BLOCK != q || row >= a + n) return;
+    }
+    const int slot = p.seq_slot[s];
+    const int b0 = start / KV8_BLOCK, last = (after - 1) / KV8_BLOCK;
+    // The open block's place holds the first block's earlier tokens until they have been read: where the step also leaves an
+    // open block behind, one warp does both, in that order.
+    const bool both = o != 0 && last > b0 && after % KV8_BLOCK != 0;
+    int b = b0 + first;
+    if (both && b == last) return;
+    __nv_bfloat16 *open = p.open + (((long long)slot * 2 + j) * p.n_kv_heads + head) * (KV8_BLOCK * HD);
+    const __nv_bfloat16 *src = p.qkv + (p.n_heads + j * p.n_kv_heads + head) * (long long)HD;
+    for (;;) {
+        const int pos0 = b * KV8_BLOCK;
+        const bool whole = pos0 + KV8_BLOCK <= after;
+        uint4 x[PIECES];
+#pragma unroll
+        for (int i = 0; i < PIECES; i++) {
+            const int t = (32 * i + lane) / LPR, c = (32 * i + lane) % LPR, pos = pos0 + t;
+            if (pos >= start && pos < after) x[i] = *(const uint4 *)(src + (long long)(a + pos - start) * p.row + 8 * c);
+            else if (pos < start && whole) x[i] = *(const uint4 *)(open + t * HD + 8 * c);
+        }
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < PIECES; i++) {
+                const int t = (32 * i + lane) / LPR, c = (32 * i + lane) % LPR, pos = pos0 + t;
+                if (pos >= start && pos < after) *(uint4 *)(open + t * HD + 8 * c) = x[i];
+            }
+        } else if (cache_keeps(p.cache, pos0, after)) {
+            float most = 0.0f;
+            bool odd = false;  // a value that is not finite
+#pragma unroll
+            for (int i = 0; i < PIECES; i++) {
+                const __nv_bfloat162 *h = (const __nv_bfloat162 *)&x[i];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float2 f = __bfloat1622float2(h[e]);
+                    most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
+                    odd |= !(fabsf(f.x) < INFINITY) || !(fabsf(f.y) < INFINITY);
+                }
+            }
+            most = warp_max(most);
+            odd = __any_sync(0xffffffffu, odd);
+            const int page = kv8_page(p.cache, p.n_pages, slot, pos0, p.status);
+            uint8_t *dst = (j == 0 ? p.k : p.v) + cache_offset(p.cache, page, head, p.n_kv_heads, pos0, HD);
+#pragma unroll
+            for (int i = 0; i < PIECES; i++) *(uint2 *)(dst + 8 * (32 * i + lane)) = kv8_pack<FORM>(x[i], odd ? 0.0f : most);
+            if (lane == 0)
+                p.scales[(((long long)page * p.n_kv_heads + head) * 2 + j) * KV8_PAGE_BLOCKS + (pos0 % KV8_PAGE) / KV8_BLOCK] =
+                    odd ? __int_as_float(0x7fffffff) : most / kv8_top<FORM>();
+        }
+        if (!both || b != b0) return;
+        __syncwarp();  // every lane has read its pieces of the old open block
+        b = last;
+    }
+}
+
+struct Kv8Read {
+    const int *first_page;  // [n_seqs + 1]: sequence s goes to pages first_page[s] .. first_page[s + 1] - 1 of the copies
+    const int *seq_len_after, *seq_slot;
+    int n_seqs, n_kv_heads;
+    PagedCache cache;
+    const uint8_t *k, *v;
+    const float *scales;
+    const __nv_bfloat16 *open;
+    void *out_k, *out_v;
+    int n_pages, *status;
+};
+
+__device__ __forceinline__ void store8(float *dst, const float *v) {
+    *(float4 *)dst = make_float4(v[0], v[1], v[2], v[3]);
+    *(float4 *)(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16 *dst, const float *v) {
+    __nv_bfloat162 h[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) h[e] = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+    *(uint4 *)dst = *(const uint4 *)h;
+}
+
+// A warp a block of 16 tokens of one head's keys or values: 8 of them to a page and head.
+template <int HD, int FORM, typename T>
+__global__ void __launch_bounds__(256) kv8_read_kernel(Kv8Read p) {
+    constexpr int LPR = HD / 8, PIECES = Kv8Block<HD>::PIECES;
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int page_out = blockIdx.x, head = blockIdx.y, j = warp >> 2, block = warp & 3;
+    const int s = last_not_above(p.first_page, p.n_seqs, lane, [&](int first, int) { return first <= page_out; });
+    if (s < 0 || page_out >= p.first_page[s + 1]) return;
+    const int after = p.seq_len_after[s], slot = p.seq_slot[s];
+    const int pos0 = (page_out - p.first_page[s]) * KV8_PAGE + block * KV8_BLOCK;
+    T *dst = (T *)(j == 0 ? p.out_k : p.out_v) +
+             (((long long)page_out * p.n_kv_heads + head) * KV8_PAGE + block * KV8_BLOCK) * HD;
+    if (pos0 + KV8_BLOCK <= after) {
+        const int page = kv8_page(p.cache, p.n_pages, slot, pos0, p.status);
+        const uint8_t *src = (j == 0 ? p.k : p.v) + cache_offset(p.cache, page, head, p.n_kv_heads, pos0, HD);
+        const float scale = p.scales[(((long long)page * p.n_kv_heads + head) * 2 + j) * KV8_PAGE_BLOCKS + block];
+        uint2 x[PIECES];
+#pragma unroll
+        for (int i = 0; i < PIECES; i++) x[i] = *(const uint2 *)(src + 8 * (32 * i + lane));
+#pragma unroll
+        for (int i = 0; i < PIECES; i++) {
+            float v[8];
+            kv8_unpack<FORM>(x[i].x, v), kv8_unpack<FORM>(x[i].y, v + 4);
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] *= scale;
+            store8(dst + 8 * (32 * i + lane), v);
+        }
+    } else {
+        const __nv_bfloat16 *open = p.open + (((long long)slot * 2 + j) * p.n_kv_heads + head) * (KV8_BLOCK * HD);
+#pragma unroll
+        for (int i = 0; i < PIECES; i++) {
+            const int t = (32 * i + lane) / LPR;
+            uint4 x = make_uint4(0, 0, 0, 0);  // behind the sequence's last token: zeros
+            if (pos0 + t < after) x = *(const uint4 *)(open + 8 * (32 * i + lane));
+            const __nv_bfloat162 *h = (const __nv_bfloat162 *)&x;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float2 f = __bfloat1622float2(h[e]);
+                v[2 * e] = f.x, v[2 * e + 1] = f.y;
+            }
+            store8(dst + 8 * (32 * i + lane), v);
+        }
+    }
+}
+
+extern "C" int abk_kv8_write(const void *qkv, long long row, int n_rows, int n_heads, int n_kv_heads, int head_dim, int form,
+                             int n_seqs, int one_each, const int *seq_start, const int *seq_pos0, const int *seq_len_after,
+                             const int *seq_slot, const int *page_table, int table_width, int ring_pages, void *k, void *v,
+                             float *scales, void *open, int pool_pages, int *status, void *stream) {
+    if (n_rows <= 0 || n_seqs <= 0) return 0;
+    if (head_dim != 64 && head_dim != 128) ABK_REFUSE("kv8_write: head_dim %d is not 64 or 128", head_dim);
+    if (form != KV8_INT8 && form != KV8_E4M3) ABK_REFUSE("kv8_write: no 8-bit form %d", form);
+    if ((((uintptr_t)qkv | (uintptr_t)k | (uintptr_t)v | (uintptr_t)open) & 15) || (row & 7) || ((uintptr_t)scales & 3))
+        ABK_REFUSE("kv8_write: rows, pools and open blocks must be 16-byte aligned");
+    const int units = one_each ? n_seqs : n_rows / KV8_BLOCK + 2 * n_seqs + 1;
+    const int groups = (2 * n_kv_heads + KV8_WARPS - 1) / KV8_WARPS;
+    if (n_kv_heads < 1 || groups > 65535) ABK_REFUSE("kv8_write: %d kv heads", n_kv_heads);
+    Kv8Write p;
+    p.qkv = (const __nv_bfloat16 *)qkv, p.row = row, p.n_heads = n_heads, p.n_kv_heads = n_kv_heads, p.n_seqs = n_seqs;
+    p.one_each = one_each, p.seq_start = seq_start, p.seq_pos0 = seq_pos0, p.seq_len_after = seq_len_after;
+    p.seq_slot = seq_slot, p.cache.page_table = page_table, p.cache.table_width = table_width, p.cache.ring_pages = ring_pages;
+    p.cache.tokens_per_page = KV8_PAGE, p.k = (uint8_t *)k, p.v = (uint8_t *)v, p.scales = scales, p.open = (__nv_bfloat16 *)open;
+    p.n_pages = pool_pages, p.status = status;
+    const dim3 grid(units, groups), block(32 * KV8_WARPS);
+    auto go = [&](auto kernel) { abk_launch(kernel, grid, block, 0, (cudaStream_t)stream, p); };
+    if (head_dim == 64) form == KV8_INT8 ? go(kv8_write_kernel<64, KV8_INT8>) : go(kv8_write_kernel<64, KV8_E4M3>);
+    else form == KV8_INT8 ? go(kv8_write_kernel<128, KV8_INT8>) : go(kv8_write_kernel<128, KV8_E4M3>);
+    return ABK_LAUNCH_RESULT();
+}
+
+extern "C" int abk_kv8_read(const void *k, const void *v, const float *scales, const void *open, int n_kv_heads, int head_dim,
+                            int form, const int *page_table, int table_width, int n_seqs, const int *seq_len_after,
+                            const int *seq_slot, const int *first_page, int n_pages, void *out_k, void *out_v, int out_dtype,
+                            int pool_pages, int *status, void *stream) {
+    if (n_pages <= 0 || n_seqs <= 0) return 0;
+    if (head_dim != 64 && head_dim != 128) ABK_REFUSE("kv8_read: head_dim %d is not 64 or 128", head_dim);
+    if (form != KV8_INT8 && form != KV8_E4M3) ABK_REFUSE("kv8_read: no 8-bit form %d", form);
+    if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)open | (uintptr_t)out_k | (uintptr_t)out_v) & 15)
+        ABK_REFUSE("kv8_read: pools, open blocks and copies must be 16-byte aligned");
+    if (n_kv_heads < 1 || n_kv_heads > 65535) ABK_REFUSE("kv8_read: %d kv heads", n_kv_heads);
+    Kv8Read p;
+    p.first_page = first_page, p.seq_len_after = seq_len_after, p.seq_slot = seq_slot, p.n_seqs = n_seqs, p.n_kv_heads = n_kv_heads;
+    p.cache.page_table = page_table, p.cache.table_width = table_width, p.cache.ring_pages = 0, p.cache.tokens_per_page = KV8_PAGE;
+    p.k = (const uint8_t *)k, p.v = (const uint8_t *)v, p.scales = scales, p.open = (const __nv_bfloat16 *)open;
+    p.out_k = out_k, p.out_v = out_v, p.n_pages = pool_pages, p.status = status;
+    const dim3 grid(n_pages, n_kv_heads), block(256);
+    auto go = [&](auto kernel) { abk_launch(kernel, grid, block, 0, (cudaStream_t)stream, p); };
+    auto by_form = [&](auto hd) {
+        constexpr int HD = decltype(hd)::value;
+        if (out_dtype == ABK_F32) form == KV8_INT8 ? go(kv8_read_kernel<HD, KV8_INT8, float>) : go(kv8_read_kernel<HD, KV8_E4M3, float>);
+        else form == KV8_INT8 ? go(kv8_read_kernel<HD, KV8_INT8, __nv_bfloat16>) : go(kv8_read_kernel<HD, KV8_E4M3, __nv_bfloat16>);
+    };
+    if (head_dim == 64) by_form(std::integral_constant<int, 64>());
+    else by_form(std::integral_constant<int, 128>());
+    return ABK_LAUNCH_RESULT();
+}

@@ -492,6 +492,140 @@ def sample_all(logits, temperature, rng_state, out, n_rows=None, rng_index=None)
                                    _p(rng_state), _p(rng_index), _p(out), _p(sums), _stream()), "sample_all", kernels=2)
 
 
+# ------------------------------------------------------------------ log probabilities (csrc/logprobs.cu)
+def _here(what, *tensors):
+    """The tensors are on the current device, whose stream the kernel goes to."""
+    _need_cuda(*tensors)
+    device = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{device}")
+
+
+LOGPROBS_MAX_TOP = 64
+
+
+def token_logprobs(logits, tokens, logprob, entropy=None, top_ids=None, top_logprobs=None, n_rows=None):
+    """logprob[r] = log softmax(logits[r])[tokens[r]] of the first n_rows rows (default: all), entropy[r] (if given) the entropy
+    of the row's distribution, and the most likely tokens: top_ids int32 [rows, k] and top_logprobs float32 [rows, k], k up to 64,
+    the larger logit first and the lower index first among equals (the order of src/main.c:43-48).
+
+    logits float32 or bfloat16 [rows, vocab], any row stride; tokens int32 [rows]; logprob and entropy float32 [rows]. A logit of
+    -inf is a token that cannot come (log probability -inf). A row with a NaN or +inf, or with nothing but -inf, is no
+    distribution: NaN, and tokens -1. A token outside the vocabulary (-1: no token given) has the log probability NaN."""
+    _here("token_logprobs", logits, tokens, logprob, entropy, top_ids, top_logprobs)
+    lib = load_module("logprobs")
+    n = logits.shape[0] if n_rows is None else n_rows
+    assert logits.dim() == 2 and 0 <= n <= logits.shape[0] and (logits.stride(1) == 1 or logits.shape[1] == 1)
+    assert tokens.dtype == torch.int32 and tokens.is_contiguous() and tokens.numel() >= n
+    for t in (logprob, entropy):
+        assert t is None or (t.dtype == torch.float32 and t.is_contiguous() and t.numel() >= n)
+    top = 0
+    if top_ids is not None or top_logprobs is not None:
+        assert top_ids is not None and top_logprobs is not None, "the most likely tokens come with their log probabilities"
+        top = top_ids.shape[1]
+        assert top_ids.dtype == torch.int32 and top_logprobs.dtype == torch.float32 and top_ids.shape == top_logprobs.shape
+        assert top_ids.is_contiguous() and top_logprobs.is_contiguous() and top_ids.shape[0] >= n
+    fn = _typed(lib.abk_token_logprobs, "piliipppippp")
+    _check(lib, fn(logits.data_ptr(), _dt(logits), logits.stride(0), n, logits.shape[1], tokens.data_ptr(), logprob.data_ptr(),
+                   _at(entropy), top, _at(top_ids), _at(top_logprobs), _raw_stream()), "token_logprobs")
+
+
+def gemm_tc_logprobs_takes(x, w):
+    """Whether gemm_tc_logprobs takes these rows and this output matrix (else the logits go through token_logprobs)."""
+    return (x.dtype == torch.bfloat16 and w.dtype == torch.bfloat16 and w.shape[1] % 8 == 0 and x.stride(1) == 1 and w.stride(1) == 1
+            and x.stride(0) % 8 == 0 and w.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0 and w.data_ptr() % 16 == 0)
+
+
+def gemm_tc_logprobs(x, w, tokens, logprob, entropy, ws, m=None):
+    """token_logprobs of the logits x[:m] . w^T (float32 sums of bfloat16 products), which are never stored: logprob[r] of tokens[r]
+    and entropy[r] (or None), float32. ws: a Workspace for the parts of the sums. A logit that is not finite makes its row NaN."""
+    _here("gemm_tc_logprobs", x, w, tokens, logprob, entropy)
+    m = x.shape[0] if m is None else m
+    (n, k), rows = w.shape, 512
+    assert x.dim() == 2 and x.shape[1] == k and 0 <= m <= x.shape[0]
+    if not gemm_tc_logprobs_takes(x, w):
+        raise KernelRefused("gemm_tc_logprobs: bfloat16 rows of a multiple of 8, 16-byte aligned")
+    logits = ws.get("logprobs_logits", (rows, n), torch.float32)
+    for lo in range(0, m, rows):
+        hi = min(m, lo + rows)
+        gemm_tc(x[lo:hi], w, logits[:hi - lo])
+        token_logprobs(logits[:hi - lo], tokens[lo:hi], logprob[lo:hi], entropy=None if entropy is None else entropy[lo:hi])
+
+
+# ------------------------------------------------------------------ keys and values in 8 bits (csrc/kv8.cu, csrc/attention_kv8.cu)
+KV8_FORMS = {"int8": 0, "e4m3": 1}
+
+
+def _kv8_fits(what, batch, cache, n_kv_heads=None, head_dim=None):
+    """The step's sequences have their slots and their positions their places in the cache."""
+    if n_kv_heads is not None and (cache.k.shape[1] != n_kv_heads or cache.k.shape[3] != head_dim):
+        raise KernelRefused(f"{what}: the cache holds {cache.k.shape[1]} kv heads of {cache.k.shape[3]}, not {n_kv_heads} of {head_dim}")
+    slots = cache.open.shape[0]
+    if any(not 0 <= s.slot < slots for s in batch.sequences):
+        raise KernelRefused(f"{what}: a sequence's slot is outside the cache's {slots}")
+    if cache.ring_pages == 0 and batch.max_len_after > cache.table_width * cache.tokens_per_page:
+        raise KernelRefused(f"{what}: {batch.max_len_after} tokens are more than the page table's {cache.table_width} pages hold")
+
+
+def kv8_write(qkv, n_heads, n_kv_heads, head_dim, batch, cache, row=None):
+    """The keys and values of the step's rows go into an 8-bit cache (cache.LayerKV8): blocks of 16 tokens that the step
+    completes into 8 bits with their scales, the last tokens of a sequence that do not fill a block into its open block.
+    qkv bfloat16 [rows, (n_heads + 2 n_kv_heads) head_dim], prepared (see qkv_prep); what a sequence holds before the
+    step (batch.seq_pos0 tokens) must be in the cache. The same step a second time is the same step only for single tokens, and where
+    no sequence both completes a block it had begun and begins another."""
+    _here("kv8_write", qkv, cache.k, batch.seq_slot)
+    lib = load_module("kv8")
+    heads_size = (n_heads + 2 * n_kv_heads) * head_dim
+    row = row or heads_size
+    assert qkv.dtype == torch.bfloat16 and qkv.is_contiguous() and qkv.shape[1] == row >= heads_size and qkv.shape[0] >= batch.n_rows
+    _kv8_fits("kv8_write", batch, cache, n_kv_heads, head_dim)
+    fn = _typed(lib.abk_kv8_write, "pliiiiiiipppppiippppipp")
+    _check(lib, fn(qkv.data_ptr(), row, batch.n_rows, n_heads, n_kv_heads, head_dim, KV8_FORMS[cache.form], batch.seq_slot.numel(),
+                   1 if batch.is_decode else 0, batch.seq_start.data_ptr(), batch.seq_pos0.data_ptr(), batch.seq_len_after.data_ptr(),
+                   batch.seq_slot.data_ptr(), cache.page_table.data_ptr(), cache.table_width, cache.ring_pages, cache.k.data_ptr(),
+                   cache.v.data_ptr(), cache.scales.data_ptr(), cache.open.data_ptr(), cache.k.shape[0],
+                   kernel_status(qkv.device).data_ptr(), _raw_stream()), "kv8_write")
+
+
+def kv8_read(cache, batch, first_page, k, v):
+    """What an 8-bit cache holds of the step's sequences, behind the step, as pages: logical page i of sequence s becomes page
+    first_page[s] + i of k and v, float32 or bfloat16 [pages, kv heads, 64, head_dim], for all first_page[s + 1] - first_page[s]
+    pages of it; places behind the sequence's last token become zeros, other pages are left alone. first_page int32
+    [sequences + 1], not falling. Not for a cache under a window."""
+    _here("kv8_read", cache.k, batch.seq_slot, first_page, k, v)
+    lib = load_module("kv8")
+    n_seqs = batch.seq_slot.numel()
+    assert first_page.dtype == torch.int32 and first_page.is_contiguous() and first_page.numel() >= n_seqs + 1
+    assert k.shape == v.shape and k.dtype == v.dtype and k.is_contiguous() and v.is_contiguous() and k.shape[1:] == cache.k.shape[1:]
+    _kv8_fits("kv8_read", batch, cache)
+    if cache.ring_pages:
+        raise KernelRefused("kv8_read: a cache under a window does not hold a sequence's first tokens")
+    fn = _typed(lib.abk_kv8_read, "ppppiiipiipppippiipp")
+    _check(lib, fn(cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(), cache.open.data_ptr(), cache.k.shape[1],
+                   cache.k.shape[3], KV8_FORMS[cache.form], cache.page_table.data_ptr(), cache.table_width, n_seqs,
+                   batch.seq_len_after.data_ptr(), batch.seq_slot.data_ptr(), first_page.data_ptr(), k.shape[0], k.data_ptr(),
+                   v.data_ptr(), _dt(k), cache.k.shape[0], kernel_status(k.device).data_ptr(), _raw_stream()), "kv8_read")
+
+
+def attention_kv8(qkv, out, n_heads, n_kv_heads, head_dim, scale, window, batch, cache, ws):
+    """Causal grouped-query attention of the step's rows (src/model.c:197-211) over an 8-bit cache that holds the step's own keys
+    and values too (kv8_write comes first): each row sees the keys up to its position, within `window` of it if given. Any
+    number of new tokens a sequence; meant for one or a few (each row reads its keys itself). q is read from qkv's q columns."""
+    _here("attention_kv8", qkv, out, cache.k, batch.token_seq)
+    lib = load_module("attention_kv8")
+    n, row = batch.n_rows, (n_heads + 2 * n_kv_heads) * head_dim
+    assert qkv.dtype == torch.bfloat16 and qkv.is_contiguous() and qkv.shape[1] == row and qkv.shape[0] >= n
+    assert out.dtype == torch.bfloat16 and out.is_contiguous() and out.shape[1] == n_heads * head_dim and out.shape[0] >= n
+    _kv8_fits("attention_kv8", batch, cache, n_kv_heads, head_dim)
+    fn = _typed(lib.abk_attention_kv8, "plpiiiiifipppppppppiiipp")
+    _check(lib, fn(qkv.data_ptr(), row, out.data_ptr(), n, n_heads, n_kv_heads, head_dim, KV8_FORMS[cache.form], scale, window or 0,
+                   batch.token_seq.data_ptr(), batch.token_pos.data_ptr(), batch.seq_slot.data_ptr(), batch.seq_len_after.data_ptr(),
+                   cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(), cache.open.data_ptr(), cache.page_table.data_ptr(),
+                   cache.table_width, cache.ring_pages, cache.k.shape[0], kernel_status(qkv.device).data_ptr(), _raw_stream()),
+           "attention_kv8")
+
+
 def attention(qkv, out, n_heads, n_kv_heads, head_dim, scale, window, batch, cache, from_step=False, ws=None, lists=None,
               prepare=None, v_dim=None, keep_first=0, sink=None, exact_weights=False, row=None, chunk=None, softcap=None,
               gate=None):
