@@ -71,6 +71,31 @@ static int bf16_rows_of_128_bytes(const void *ptr, long long rows, long long col
     return 0;
 }
 
+// A map over bytes as rows of 128: boxes of box_rows rows, 128-byte swizzle. 0 on success.
+static int bytes_in_rows_of_128(const void *ptr, long long rows, int box_rows, CUtensorMap *out) {
+    static std::unordered_map<Key, CUtensorMap, KeyHash> cache;
+    static std::mutex lock;
+    const Key key{ptr, rows, 128, 128, box_rows};
+    std::lock_guard<std::mutex> guard(lock);
+    auto it = cache.find(key);
+    if (it != cache.end()) {
+        *out = it->second;
+        return 0;
+    }
+    EncodeTiled enc = encode_tiled();
+    if (!enc) ABK_REFUSE("the driver gives no cuTensorMapEncodeTiled");
+    if (((uintptr_t)ptr & 15) || rows < 1 || rows > 0x7fffffffll) ABK_REFUSE("a TMA operand must be 16-byte aligned, of 1 to 2^31 - 1 rows of 128 bytes");
+    cuuint64_t dims[2] = {128, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {128};
+    cuuint32_t box[2] = {128, (cuuint32_t)box_rows}, elem[2] = {1, 1};
+    CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void *)ptr, dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) ABK_REFUSE("cuTensorMapEncodeTiled failed with %d", (int)r);
+    if (cache.size() > 4096) cache.clear();
+    cache[key] = *out;
+    return 0;
+}
+
 // A map over the heads of the rows of a step: bfloat16 [rows][heads][size], heads side by side (size elements apart), rows
 // `pitch` elements apart. Boxes of [box_rows, 1 head, 64] elements (128 bytes a row), 128-byte swizzle; what lies outside a
 // head or beyond the last row is zeros.
