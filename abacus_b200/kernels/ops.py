@@ -618,15 +618,14 @@ def attention_kv8(qkv, out, n_heads, n_kv_heads, head_dim, scale, window, batch,
     assert qkv.dtype == torch.bfloat16 and qkv.is_contiguous() and qkv.shape[1] == row and qkv.shape[0] >= n
     assert out.dtype == torch.bfloat16 and out.is_contiguous() and out.shape[1] == n_heads * head_dim and out.shape[0] >= n
     _kv8_fits("attention_kv8", batch, cache, n_kv_heads, head_dim)
-    max_positions = getattr(batch, "position_bound", None) or batch.max_len_after
-    if batch.max_len_after > max_positions:
-        raise KernelError(f"a row at position {batch.max_len_after - 1} is beyond the bound {max_positions}")
-    fn = _typed(lib.abk_attention_kv8, "plpiiiiifipppppppppiiiipp")
+    lib.abk_attention_kv8_part_floats.restype = ctypes.c_longlong
+    parts = ws.get("attention_kv8_parts", (lib.abk_attention_kv8_part_floats(n_heads, n_kv_heads, head_dim),), torch.float32)
+    fn = _typed(lib.abk_attention_kv8, "plpiiiiifipppppppppiiiplpp")
     _check(lib, fn(qkv.data_ptr(), row, out.data_ptr(), n, n_heads, n_kv_heads, head_dim, KV8_FORMS[cache.form], scale, window or 0,
                    batch.token_seq.data_ptr(), batch.token_pos.data_ptr(), batch.seq_slot.data_ptr(), batch.seq_len_after.data_ptr(),
                    cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(), cache.open.data_ptr(), cache.page_table.data_ptr(),
-                   cache.table_width, cache.ring_pages, cache.k.shape[0], max_positions, kernel_status(qkv.device).data_ptr(), _raw_stream()),
-           "attention_kv8")
+                   cache.table_width, cache.ring_pages, cache.k.shape[0], parts.data_ptr(), parts.numel(), kernel_status(qkv.device).data_ptr(),
+                   _raw_stream()), "attention_kv8", kernels=2 * -(-n // 512))
 
 
 def attention(qkv, out, n_heads, n_kv_heads, head_dim, scale, window, batch, cache, from_step=False, ws=None, lists=None,
