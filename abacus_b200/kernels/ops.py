@@ -495,8 +495,10 @@ def sample_all(logits, temperature, rng_state, out, n_rows=None, rng_index=None)
 # ------------------------------------------------------------------ log probabilities (csrc/logprobs.cu)
 def _here(what, *tensors):
     """The tensors are on the current device, whose stream the kernel goes to."""
-    _need_cuda(*tensors)
-    device = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and not t.is_cuda:
+            _need_cuda(t)
+    device = torch._C._cuda_getDevice()
     for t in tensors:
         if t is not None and t.get_device() != device:
             raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{device}")
