@@ -6,31 +6,27 @@
 // with nothing but -inf, is no distribution: its numbers are NaN and its tokens -1. A token outside the vocabulary has the log
 // probability NaN.
 //
-// A row is read once: a cluster of up to 8 CTAs takes it, a slice each, which stays in the CTA's shared memory as it came
-// (what does not fit there is read a second time). Every CTA finds its slice's maximum, then in one walk over shared memory the
-// two sums and the candidates for the most likely tokens, and the cluster folds the CTAs' numbers through distributed shared memory.
-// l is kept without its maxima's ones, l = n + l', n the number of maxima: log l = log(n + l') is log1p(l' + n - 1) to all its
-// digits where one token has nearly all of the weight.
-//
-// The most likely k of a slice: at least k elements reach the smallest of the warps' ceil(k / warps)-th largest thread maxima, so
-// what reaches it is collected (some tens of elements) and each is ranked by counting those before it. Where more reach it
-// than there is room for (ties; a slice that is nearly all -inf), the k-th largest is found digit by digit of the ordered bits, and of
-// its equals the first are taken. CTA 0 ranks the slices' k the same way.
+// A row is read once, by a CTA or, where there are few rows, by a cluster of up to 8 CTAs, a slice each. Every thread keeps a
+// running maximum and the two sums over its elements, 16 at a time; nothing in the walk waits for another warp. The most
+// likely tokens: every warp keeps its best 32 (or 64) so far sorted across its lanes. An element is looked at only where it reaches a
+// bound that at least k elements of the slice reach, the smallest of the warps' ceil(k / 8)-th best, which the warps leave in
+// shared memory as they go (a bound that is out of date is only lower). A warp meets its elements by rising index, so among
+// equals the one it has comes before the one it meets. Sorted lists are merged by counting: an element's place is its place in
+// its own list and, by halving, the elements of the other lists before it; the warps' first, then the cluster's.
 #define ABK_DEFINE_ERROR
 #include "common.cuh"
 #include "tc_common.cuh"
 
 #define LOGPROBS_MAX_TOP 64
-#define LOGPROBS_THREADS 512
-#define LOGPROBS_WARPS (LOGPROBS_THREADS / 32)
-#define LOGPROBS_CANDIDATES 512
+#define LOGPROBS_WARPS 8
+#define LOGPROBS_THREADS (32 * LOGPROBS_WARPS)
 #define LOGPROBS_MAX_SPLITS 8
-#define LOGPROBS_KEPT_BYTES (96 * 1024)  // of a slice in shared memory, so that an SM holds two CTAs
+#define LOGPROBS_FAR (-1e30f)  // a distance below the maximum at which nothing is left, and a finite one
 
 struct LogProbs {
     const void *logits;
     long long stride;
-    int vocab, top, slice, kept;  // elements of a CTA's slice (a multiple of 16 bytes), and how many of them are kept
+    int vocab, top, slice;  // elements of a CTA's slice (whole pieces of 16 bytes)
     const int *tokens;
     float *logprob, *entropy;
     int *top_ids;
@@ -41,244 +37,270 @@ struct __align__(8) Ranked {
     int i;
 };
 __device__ __forceinline__ bool ranks_before(Ranked a, Ranked b) { return a.v > b.v || (a.v == b.v && a.i < b.i); }
-// The bits of x in the order of the numbers (-0 as 0; no NaN).
-__device__ __forceinline__ uint32_t ordered(float x) {
-    const uint32_t b = __float_as_uint(x + 0.0f);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
-}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-struct __align__(16) SliceSums {
-    float m, l, t;  // maximum; sum of e^(x - m) without the maxima; sum of e^(x - m) (x - m)
-    int ties;       // how many maxima
+// Maximum m; l = sum e^(x - m) and t = sum (x - m) e^(x - m). Without elements m is the lowest number and l is zero.
+struct __align__(16) RowSums {
+    float m, l, t, pad;
 };
+__device__ __forceinline__ RowSums joined(RowSums a, RowSums b) {
+    RowSums r;
+    r.m = fmaxf(a.m, b.m), r.pad = 0.0f;
+    const float da = fmaxf(a.m - r.m, LOGPROBS_FAR), db = fmaxf(b.m - r.m, LOGPROBS_FAR);
+    const float ea = ex2(da * 1.4426950408889634f), eb = ex2(db * 1.4426950408889634f);
+    r.l = fmaf(a.l, ea, b.l * eb);
+    r.t = fmaf(fmaf(a.l, da, a.t), ea, fmaf(b.l, db, b.t) * eb);
+    return r;
+}
+// The next float32 number above x (which is not NaN).
+__device__ __forceinline__ float next_up(float x) {
+    if (x == 0.0f) return __int_as_float(1);
+    return __int_as_float(__float_as_int(x) + (x > 0.0f ? 1 : -1));
+}
 
 // Elements of a 16-byte piece.
 template <typename T> struct Piece;
 template <> struct Piece<float> {
     static constexpr int N = 4;
-    __device__ static void floats(uint4 w, float *v) {
+    __device__ __forceinline__ static void floats(uint4 w, float *v) {
         v[0] = __uint_as_float(w.x), v[1] = __uint_as_float(w.y), v[2] = __uint_as_float(w.z), v[3] = __uint_as_float(w.w);
     }
+    __device__ __forceinline__ static uint4 nothing() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
 };
 template <> struct Piece<__nv_bfloat16> {
     static constexpr int N = 8;
-    __device__ static void floats(uint4 w, float *v) {
+    __device__ __forceinline__ static void floats(uint4 w, float *v) {
         const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int e = 0; e < 4; e++) v[2 * e] = __uint_as_float(u[e] << 16), v[2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u);
     }
+    __device__ __forceinline__ static uint4 nothing() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
 };
 
-// The k best of cand[0..n), n <= LOGPROBS_CANDIDATES, in order, into best[0..k): each is counted past by all that come before it.
-__device__ __forceinline__ void rank_candidates(const Ranked *cand, int n, int k, Ranked *best) {
-    for (int j = threadIdx.x; j < n; j += LOGPROBS_THREADS) {
-        const Ranked c = cand[j];
-        int rank = 0;
-        for (int i = 0; i < n; i++) rank += ranks_before(cand[i], c);
-        if (rank < k) best[rank] = c;
+// A warp's best so far, the best first: element 32 r + lane in v[r], i[r]; NaN where there is none yet.
+template <int R> struct Best {
+    float v[R > 0 ? R : 1];
+    int i[R > 0 ? R : 1];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int r = 0; r < R; r++) v[r] = __int_as_float(0x7fffffff), i[r] = 0x7fffffff;
+    }
+    __device__ __forceinline__ float at(int n) const {
+        float x = __shfl_sync(0xffffffffu, v[0], n & 31);
+        if (R > 1) {
+            const float y = __shfl_sync(0xffffffffu, v[R - 1], n & 31);
+            x = n < 32 ? x : y;
+        }
+        return x;
+    }
+    // x at index xi, which is larger than that of every equal element that is here
+    __device__ __forceinline__ void insert(float x, int xi, int lane) {
+        int pos = 0;
+#pragma unroll
+        for (int r = 0; r < R; r++) pos += __popc(__ballot_sync(0xffffffffu, v[r] >= x));
+#pragma unroll
+        for (int r = R - 1; r >= 0; r--) {
+            float up = __shfl_up_sync(0xffffffffu, v[r], 1);
+            int up_i = __shfl_up_sync(0xffffffffu, i[r], 1);
+            if (r > 0) {
+                const float over = __shfl_sync(0xffffffffu, v[0], 31);
+                const int over_i = __shfl_sync(0xffffffffu, i[0], 31);
+                if (lane == 0) up = over, up_i = over_i;
+            }
+            const int n = 32 * r + lane;
+            if (n > pos) v[r] = up, i[r] = up_i;
+            else if (n == pos) v[r] = x, i[r] = xi;
+        }
+    }
+};
+
+// Merges sorted lists in shared memory: list c at lists + c * LOGPROBS_MAX_TOP has counts(c) elements; f(rank, element) for the first k.
+template <typename Counts, typename F>
+__device__ __forceinline__ void merge_lists(const Ranked *lists, int n_lists, int k, Counts counts, F f) {
+    for (int j = threadIdx.x; j < n_lists * k; j += LOGPROBS_THREADS) {
+        const int mine = j / k, at = j - mine * k;
+        if (at >= counts(mine)) continue;
+        const Ranked c = lists[mine * LOGPROBS_MAX_TOP + at];
+        int rank = at;
+        for (int o = 0; o < n_lists && rank < k; o++) {
+            if (o == mine) continue;
+            int lo = 0, hi = counts(o);
+            while (lo < hi) {
+                const int mid = (lo + hi) / 2;
+                if (ranks_before(lists[o * LOGPROBS_MAX_TOP + mid], c)) lo = mid + 1;
+                else hi = mid;
+            }
+            rank += lo;
+        }
+        if (rank < k) f(rank, c);
     }
 }
 
-template <typename T>
+template <typename T, int R>
 __global__ void __launch_bounds__(LOGPROBS_THREADS) logprobs_kernel(LogProbs p) {
-    constexpr int N = Piece<T>::N;
-    extern __shared__ __align__(16) uint8_t kept_raw[];
-    T *kept = (T *)kept_raw;
-    __shared__ float scratch[33], bound_s[LOGPROBS_WARPS];
-    __shared__ Ranked cand[LOGPROBS_CANDIDATES], best[LOGPROBS_MAX_TOP];
-    __shared__ SliceSums sums;
-    __shared__ int count, digits[256], wanted, prefix;
+    constexpr int N = Piece<T>::N, U = 16 / N;  // elements of a piece, pieces a thread takes at a time
+    __shared__ Ranked lists[(R ? LOGPROBS_WARPS : 1) * LOGPROBS_MAX_TOP], best[R ? LOGPROBS_MAX_TOP : 1];
+    __shared__ volatile float bounds[LOGPROBS_WARPS];
+    __shared__ RowSums warp_sums[LOGPROBS_WARPS], cta_sums;
+    __shared__ int have[LOGPROBS_WARPS], cta_have;
     const int split = (int)tc::cluster_rank(), splits = (int)tc::cluster_size(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int row = blockIdx.y;
+    if (threadIdx.x < LOGPROBS_WARPS) bounds[threadIdx.x] = -INFINITY;
     pdl_wait();
+    __syncthreads();
     const T *x = (const T *)p.logits + row * p.stride;
-    // slices start on a 16-byte boundary of memory: slice 0 also takes the elements before the first one
-    const int skew = (int)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(T)), ahead = min(skew, p.vocab);
+    // slices start on a 16-byte boundary of memory; slice 0 also takes the elements before the first one
+    const int ahead = min((int)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(T)), p.vocab);
     const int lo = split == 0 ? 0 : min(p.vocab, ahead + split * p.slice), hi = split == splits - 1 ? p.vocab : min(p.vocab, ahead + (split + 1) * p.slice);
-    const int pieces = (hi - max(lo, ahead)) / N, body = max(lo, ahead), tail = body + pieces * N;  // [lo, body) and [tail, hi) are less than a piece
+    const int body = max(lo, ahead), pieces = (hi - body) / N, tail = body + pieces * N;  // [lo, body) and [tail, hi): less than a piece each
     const uint4 *src = (const uint4 *)(x + body);
-    const int kept_pieces = min(pieces, p.kept / N);
-    float most = -INFINITY;
-    bool odd = false;  // a NaN or +inf
-    // every element once: into shared memory, the maximum on the way
-    {
-        constexpr int U = 4;
-        for (int j = threadIdx.x; j < pieces; j += U * LOGPROBS_THREADS) {
-            uint4 w[U];
-#pragma unroll
-            for (int i = 0; i < U; i++)
-                if (j + i * LOGPROBS_THREADS < pieces) w[i] = __ldg(src + j + i * LOGPROBS_THREADS);
-#pragma unroll
-            for (int i = 0; i < U; i++) {
-                const int at = j + i * LOGPROBS_THREADS;
-                if (at < pieces) {
-                    if (at < kept_pieces) ((uint4 *)kept)[at] = w[i];
-                    float v[N];
-                    Piece<T>::floats(w[i], v);
-#pragma unroll
-                    for (int e = 0; e < N; e++) most = fmaxf(most, v[e]), odd |= !(v[e] < INFINITY);
-                }
-            }
+    float m = -3.402823466e38f, l = 0.0f, t = 0.0f;
+    Best<R> top;
+    top.clear();
+    float cut = -INFINITY;  // what an element has to reach to be looked at
+    const int jth = (p.top + LOGPROBS_WARPS - 1) / LOGPROBS_WARPS - 1;
+    auto sum = [&](const float *v, int n, float most) {
+        if (most > m) {
+            const float d = fmaxf(m - most, LOGPROBS_FAR), e = ex2(d * 1.4426950408889634f);
+            t = e * fmaf(l, d, t), l *= e, m = most;
         }
-    }
-    const int loose = (body - lo) + (hi - tail);  // elements outside the pieces: at most 14
-    float mine_loose = -INFINITY;
-    int loose_at = 0;
-    if (threadIdx.x < loose) {
-        loose_at = threadIdx.x < body - lo ? lo + threadIdx.x : tail + threadIdx.x - (body - lo);
-        mine_loose = to_float(x[loose_at]);
-        most = fmaxf(most, mine_loose), odd |= !(mine_loose < INFINITY);
-    }
-    // f(value, index) for every element of the slice, the thread's own as above
-    auto each = [&](auto f) {
-        for (int j = threadIdx.x; j < pieces; j += LOGPROBS_THREADS) {
-            const uint4 w = j < kept_pieces ? ((const uint4 *)kept)[j] : __ldg(src + j);
-            float v[N];
-            Piece<T>::floats(w, v);
 #pragma unroll
-            for (int e = 0; e < N; e++) f(v[e], body + j * N + e);
+        for (int e = 0; e < n; e++) {
+            const float d = v[e] - m, w = ex2(d * 1.4426950408889634f);
+            l += w, t = fmaf(w, fmaxf(d, LOGPROBS_FAR), t);
         }
-        if (threadIdx.x < loose) f(mine_loose, loose_at);
     };
-    if (threadIdx.x == 0) count = 0;
-    const int k = min(p.top, hi - lo);  // of this slice
-    if (k > 0) {  // this warp's ceil(k / warps)-th largest thread maximum
-        float v = most, m = -INFINITY;
-        for (int r = 0; r < (k + LOGPROBS_WARPS - 1) / LOGPROBS_WARPS; r++) {
-            m = warp_max(v);
-            const unsigned holders = __ballot_sync(0xffffffffu, v == m);
-            if (lane == __ffs(holders) - 1) v = -INFINITY;  // one of them is taken out
+    auto meet = [&](float v, int at) {  // (the whole warp with the same element)
+        if (!(v >= cut)) return;
+        top.insert(v, at, lane);
+        const float last = top.at(p.top - 1), mine = top.at(jth);
+        cut = fmaxf(cut, last == last ? next_up(last) : -INFINITY);
+        if (lane == 0 && mine > bounds[warp]) bounds[warp] = mine;
+    };
+    auto loose = [&](int from, int to) {  // elements outside the pieces, a lane each
+        const int at = from + lane;
+        const float v = at < to ? to_float(x[at]) : -INFINITY;
+        if (at < to) sum(&v, 1, v);
+        if (R)
+            for (int i = 0; i < to - from; i++) meet(__shfl_sync(0xffffffffu, v, i), from + i);
+    };
+    auto load = [&](int j0, float *v) {
+        uint4 w[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) w[u] = j0 + 32 * u + lane < pieces ? __ldcs(src + j0 + 32 * u + lane) : Piece<T>::nothing();
+#pragma unroll
+        for (int u = 0; u < U; u++) Piece<T>::floats(w[u], v + u * N);
+        float most = v[0];
+#pragma unroll
+        for (int e = 1; e < 16; e++) most = fmaxf(most, v[e]);
+        return most;
+    };
+    float v[16], most = load(warp * U * 32, v);
+    if (R) {  // the first bounds: ceil(k / 8) lanes of every warp have an element that reaches their warp's
+        float rest = most, b = -INFINITY;
+        for (int r = 0; r <= jth; r++) {
+            b = warp_max(rest);
+            const unsigned holders = __ballot_sync(0xffffffffu, rest == b);
+            if (lane == __ffs(holders) - 1) rest = -INFINITY;  // one of them is taken out
         }
-        if (lane == 0) bound_s[warp] = m;
-    }
-    const float m = block_max(most, scratch);
-    odd = __syncthreads_or(odd);
-    float bound = INFINITY;
-    if (k > 0)
-        for (int w = 0; w < LOGPROBS_WARPS; w++) bound = fminf(bound, bound_s[w]);
-    float l = 0.0f, t = 0.0f;
-    int ties = 0;
-    const float m2 = m == -INFINITY ? 0.0f : m;
-    each([&](float v, int at) {
-        const float d = v - m2, e = ex2(d * 1.4426950408889634f);
-        ties += v == m, l += v == m ? 0.0f : e, t = fmaf(e, fmaxf(d, -1e30f), t);
-        if (v >= bound) {
-            const int c = atomicAdd(&count, 1);
-            if (c < LOGPROBS_CANDIDATES) cand[c] = {v, at};
-        }
-    });
-    l = block_sum(l, scratch), t = block_sum(t, scratch);
-    const float n_ties = block_sum((float)ties, scratch);
-    if (threadIdx.x == 0) sums = {odd ? NAN : m, l, t, (int)n_ties};
-    if (k > 0) {
-        if (count > LOGPROBS_CANDIDATES) {  // (the same for the whole CTA) the k-th largest, eight bits of the ordered numbers at a time
-            if (threadIdx.x == 0) wanted = k, prefix = 0;
-            for (int shift = 24; shift >= 0; shift -= 8) {
-                for (int i = threadIdx.x; i < 256; i += LOGPROBS_THREADS) digits[i] = 0;
-                __syncthreads();
-                const uint32_t above = shift == 24 ? 0 : 0xffffffffu << (shift + 8), have = (uint32_t)prefix;
-                each([&](float v, int) {
-                    const uint32_t b = ordered(v);
-                    if ((b & above) == have) atomicAdd(&digits[b >> shift & 255], 1);
-                });
-                __syncthreads();
-                if (threadIdx.x == 0) {
-                    int left = wanted, d = 255;
-                    while (d > 0 && digits[d] < left) left -= digits[d], d--;
-                    wanted = left, prefix = (int)(have | (uint32_t)d << shift);
-                }
-                __syncthreads();
-            }
-            // all above it, and of its equals the `wanted` first ones
-            const uint32_t kth = (uint32_t)prefix;
-            if (threadIdx.x == 0) count = 0;
-            __syncthreads();
-            each([&](float v, int at) {
-                if (ordered(v) > kth) cand[atomicAdd(&count, 1)] = {v, at};
-            });
-            __syncthreads();
-            int found = 0;
-            for (int j0 = lo; j0 < hi && found < wanted; j0 += LOGPROBS_THREADS) {
-                const int j = j0 + threadIdx.x;
-                const float v = j < hi ? to_float(x[j]) : 0.0f;
-                const bool same = j < hi && ordered(v) == kth;
-                const unsigned votes = __ballot_sync(0xffffffffu, same);
-                if (lane == 0) digits[warp] = __popc(votes);
-                __syncthreads();
-                int before = found, all = 0;
-                for (int w = 0; w < LOGPROBS_WARPS; w++) before += w < warp ? digits[w] : 0, all += digits[w];
-                before += __popc(votes & ((1u << lane) - 1));
-                if (same && before < wanted) cand[k - wanted + before] = {v, j};
-                found += all;
-                __syncthreads();
-            }
-            if (threadIdx.x == 0) count = k;
-        }
+        if (lane == 0) bounds[warp] = b;
         __syncthreads();
-        rank_candidates(cand, min(count, LOGPROBS_CANDIDATES), k, best);
+    }
+    if (warp == 0) loose(lo, body);
+    for (int j0 = warp * U * 32; j0 < pieces; j0 += LOGPROBS_THREADS * U) {
+        if (R) {
+            float b = bounds[lane & (LOGPROBS_WARPS - 1)];
+#pragma unroll
+            for (int o = LOGPROBS_WARPS / 2; o > 0; o >>= 1) b = fminf(b, __shfl_xor_sync(0xffffffffu, b, o));
+            cut = fmaxf(cut, b);
+            if (__any_sync(0xffffffffu, most >= cut)) {
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int at = j0 + 32 * u + lane;
+                    float of_piece = v[u * N];
+#pragma unroll
+                    for (int e = 1; e < N; e++) of_piece = fmaxf(of_piece, v[u * N + e]);
+                    for (unsigned hits = __ballot_sync(0xffffffffu, of_piece >= cut && at < pieces); hits; hits &= hits - 1) {
+                        const int from = __ffs(hits) - 1;
+#pragma unroll
+                        for (int e = 0; e < N; e++) meet(__shfl_sync(0xffffffffu, v[u * N + e], from), body + (j0 + 32 * u + from) * N + e);
+                    }
+                }
+            }
+        }
+        sum(v, 16, most);
+        most = load(j0 + LOGPROBS_THREADS * U, v);
+    }
+    if (warp == LOGPROBS_WARPS - 1) loose(tail, hi);
+    RowSums mine = {m, l, t, 0.0f};
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        RowSums other;
+        other.m = __shfl_xor_sync(0xffffffffu, mine.m, o), other.l = __shfl_xor_sync(0xffffffffu, mine.l, o), other.t = __shfl_xor_sync(0xffffffffu, mine.t, o);
+        mine = joined(mine, other);
+    }
+    if (lane == 0) warp_sums[warp] = mine;
+    if (R) {
+        int n = 0;
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            lists[warp * LOGPROBS_MAX_TOP + 32 * r + lane] = {top.v[r], top.i[r]};
+            n += __popc(__ballot_sync(0xffffffffu, top.v[r] == top.v[r]));
+        }
+        if (lane == 0) have[warp] = min(n, p.top);
+    }
+    __syncthreads();
+    if (R) {
+        merge_lists(lists, LOGPROBS_WARPS, p.top, [&](int c) { return have[c]; }, [&](int rank, Ranked c) { best[rank] = c; });
+        if (threadIdx.x == 0) {
+            int n = 0;
+            for (int w = 0; w < LOGPROBS_WARPS; w++) n += have[w];
+            cta_have = min(n, p.top);
+        }
+    }
+    if (warp == 0) {
+        RowSums s = warp_sums[0];
+        for (int w = 1; w < LOGPROBS_WARPS; w++) s = joined(s, warp_sums[w]);
+        if (lane == 0) cta_sums = s;
     }
     if (splits > 1) tc::cluster_sync();
     else __syncthreads();
-    // the row's numbers, in every CTA that needs them
-    auto of_cta = [&](const void *at, int c) { return tc::peer_smem(tc::smem_addr(at), c); };
     if (split == 0) {
-        float mm = -INFINITY;
-        bool none = false;
-        for (int c = 0; c < splits; c++) {
-            const float4 s = tc::ld_cluster_f4(of_cta(&sums, c));
-            none |= !(s.x == s.x), mm = fmaxf(mm, s.x);
+        RowSums s = cta_sums;
+        for (int c = 1; c < splits; c++) {
+            const float4 o = tc::ld_cluster_f4(tc::peer_smem(tc::smem_addr(&cta_sums), c));
+            s = joined(s, {o.x, o.y, o.z, 0.0f});
         }
-        none |= mm == -INFINITY;
-        float ll = 0.0f, tt = 0.0f;
-        int n = 0;
-        for (int c = 0; c < splits; c++) {
-            const float4 s = tc::ld_cluster_f4(of_cta(&sums, c));
-            const int n_c = __float_as_int(s.w);
-            if (s.x == -INFINITY) continue;  // nothing in this slice can come
-            if (s.x == mm) {
-                ll += s.y, tt += s.z, n += n_c;
-            } else {
-                const float d = s.x - mm, e = exp2f(d * 1.4426950408889634f);
-                ll = fmaf((float)n_c + s.y, e, ll), tt = fmaf(fmaf((float)n_c + s.y, d, s.z), e, tt);
-            }
-        }
-        const float log_l = log1pf(ll + (float)(n - 1)), nan = __int_as_float(0x7fffffff);
+        const float log_l = logf(s.l), nan = __int_as_float(0x7fffffff);
+        const bool none = !(s.l > 0.0f);  // nothing can come, or a NaN, or +inf (which is one less itself)
         if (threadIdx.x == 0) {
             const int token = p.tokens[row];
-            p.logprob[row] = none || token < 0 || token >= p.vocab ? nan : to_float(x[token]) - mm - log_l;
-            if (p.entropy) p.entropy[row] = none ? nan : log_l - tt / (ll + (float)n);
+            p.logprob[row] = none || token < 0 || token >= p.vocab ? nan : to_float(x[token]) - s.m - log_l;
+            if (p.entropy) p.entropy[row] = none ? nan : log_l - s.t / s.l;
         }
-        if (p.top > 0) {
-            // the slices' best, at most 8 x 64, into cand: they are at most LOGPROBS_CANDIDATES
-            const int per = p.top;
-            int n_cand = 0;
-            __syncthreads();
-            for (int c = 0; c < splits; c++) {
-                const int c_lo = c == 0 ? 0 : min(p.vocab, ahead + c * p.slice), c_hi = c == splits - 1 ? p.vocab : min(p.vocab, ahead + (c + 1) * p.slice);
-                const int have = min(per, c_hi - c_lo);
-                for (int i = threadIdx.x; i < have; i += LOGPROBS_THREADS) {
-                    const float2 b = tc::ld_cluster_f2(of_cta(best + i, c));
-                    cand[n_cand + i] = {b.x, __float_as_int(b.y)};
+        if (R) {
+            const long long at = (long long)row * p.top;
+            auto put = [&](int rank, Ranked c) {
+                p.top_ids[at + rank] = none ? -1 : c.i, p.top_logprobs[at + rank] = none ? nan : c.v - s.m - log_l;
+            };
+            if (none) {
+                for (int j = threadIdx.x; j < p.top; j += LOGPROBS_THREADS) put(j, {0.0f, 0});
+            } else if (splits == 1) {
+                if (threadIdx.x < p.top) put(threadIdx.x, best[threadIdx.x]);
+            } else {
+                __shared__ int of_cta[LOGPROBS_MAX_SPLITS];
+                for (int j = threadIdx.x; j < splits * p.top; j += LOGPROBS_THREADS) {
+                    const int c = j / p.top, i = j - c * p.top;
+                    const float2 b = tc::ld_cluster_f2(tc::peer_smem(tc::smem_addr(best + i), c));
+                    lists[c * LOGPROBS_MAX_TOP + i] = {b.x, __float_as_int(b.y)};
                 }
-                n_cand += have;
+                if (threadIdx.x < splits) of_cta[threadIdx.x] = __float_as_int(tc::ld_cluster_f1(tc::peer_smem(tc::smem_addr(&cta_have), threadIdx.x)));
+                __syncthreads();
+                merge_lists(lists, splits, p.top, [&](int c) { return of_cta[c]; }, put);
             }
-            __syncthreads();
-            for (int j = threadIdx.x; j < n_cand; j += LOGPROBS_THREADS) {
-                const Ranked c = cand[j];
-                int rank = 0;
-                for (int i = 0; i < n_cand; i++) rank += ranks_before(cand[i], c);
-                if (rank < p.top && !none) {
-                    p.top_ids[(long long)row * p.top + rank] = c.i;
-                    p.top_logprobs[(long long)row * p.top + rank] = c.v - mm - log_l;
-                }
-            }
-            if (none)
-                for (int j = threadIdx.x; j < p.top; j += LOGPROBS_THREADS)
-                    p.top_ids[(long long)row * p.top + j] = -1, p.top_logprobs[(long long)row * p.top + j] = nan;
         }
     }
     if (splits > 1) tc::cluster_sync();  // nobody leaves while its numbers may still be read
@@ -291,26 +313,25 @@ extern "C" int abk_token_logprobs(const void *logits, int dtype, long long strid
     if (top < 0 || top > LOGPROBS_MAX_TOP || top > vocab)
         ABK_REFUSE("token_logprobs: %d most likely tokens of a vocabulary of %d (at most %d)", top, vocab, LOGPROBS_MAX_TOP);
     const int size = dtype == ABK_F32 ? 4 : 2, piece = 16 / size;
-    // slices of at least 4,096 elements, as many as a cluster holds
-    int splits = (vocab + 4095) / 4096;
-    if (splits > LOGPROBS_MAX_SPLITS) splits = LOGPROBS_MAX_SPLITS;
+    if ((uintptr_t)logits % size) ABK_REFUSE("token_logprobs: logits that are not aligned to their own size");
+    // CTAs to a row: until the GPU is full (8 to an SM), in slices of at least 4,096 elements, as many as a cluster holds
+    const int full = 8 * abk_sm_count();
+    int splits = 1;
+    while (splits < LOGPROBS_MAX_SPLITS && (long long)n_rows * splits * 2 <= full && vocab / (splits * 2) >= 4096) splits *= 2;
     LogProbs p;
     p.logits = logits, p.stride = stride, p.vocab = vocab, p.top = top, p.tokens = tokens, p.logprob = logprob, p.entropy = entropy;
     p.top_ids = top_ids, p.top_logprobs = top_logprobs;
     p.slice = (vocab + splits * piece - 1) / (splits * piece) * piece;
-    p.kept = p.slice + piece;  // (the last slice may have an element or two more than the others)
-    if (p.kept > LOGPROBS_KEPT_BYTES / size) p.kept = LOGPROBS_KEPT_BYTES / size;
-    const int smem = p.kept * size;
-    void (*kernel)(LogProbs) = dtype == ABK_F32 ? logprobs_kernel<float> : logprobs_kernel<__nv_bfloat16>;
-    const cudaError_t e = abk_allow_shared_memory((const void *)kernel, smem);
-    if (e != cudaSuccess) return (int)e;
+    void (*kernel)(LogProbs) = nullptr;
+    if (dtype == ABK_F32) kernel = top == 0 ? logprobs_kernel<float, 0> : top <= 32 ? logprobs_kernel<float, 1> : logprobs_kernel<float, 2>;
+    else kernel = top == 0 ? logprobs_kernel<__nv_bfloat16, 0> : top <= 32 ? logprobs_kernel<__nv_bfloat16, 1> : logprobs_kernel<__nv_bfloat16, 2>;
     for (int first = 0; first < n_rows; first += 32768) {  // (rows of a grid)
         LogProbs q = p;
         const int rows = n_rows - first < 32768 ? n_rows - first : 32768;
         q.logits = (const char *)logits + first * stride * size, q.tokens = tokens + first, q.logprob = logprob + first;
         q.entropy = entropy ? entropy + first : nullptr;
         q.top_ids = top ? top_ids + (long long)first * top : nullptr, q.top_logprobs = top ? top_logprobs + (long long)first * top : nullptr;
-        abk_launch_clusters(kernel, dim3(splits, rows), dim3(LOGPROBS_THREADS), smem, (cudaStream_t)stream, splits, q);
+        abk_launch_clusters(kernel, dim3(splits, rows), dim3(LOGPROBS_THREADS), 0, (cudaStream_t)stream, splits, q);
         const int rc = ABK_LAUNCH_RESULT();
         if (rc) return rc;
     }

@@ -97,6 +97,11 @@ __device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
     asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr));
     return v;
 }
+__device__ __forceinline__ float ld_cluster_f1(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+    return v;
+}
 
 // ------------------------------------------------------------------ TMA
 // Loads the box of `map` whose first element is (x, y) (x: innermost, in elements) into shared
