@@ -6,13 +6,14 @@
 // with nothing but -inf, is no distribution: its numbers are NaN and its tokens -1. A token outside the vocabulary has the log
 // probability NaN.
 //
-// A row is read once, by a CTA or, where there are few rows, by a cluster of up to 8 CTAs, a slice each. Every thread keeps a
-// running maximum and the two sums over its elements, 16 at a time; nothing in the walk waits for another warp. The most
-// likely tokens: every warp keeps its best 32 (or 64) so far sorted across its lanes. An element is looked at only where it reaches a
-// bound that at least k elements of the slice reach, the smallest of the warps' ceil(k / 8)-th best, which the warps leave in
-// shared memory as they go (a bound that is out of date is only lower). A warp meets its elements by rising index, so among
-// equals the one it has comes before the one it meets. Sorted lists are merged by counting: an element's place is its place in
-// its own list and, by halving, the elements of the other lists before it; the warps' first, then the cluster's.
+// A row is read once, by a CTA or, where there are few rows, by a cluster of up to 16 CTAs, a slice each. Every thread keeps a
+// running maximum and the two sums over its elements, 16 at a time, the next 16 on their way; nothing in the walk waits for
+// another warp. The most likely tokens: an element is noted, in the warp's own list in shared memory, only where it reaches a bound
+// that at least k elements of the slice reach: the smallest of the warps' ceil(k / 8)-th largest thread maxima, which the warps
+// leave in shared memory as they go (a bound that is out of date is only lower). A list that fills up is cut to its best k; a
+// warp meets its elements by rising index, so from then on an equal of the k-th need not be noted. At the end the elements that
+// reach the last bound, some tens, are ranked by counting those before each, and once more those of a cluster's CTAs. Elements of -inf are
+// never noted: where a row has fewer than k others, the first of them fill its places.
 #define ABK_DEFINE_ERROR
 #include "common.cuh"
 #include "tc_common.cuh"
@@ -20,7 +21,9 @@
 #define LOGPROBS_MAX_TOP 64
 #define LOGPROBS_WARPS 8
 #define LOGPROBS_THREADS (32 * LOGPROBS_WARPS)
-#define LOGPROBS_MAX_SPLITS 8
+#define LOGPROBS_MAX_SPLITS 16
+static_assert(LOGPROBS_MAX_SPLITS >= 2 * LOGPROBS_WARPS, "room for all lists");
+#define LOGPROBS_NOTED 128  // elements a warp's list has room for beside those of one piece of every lane
 #define LOGPROBS_FAR (-1e30f)  // a distance below the maximum at which nothing is left, and a finite one
 
 struct LogProbs {
@@ -41,6 +44,28 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// The largest number of a warp's lanes.
+__device__ __forceinline__ float largest_of_lanes(float v) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+// Two float32 operations at once.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(*(unsigned long long *)&r) : "l"(*(unsigned long long *)&a), "l"(*(unsigned long long *)&b));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(*(unsigned long long *)&r) : "l"(*(unsigned long long *)&a), "l"(*(unsigned long long *)&b));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(*(unsigned long long *)&r) : "l"(*(unsigned long long *)&a), "l"(*(unsigned long long *)&b), "l"(*(unsigned long long *)&c));
+    return r;
 }
 // Maximum m; l = sum e^(x - m) and t = sum (x - m) e^(x - m). Without elements m is the lowest number and l is zero.
 struct __align__(16) RowSums {
@@ -80,162 +105,153 @@ template <> struct Piece<__nv_bfloat16> {
     __device__ __forceinline__ static uint4 nothing() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
 };
 
-// A warp's best so far, the best first: element 32 r + lane in v[r], i[r]; NaN where there is none yet.
-template <int R> struct Best {
-    float v[R > 0 ? R : 1];
-    int i[R > 0 ? R : 1];
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int r = 0; r < R; r++) v[r] = __int_as_float(0x7fffffff), i[r] = 0x7fffffff;
+// The best k of the n elements noted at `list`, in order, in its first places (by way of `spare`, room for k); returns how many those
+// are. By one warp.
+__device__ __noinline__ int cut_to_best(Ranked *list, Ranked *spare, int n, int k, int lane) {
+    for (int j = lane; j < n; j += 32) {
+        const Ranked c = list[j];
+        int rank = 0;
+        for (int i = 0; i < n; i++) rank += ranks_before(list[i], c);
+        if (rank < k) spare[rank] = c;
     }
-    __device__ __forceinline__ float at(int n) const {
-        float x = __shfl_sync(0xffffffffu, v[0], n & 31);
-        if (R > 1) {
-            const float y = __shfl_sync(0xffffffffu, v[R - 1], n & 31);
-            x = n < 32 ? x : y;
-        }
-        return x;
-    }
-    // x at index xi, which is larger than that of every equal element that is here
-    __device__ __forceinline__ void insert(float x, int xi, int lane) {
-        int pos = 0;
-#pragma unroll
-        for (int r = 0; r < R; r++) pos += __popc(__ballot_sync(0xffffffffu, v[r] >= x));
-#pragma unroll
-        for (int r = R - 1; r >= 0; r--) {
-            float up = __shfl_up_sync(0xffffffffu, v[r], 1);
-            int up_i = __shfl_up_sync(0xffffffffu, i[r], 1);
-            if (r > 0) {
-                const float over = __shfl_sync(0xffffffffu, v[0], 31);
-                const int over_i = __shfl_sync(0xffffffffu, i[0], 31);
-                if (lane == 0) up = over, up_i = over_i;
-            }
-            const int n = 32 * r + lane;
-            if (n > pos) v[r] = up, i[r] = up_i;
-            else if (n == pos) v[r] = x, i[r] = xi;
-        }
-    }
-};
-
-// Merges sorted lists in shared memory: list c at lists + c * LOGPROBS_MAX_TOP has counts(c) elements; f(rank, element) for the first k.
-template <typename Counts, typename F>
-__device__ __forceinline__ void merge_lists(const Ranked *lists, int n_lists, int k, Counts counts, F f) {
-    for (int j = threadIdx.x; j < n_lists * k; j += LOGPROBS_THREADS) {
-        const int mine = j / k, at = j - mine * k;
-        if (at >= counts(mine)) continue;
-        const Ranked c = lists[mine * LOGPROBS_MAX_TOP + at];
-        int rank = at;
-        for (int o = 0; o < n_lists && rank < k; o++) {
-            if (o == mine) continue;
-            int lo = 0, hi = counts(o);
-            while (lo < hi) {
-                const int mid = (lo + hi) / 2;
-                if (ranks_before(lists[o * LOGPROBS_MAX_TOP + mid], c)) lo = mid + 1;
-                else hi = mid;
-            }
-            rank += lo;
-        }
-        if (rank < k) f(rank, c);
-    }
+    __syncwarp();
+    n = min(n, k);
+    for (int j = lane; j < n; j += 32) list[j] = spare[j];
+    __syncwarp();
+    return n;
 }
 
-template <typename T, int R>
-__global__ void __launch_bounds__(LOGPROBS_THREADS) logprobs_kernel(LogProbs p) {
-    constexpr int N = Piece<T>::N, U = 16 / N;  // elements of a piece, pieces a thread takes at a time
-    __shared__ Ranked lists[(R ? LOGPROBS_WARPS : 1) * LOGPROBS_MAX_TOP], best[R ? LOGPROBS_MAX_TOP : 1];
-    __shared__ volatile float bounds[LOGPROBS_WARPS];
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(LOGPROBS_THREADS, 4) logprobs_kernel(LogProbs p) {
+    constexpr int N = Piece<T>::N, U = 16 / N, ROOM = LOGPROBS_NOTED + 32 * N;  // elements of a piece, pieces a thread takes at a time
+    __shared__ Ranked noted[TOP ? LOGPROBS_WARPS : 1][TOP ? ROOM : 1], best[TOP ? LOGPROBS_MAX_TOP : 1];
+    __shared__ Ranked cand[TOP ? LOGPROBS_MAX_SPLITS * LOGPROBS_MAX_TOP : 1];  // in turn: room to sort a list, all lists, the cluster's
+    __shared__ volatile float bounds[LOGPROBS_WARPS], common_s;
     __shared__ RowSums warp_sums[LOGPROBS_WARPS], cta_sums;
-    __shared__ int have[LOGPROBS_WARPS], cta_have;
+    __shared__ int count, in_cta, in_row, have[LOGPROBS_MAX_SPLITS];
     const int split = (int)tc::cluster_rank(), splits = (int)tc::cluster_size(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int row = blockIdx.y;
-    if (threadIdx.x < LOGPROBS_WARPS) bounds[threadIdx.x] = -INFINITY;
+    if (threadIdx.x == 0) count = 0, common_s = -INFINITY;
     pdl_wait();
-    __syncthreads();
     const T *x = (const T *)p.logits + row * p.stride;
     // slices start on a 16-byte boundary of memory; slice 0 also takes the elements before the first one
     const int ahead = min((int)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(T)), p.vocab);
     const int lo = split == 0 ? 0 : min(p.vocab, ahead + split * p.slice), hi = split == splits - 1 ? p.vocab : min(p.vocab, ahead + (split + 1) * p.slice);
     const int body = max(lo, ahead), pieces = (hi - body) / N, tail = body + pieces * N;  // [lo, body) and [tail, hi): less than a piece each
     const uint4 *src = (const uint4 *)(x + body);
-    float m = -3.402823466e38f, l = 0.0f, t = 0.0f;
-    Best<R> top;
-    top.clear();
-    float cut = -INFINITY;  // what an element has to reach to be looked at
-    const int jth = (p.top + LOGPROBS_WARPS - 1) / LOGPROBS_WARPS - 1;
-    auto sum = [&](const float *v, int n, float most) {
+    float m = -3.402823466e38f;
+    float2 l = make_float2(0.0f, 0.0f), t = l;  // of the elements at even places and at odd ones
+    auto sum = [&](const float2 *v, int pairs, float most) {
         if (most > m) {
             const float d = fmaxf(m - most, LOGPROBS_FAR), e = ex2(d * 1.4426950408889634f);
-            t = e * fmaf(l, d, t), l *= e, m = most;
+            t = mul2(make_float2(e, e), fma2(l, make_float2(d, d), t)), l = mul2(make_float2(e, e), l), m = most;
         }
+        const float2 down = make_float2(-m, -m), unit = make_float2(1.4426950408889634f, 1.4426950408889634f);
 #pragma unroll
-        for (int e = 0; e < n; e++) {
-            const float d = v[e] - m, w = ex2(d * 1.4426950408889634f);
-            l += w, t = fmaf(w, fmaxf(d, LOGPROBS_FAR), t);
+        for (int i = 0; i < pairs; i++) {
+            const float2 d = add2(v[i], down), y = mul2(d, unit), w = make_float2(ex2(y.x), ex2(y.y));
+            l = add2(l, w), t = fma2(w, make_float2(fmaxf(d.x, LOGPROBS_FAR), fmaxf(d.y, LOGPROBS_FAR)), t);
         }
     };
-    auto meet = [&](float v, int at) {  // (the whole warp with the same element)
-        if (!(v >= cut)) return;
-        top.insert(v, at, lane);
-        const float last = top.at(p.top - 1), mine = top.at(jth);
-        cut = fmaxf(cut, last == last ? next_up(last) : -INFINITY);
-        if (lane == 0 && mine > bounds[warp]) bounds[warp] = mine;
+    Ranked *list = noted[TOP ? warp : 0];
+    int n = 0;                        // elements in the warp's list
+    float cut = -3.402823466e38f;     // what an element has to reach to be noted
+    auto note = [&](float v, int at, bool real) {  // (the whole warp, an element a lane)
+        const bool hit = real && v >= cut;
+        const unsigned hits = __ballot_sync(0xffffffffu, hit);
+        if (hits) {
+            if (hit) list[n + __popc(hits & ((1u << lane) - 1))] = {v, at};
+            n += __popc(hits);
+        }
+    };
+    auto make_room = [&]() {  // for an element of every lane's next piece
+        if (n <= LOGPROBS_NOTED) return;
+        __syncwarp();
+        n = cut_to_best(list, cand + warp * LOGPROBS_MAX_TOP, n, p.top, lane);
+        if (n == p.top) cut = fmaxf(cut, next_up(list[n - 1].v));
+    };
+    const int in_warp = (p.top + LOGPROBS_WARPS - 1) / LOGPROBS_WARPS;
+    auto bound = [&](float of_lane) {  // the warp's in_warp-th largest of its lanes' numbers
+        float b = -INFINITY;
+        for (int r = 0; r < in_warp; r++) {
+            b = largest_of_lanes(of_lane);
+            const unsigned holders = __ballot_sync(0xffffffffu, of_lane == b);
+            if (lane == __ffs(holders) - 1) of_lane = -INFINITY;  // one of them is taken out
+        }
+        if (lane == 0) bounds[warp] = b;
+    };
+    // What k elements of the slice reach: ceil(k / in_warp) warps have in_warp of them that reach it. The bounds of this moment or earlier
+    // ones, either will do.
+    auto common = [&]() {
+        const float b = bounds[lane & (LOGPROBS_WARPS - 1)];
+        int above = 0;  // (equals in the order of the warps)
+#pragma unroll
+        for (int w = 0; w < LOGPROBS_WARPS; w++) {
+            const float o = __shfl_sync(0xffffffffu, b, w);
+            above += o > b || (o == b && w < (lane & (LOGPROBS_WARPS - 1)));
+        }
+        const unsigned at = __ballot_sync(0xffffffffu, above == (p.top + in_warp - 1) / in_warp - 1);
+        return __shfl_sync(0xffffffffu, b, __ffs(at) - 1);
     };
     auto loose = [&](int from, int to) {  // elements outside the pieces, a lane each
         const int at = from + lane;
         const float v = at < to ? to_float(x[at]) : -INFINITY;
-        if (at < to) sum(&v, 1, v);
-        if (R)
-            for (int i = 0; i < to - from; i++) meet(__shfl_sync(0xffffffffu, v, i), from + i);
+        const float2 alone = make_float2(v, -INFINITY);
+        if (at < to) sum(&alone, 1, v);
+        if (TOP) make_room(), note(v, at, at < to);
     };
-    auto load = [&](int j0, float *v) {
-        uint4 w[U];
+    auto load = [&](int j0, uint4 *w) {
+        if (j0 + 32 * U <= pieces) {
 #pragma unroll
-        for (int u = 0; u < U; u++) w[u] = j0 + 32 * u + lane < pieces ? __ldcs(src + j0 + 32 * u + lane) : Piece<T>::nothing();
+            for (int u = 0; u < U; u++) w[u] = __ldcs(src + j0 + 32 * u + lane);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; u++) w[u] = j0 + 32 * u + lane < pieces ? __ldcs(src + j0 + 32 * u + lane) : Piece<T>::nothing();
+        }
+    };
+    uint4 w[U];
+    load(warp * U * 32, w);
+    bool first = true;
+    for (int j0 = warp * U * 32; first || j0 < pieces; j0 += LOGPROBS_THREADS * U) {
+        __align__(8) float v[16];
 #pragma unroll
         for (int u = 0; u < U; u++) Piece<T>::floats(w[u], v + u * N);
+        load(j0 + LOGPROBS_THREADS * U, w);
         float most = v[0];
 #pragma unroll
         for (int e = 1; e < 16; e++) most = fmaxf(most, v[e]);
-        return most;
-    };
-    float v[16], most = load(warp * U * 32, v);
-    if (R) {  // the first bounds: ceil(k / 8) lanes of every warp have an element that reaches their warp's
-        float rest = most, b = -INFINITY;
-        for (int r = 0; r <= jth; r++) {
-            b = warp_max(rest);
-            const unsigned holders = __ballot_sync(0xffffffffu, rest == b);
-            if (lane == __ffs(holders) - 1) rest = -INFINITY;  // one of them is taken out
+        if (TOP) {
+            if (first) {  // the first bounds
+                bound(most);
+                __syncthreads();
+                cut = fmaxf(cut, common());
+            }
+            else cut = fmaxf(cut, common_s);
         }
-        if (lane == 0) bounds[warp] = b;
-        __syncthreads();
-    }
-    if (warp == 0) loose(lo, body);
-    for (int j0 = warp * U * 32; j0 < pieces; j0 += LOGPROBS_THREADS * U) {
-        if (R) {
-            float b = bounds[lane & (LOGPROBS_WARPS - 1)];
+        if (first && warp == 0) loose(lo, body);
+        if (TOP && __any_sync(0xffffffffu, most >= cut)) {
 #pragma unroll
-            for (int o = LOGPROBS_WARPS / 2; o > 0; o >>= 1) b = fminf(b, __shfl_xor_sync(0xffffffffu, b, o));
-            cut = fmaxf(cut, b);
-            if (__any_sync(0xffffffffu, most >= cut)) {
+            for (int u = 0; u < U; u++) {
+                float of_piece = v[u * N];
 #pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const int at = j0 + 32 * u + lane;
-                    float of_piece = v[u * N];
+                for (int e = 1; e < N; e++) of_piece = fmaxf(of_piece, v[u * N + e]);
+                if (!__any_sync(0xffffffffu, of_piece >= cut)) continue;
+                make_room();
 #pragma unroll
-                    for (int e = 1; e < N; e++) of_piece = fmaxf(of_piece, v[u * N + e]);
-                    for (unsigned hits = __ballot_sync(0xffffffffu, of_piece >= cut && at < pieces); hits; hits &= hits - 1) {
-                        const int from = __ffs(hits) - 1;
-#pragma unroll
-                        for (int e = 0; e < N; e++) meet(__shfl_sync(0xffffffffu, v[u * N + e], from), body + (j0 + 32 * u + from) * N + e);
-                    }
-                }
+                for (int e = 0; e < N; e++) note(v[u * N + e], body + (j0 + 32 * u + lane) * N + e, j0 + 32 * u + lane < pieces);
+            }
+            if (!first && __any_sync(0xffffffffu, most >= cut && most > m)) {  // (else no thread's maximum that counts has moved)
+                bound(fmaxf(m, most));
+                __syncwarp();
+                const float b = common();
+                if (lane == 0) common_s = b;
             }
         }
-        sum(v, 16, most);
-        most = load(j0 + LOGPROBS_THREADS * U, v);
+        sum((const float2 *)v, 8, most);
+        first = false;
     }
     if (warp == LOGPROBS_WARPS - 1) loose(tail, hi);
-    RowSums mine = {m, l, t, 0.0f};
+    RowSums mine = {m, l.x + l.y, t.x + t.y, 0.0f};
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         RowSums other;
@@ -243,28 +259,29 @@ __global__ void __launch_bounds__(LOGPROBS_THREADS) logprobs_kernel(LogProbs p) 
         mine = joined(mine, other);
     }
     if (lane == 0) warp_sums[warp] = mine;
-    if (R) {
-        int n = 0;
-#pragma unroll
-        for (int r = 0; r < R; r++) {
-            lists[warp * LOGPROBS_MAX_TOP + 32 * r + lane] = {top.v[r], top.i[r]};
-            n += __popc(__ballot_sync(0xffffffffu, top.v[r] == top.v[r]));
-        }
-        if (lane == 0) have[warp] = min(n, p.top);
-    }
+    if (TOP) make_room();
     __syncthreads();
-    if (R) {
-        merge_lists(lists, LOGPROBS_WARPS, p.top, [&](int c) { return have[c]; }, [&](int rank, Ranked c) { best[rank] = c; });
-        if (threadIdx.x == 0) {
-            int n = 0;
-            for (int w = 0; w < LOGPROBS_WARPS; w++) n += have[w];
-            cta_have = min(n, p.top);
-        }
+    if (TOP) {
+        const float b = common();
+        for (int i = lane; i < n; i += 32)
+            if (list[i].v >= b) cand[atomicAdd(&count, 1)] = list[i];
     }
     if (warp == 0) {
         RowSums s = warp_sums[0];
         for (int w = 1; w < LOGPROBS_WARPS; w++) s = joined(s, warp_sums[w]);
         if (lane == 0) cta_sums = s;
+    }
+    __syncthreads();
+    if (TOP) {
+        const int all = count;
+        if (threadIdx.x == 0) in_cta = all;
+        for (int j = threadIdx.x; j < all; j += LOGPROBS_THREADS) {
+            const Ranked c = cand[j];
+            int rank = 0;
+#pragma unroll 8
+            for (int i = 0; i < all; i++) rank += ranks_before(cand[i], c);
+            if (rank < p.top) best[rank] = c;
+        }
     }
     if (splits > 1) tc::cluster_sync();
     else __syncthreads();
@@ -281,25 +298,57 @@ __global__ void __launch_bounds__(LOGPROBS_THREADS) logprobs_kernel(LogProbs p) 
             p.logprob[row] = none || token < 0 || token >= p.vocab ? nan : to_float(x[token]) - s.m - log_l;
             if (p.entropy) p.entropy[row] = none ? nan : log_l - s.t / s.l;
         }
-        if (R) {
+        if (TOP) {
             const long long at = (long long)row * p.top;
             auto put = [&](int rank, Ranked c) {
                 p.top_ids[at + rank] = none ? -1 : c.i, p.top_logprobs[at + rank] = none ? nan : c.v - s.m - log_l;
             };
+            int found = min(in_cta, p.top);
             if (none) {
                 for (int j = threadIdx.x; j < p.top; j += LOGPROBS_THREADS) put(j, {0.0f, 0});
+                found = p.top;
             } else if (splits == 1) {
-                if (threadIdx.x < p.top) put(threadIdx.x, best[threadIdx.x]);
+                if (threadIdx.x < found) put(threadIdx.x, best[threadIdx.x]);
             } else {
-                __shared__ int of_cta[LOGPROBS_MAX_SPLITS];
+                // of the CTAs' best those that reach the largest of their k-th, ranked
+                if (threadIdx.x == 0) count = 0;
+                if (warp == 0) {
+                    int n_c = 0;
+                    float kth = -INFINITY;
+                    if (lane < splits) {
+                        n_c = min(__float_as_int(tc::ld_cluster_f1(tc::peer_smem(tc::smem_addr(&in_cta), lane))), p.top);
+                        const float v = tc::ld_cluster_f1(tc::peer_smem(tc::smem_addr(&best[p.top - 1].v), lane));
+                        have[lane] = n_c, kth = n_c == p.top ? v : -INFINITY;
+                    }
+                    found = __reduce_add_sync(0xffffffffu, n_c), kth = warp_max(kth);
+                    if (lane == 0) common_s = kth, in_row = found;
+                }
+                __syncthreads();
+                const float kth = common_s;
                 for (int j = threadIdx.x; j < splits * p.top; j += LOGPROBS_THREADS) {
                     const int c = j / p.top, i = j - c * p.top;
+                    if (i >= have[c]) continue;
                     const float2 b = tc::ld_cluster_f2(tc::peer_smem(tc::smem_addr(best + i), c));
-                    lists[c * LOGPROBS_MAX_TOP + i] = {b.x, __float_as_int(b.y)};
+                    if (b.x >= kth) cand[atomicAdd(&count, 1)] = {b.x, __float_as_int(b.y)};
                 }
-                if (threadIdx.x < splits) of_cta[threadIdx.x] = __float_as_int(tc::ld_cluster_f1(tc::peer_smem(tc::smem_addr(&cta_have), threadIdx.x)));
                 __syncthreads();
-                merge_lists(lists, splits, p.top, [&](int c) { return of_cta[c]; }, put);
+                const int all = count;
+                for (int j = threadIdx.x; j < all; j += LOGPROBS_THREADS) {
+                    const Ranked c = cand[j];
+                    int rank = 0;
+#pragma unroll 8
+                    for (int i = 0; i < all; i++) rank += ranks_before(cand[i], c);
+                    if (rank < p.top) put(rank, c);
+                }
+                found = in_row;
+            }
+            // fewer than k tokens can come: the first of the others fill the places
+            for (int j0 = 0; j0 < p.vocab && found < p.top && warp == 0; j0 += 32) {
+                const bool hit = j0 + lane < p.vocab && to_float(x[j0 + lane]) == -INFINITY;
+                const unsigned hits = __ballot_sync(0xffffffffu, hit);
+                const int rank = found + __popc(hits & ((1u << lane) - 1));
+                if (hit && rank < p.top) put(rank, {-INFINITY, j0 + lane});
+                found += __popc(hits);
             }
         }
     }
@@ -314,8 +363,8 @@ extern "C" int abk_token_logprobs(const void *logits, int dtype, long long strid
         ABK_REFUSE("token_logprobs: %d most likely tokens of a vocabulary of %d (at most %d)", top, vocab, LOGPROBS_MAX_TOP);
     const int size = dtype == ABK_F32 ? 4 : 2, piece = 16 / size;
     if ((uintptr_t)logits % size) ABK_REFUSE("token_logprobs: logits that are not aligned to their own size");
-    // CTAs to a row: until the GPU is full (8 to an SM), in slices of at least 4,096 elements, as many as a cluster holds
-    const int full = 8 * abk_sm_count();
+    // CTAs to a row: until the GPU is full (4 to an SM), in slices of at least 4,096 elements, as many as a cluster holds
+    const int full = 4 * abk_sm_count();
     int splits = 1;
     while (splits < LOGPROBS_MAX_SPLITS && (long long)n_rows * splits * 2 <= full && vocab / (splits * 2) >= 4096) splits *= 2;
     LogProbs p;
@@ -323,8 +372,12 @@ extern "C" int abk_token_logprobs(const void *logits, int dtype, long long strid
     p.top_ids = top_ids, p.top_logprobs = top_logprobs;
     p.slice = (vocab + splits * piece - 1) / (splits * piece) * piece;
     void (*kernel)(LogProbs) = nullptr;
-    if (dtype == ABK_F32) kernel = top == 0 ? logprobs_kernel<float, 0> : top <= 32 ? logprobs_kernel<float, 1> : logprobs_kernel<float, 2>;
-    else kernel = top == 0 ? logprobs_kernel<__nv_bfloat16, 0> : top <= 32 ? logprobs_kernel<__nv_bfloat16, 1> : logprobs_kernel<__nv_bfloat16, 2>;
+    if (dtype == ABK_F32) kernel = top == 0 ? logprobs_kernel<float, false> : logprobs_kernel<float, true>;
+    else kernel = top == 0 ? logprobs_kernel<__nv_bfloat16, false> : logprobs_kernel<__nv_bfloat16, true>;
+    if (splits > 8) {
+        const cudaError_t e = cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return (int)e;
+    }
     for (int first = 0; first < n_rows; first += 32768) {  // (rows of a grid)
         LogProbs q = p;
         const int rows = n_rows - first < 32768 ? n_rows - first : 32768;
