@@ -80,6 +80,15 @@ __device__ __forceinline__ RowSums joined(RowSums a, RowSums b) {
     r.t = fmaf(fmaf(a.l, da, a.t), ea, fmaf(b.l, db, b.t) * eb);
     return r;
 }
+// Of the 2 * `half` neighbouring lanes together, in every one of them.
+__device__ __forceinline__ RowSums joined_lanes(RowSums a, int half) {
+    for (int o = half; o > 0; o >>= 1) {
+        RowSums b;
+        b.m = __shfl_xor_sync(0xffffffffu, a.m, o), b.l = __shfl_xor_sync(0xffffffffu, a.l, o), b.t = __shfl_xor_sync(0xffffffffu, a.t, o);
+        a = joined(a, b);
+    }
+    return a;
+}
 // The next float32 number above x (which is not NaN).
 __device__ __forceinline__ float next_up(float x) {
     if (x == 0.0f) return __int_as_float(1);
@@ -139,6 +148,11 @@ __global__ void __launch_bounds__(LOGPROBS_THREADS, 4) logprobs_kernel(LogProbs 
     const int lo = split == 0 ? 0 : min(p.vocab, ahead + split * p.slice), hi = split == splits - 1 ? p.vocab : min(p.vocab, ahead + (split + 1) * p.slice);
     const int body = max(lo, ahead), pieces = (hi - body) / N, tail = body + pieces * N;  // [lo, body) and [tail, hi): less than a piece each
     const uint4 *src = (const uint4 *)(x + body);
+    float given = __int_as_float(0x7fffffff);  // the given token's logit
+    if (split == 0 && threadIdx.x == 0) {
+        const int token = p.tokens[row];
+        if (token >= 0 && token < p.vocab) given = to_float(x[token]);
+    }
     float m = -3.402823466e38f;
     float2 l = make_float2(0.0f, 0.0f), t = l;  // of the elements at even places and at odd ones
     auto sum = [&](const float2 *v, int pairs, float most) {
@@ -251,13 +265,7 @@ __global__ void __launch_bounds__(LOGPROBS_THREADS, 4) logprobs_kernel(LogProbs 
         first = false;
     }
     if (warp == LOGPROBS_WARPS - 1) loose(tail, hi);
-    RowSums mine = {m, l.x + l.y, t.x + t.y, 0.0f};
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        RowSums other;
-        other.m = __shfl_xor_sync(0xffffffffu, mine.m, o), other.l = __shfl_xor_sync(0xffffffffu, mine.l, o), other.t = __shfl_xor_sync(0xffffffffu, mine.t, o);
-        mine = joined(mine, other);
-    }
+    const RowSums mine = joined_lanes({m, l.x + l.y, t.x + t.y, 0.0f}, 16);
     if (lane == 0) warp_sums[warp] = mine;
     if (TOP) make_room();
     __syncthreads();
@@ -267,8 +275,7 @@ __global__ void __launch_bounds__(LOGPROBS_THREADS, 4) logprobs_kernel(LogProbs 
             if (list[i].v >= b) cand[atomicAdd(&count, 1)] = list[i];
     }
     if (warp == 0) {
-        RowSums s = warp_sums[0];
-        for (int w = 1; w < LOGPROBS_WARPS; w++) s = joined(s, warp_sums[w]);
+        const RowSums s = joined_lanes(warp_sums[lane & (LOGPROBS_WARPS - 1)], LOGPROBS_WARPS / 2);
         if (lane == 0) cta_sums = s;
     }
     __syncthreads();
@@ -287,15 +294,14 @@ __global__ void __launch_bounds__(LOGPROBS_THREADS, 4) logprobs_kernel(LogProbs 
     else __syncthreads();
     if (split == 0) {
         RowSums s = cta_sums;
-        for (int c = 1; c < splits; c++) {
-            const float4 o = tc::ld_cluster_f4(tc::peer_smem(tc::smem_addr(&cta_sums), c));
-            s = joined(s, {o.x, o.y, o.z, 0.0f});
+        if (splits > 1) {  // a CTA's a lane
+            const float4 o = tc::ld_cluster_f4(tc::peer_smem(tc::smem_addr(&cta_sums), lane & (splits - 1)));
+            s = joined_lanes({o.x, o.y, o.z, 0.0f}, splits / 2);
         }
         const float log_l = logf(s.l), nan = __int_as_float(0x7fffffff);
         const bool none = !(s.l > 0.0f);  // nothing can come, or a NaN, or +inf (which is one less itself)
         if (threadIdx.x == 0) {
-            const int token = p.tokens[row];
-            p.logprob[row] = none || token < 0 || token >= p.vocab ? nan : to_float(x[token]) - s.m - log_l;
+            p.logprob[row] = none ? nan : given - s.m - log_l;
             if (p.entropy) p.entropy[row] = none ? nan : log_l - s.t / s.l;
         }
         if (TOP) {
@@ -310,17 +316,19 @@ __global__ void __launch_bounds__(LOGPROBS_THREADS, 4) logprobs_kernel(LogProbs 
             } else if (splits == 1) {
                 if (threadIdx.x < found) put(threadIdx.x, best[threadIdx.x]);
             } else {
-                // of the CTAs' best those that reach the largest of their k-th, ranked
+                // of the CTAs' best those that reach what k of them reach: the largest of their k-th, the smallest of their ceil(k / CTAs)-th
                 if (threadIdx.x == 0) count = 0;
                 if (warp == 0) {
                     int n_c = 0;
-                    float kth = -INFINITY;
+                    const int few = (p.top + splits - 1) / splits;
+                    float kth = -INFINITY, all_have = INFINITY;
                     if (lane < splits) {
                         n_c = min(__float_as_int(tc::ld_cluster_f1(tc::peer_smem(tc::smem_addr(&in_cta), lane))), p.top);
                         const float v = tc::ld_cluster_f1(tc::peer_smem(tc::smem_addr(&best[p.top - 1].v), lane));
-                        have[lane] = n_c, kth = n_c == p.top ? v : -INFINITY;
+                        const float w = tc::ld_cluster_f1(tc::peer_smem(tc::smem_addr(&best[few - 1].v), lane));
+                        have[lane] = n_c, kth = n_c == p.top ? v : -INFINITY, all_have = n_c >= few ? w : -INFINITY;
                     }
-                    found = __reduce_add_sync(0xffffffffu, n_c), kth = warp_max(kth);
+                    found = __reduce_add_sync(0xffffffffu, n_c), kth = fmaxf(warp_max(kth), -warp_max(-all_have));
                     if (lane == 0) common_s = kth, in_row = found;
                 }
                 __syncthreads();
