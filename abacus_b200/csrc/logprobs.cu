@@ -17,6 +17,7 @@
 #define ABK_DEFINE_ERROR
 #include "common.cuh"
 #include "tc_common.cuh"
+#include "logprobs.cuh"
 
 #define LOGPROBS_MAX_TOP 64
 #define LOGPROBS_WARPS 8
@@ -24,7 +25,6 @@
 #define LOGPROBS_MAX_SPLITS 16
 static_assert(LOGPROBS_MAX_SPLITS >= 2 * LOGPROBS_WARPS, "room for all lists");
 #define LOGPROBS_NOTED 128  // elements a warp's list has room for beside those of one piece of every lane
-#define LOGPROBS_FAR (-1e30f)  // a distance below the maximum at which nothing is left, and a finite one
 
 struct LogProbs {
     const void *logits;
@@ -40,54 +40,11 @@ struct __align__(8) Ranked {
     int i;
 };
 __device__ __forceinline__ bool ranks_before(Ranked a, Ranked b) { return a.v > b.v || (a.v == b.v && a.i < b.i); }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 // The largest number of a warp's lanes.
 __device__ __forceinline__ float largest_of_lanes(float v) {
     float r;
     asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
     return r;
-}
-// Two float32 operations at once.
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(*(unsigned long long *)&r) : "l"(*(unsigned long long *)&a), "l"(*(unsigned long long *)&b));
-    return r;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(*(unsigned long long *)&r) : "l"(*(unsigned long long *)&a), "l"(*(unsigned long long *)&b));
-    return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(*(unsigned long long *)&r) : "l"(*(unsigned long long *)&a), "l"(*(unsigned long long *)&b), "l"(*(unsigned long long *)&c));
-    return r;
-}
-// Maximum m; l = sum e^(x - m) and t = sum (x - m) e^(x - m). Without elements m is the lowest number and l is zero.
-struct __align__(16) RowSums {
-    float m, l, t, pad;
-};
-__device__ __forceinline__ RowSums joined(RowSums a, RowSums b) {
-    RowSums r;
-    r.m = fmaxf(a.m, b.m), r.pad = 0.0f;
-    const float da = fmaxf(a.m - r.m, LOGPROBS_FAR), db = fmaxf(b.m - r.m, LOGPROBS_FAR);
-    const float ea = ex2(da * 1.4426950408889634f), eb = ex2(db * 1.4426950408889634f);
-    r.l = fmaf(a.l, ea, b.l * eb);
-    r.t = fmaf(fmaf(a.l, da, a.t), ea, fmaf(b.l, db, b.t) * eb);
-    return r;
-}
-// Of the 2 * `half` neighbouring lanes together, in every one of them.
-__device__ __forceinline__ RowSums joined_lanes(RowSums a, int half) {
-    for (int o = half; o > 0; o >>= 1) {
-        RowSums b;
-        b.m = __shfl_xor_sync(0xffffffffu, a.m, o), b.l = __shfl_xor_sync(0xffffffffu, a.l, o), b.t = __shfl_xor_sync(0xffffffffu, a.t, o);
-        a = joined(a, b);
-    }
-    return a;
 }
 // The next float32 number above x (which is not NaN).
 __device__ __forceinline__ float next_up(float x) {

@@ -544,15 +544,26 @@ def gemm_tc_logprobs(x, w, tokens, logprob, entropy, ws, m=None):
     and entropy[r] (or None), float32. ws: a Workspace for the parts of the sums. A logit that is not finite makes its row NaN."""
     _here("gemm_tc_logprobs", x, w, tokens, logprob, entropy)
     m = x.shape[0] if m is None else m
-    (n, k), rows = w.shape, 512
+    vocab, k = w.shape
     assert x.dim() == 2 and x.shape[1] == k and 0 <= m <= x.shape[0]
+    assert tokens.dtype == torch.int32 and tokens.is_contiguous() and tokens.numel() >= m
+    for t in (logprob, entropy):
+        assert t is None or (t.dtype == torch.float32 and t.is_contiguous() and t.numel() >= m)
     if not gemm_tc_logprobs_takes(x, w):
         raise KernelRefused("gemm_tc_logprobs: bfloat16 rows of a multiple of 8, 16-byte aligned")
-    logits = ws.get("logprobs_logits", (rows, n), torch.float32)
-    for lo in range(0, m, rows):
-        hi = min(m, lo + rows)
-        gemm_tc(x[lo:hi], w, logits[:hi - lo])
-        token_logprobs(logits[:hi - lo], tokens[lo:hi], logprob[lo:hi], entropy=None if entropy is None else entropy[lo:hi])
+    lib = load_module("gemm_logprobs")
+    memory = ws.get("logprobs_sums", (_gemm_logprobs_floats(m),), torch.float32)
+    fn = _typed(lib.abk_gemm_logprobs, "ppiiillpppplpp")
+    _check(lib, fn(x.data_ptr(), w.data_ptr(), m, vocab, k, x.stride(0), w.stride(0), tokens.data_ptr(), logprob.data_ptr(), _at(entropy),
+                   memory.data_ptr(), memory.numel(), kernel_status(x.device).data_ptr(), _raw_stream()), "gemm_tc_logprobs",
+           kernels=2 * -(-m // 16384))
+
+
+@functools.lru_cache(maxsize=4096)
+def _gemm_logprobs_floats(m):
+    lib = load_module("gemm_logprobs")
+    lib.abk_gemm_logprobs_floats.restype = ctypes.c_longlong
+    return lib.abk_gemm_logprobs_floats(_i(m))
 
 
 # ------------------------------------------------------------------ keys and values in 8 bits (csrc/kv8.cu, csrc/attention_kv8.cu)
