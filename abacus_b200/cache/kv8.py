@@ -17,9 +17,10 @@ PAGE, BLOCK = 64, 16
 FORMS = {"int8": torch.uint8, "e4m3": torch.float8_e4m3fn}
 
 
-@dataclass
+@dataclass(frozen=True)
 class LayerKV8:
-    """What the kernels need to find a sequence's keys and values of one schedule entry in an 8-bit cache."""
+    """What the kernels need to find a sequence's keys and values of one schedule entry in an 8-bit cache. The tensors are looked at
+    once, here: their addresses and sizes go to every call."""
     k: torch.Tensor       # uint8 ("int8") or float8_e4m3fn ("e4m3") [pages, kv heads, 64, head_dim]
     v: torch.Tensor
     scales: torch.Tensor  # float32 [pages, kv heads, 2 (keys, values), 4 blocks of the page]
@@ -49,9 +50,12 @@ class LayerKV8:
             if t.device != self.k.device:
                 raise ValueError(f"{name} of an 8-bit cache is on {t.device}, its keys on {self.k.device}")
 
-    @property
-    def form(self):
-        return "int8" if self.k.dtype == torch.uint8 else "e4m3"
+        known = dict(form="int8" if self.k.dtype == torch.uint8 else "e4m3", n_pages=pages, n_kv_heads=heads, head_dim=dim,
+                     n_slots=self.open.shape[0], device_index=self.k.get_device(),
+                     pointers=tuple(t.data_ptr() for t in (self.k, self.v, self.scales, self.open)), table_pointer=self.page_table.data_ptr(),
+                     room=None if self.ring_pages else self.table_width * PAGE)
+        for name, value in known.items():
+            object.__setattr__(self, name, value)
 
 
 def pools(n_entries, n_pages, n_slots, n_kv_heads, head_dim, form, device):

@@ -50,7 +50,7 @@ struct AttnKv8 {
     PagedCache cache;
     const float *scales;
     const __nv_bfloat16 *open;
-    int n_pages, *status, stages;
+    int n_pages, n_slots, *status, stages;
     int n_rows, pairs;       // rows of the launch; pairs of a row: n_kv_heads * runs
     int first_row;           // of the step, of this launch
     float *parts;            // [2 * grid][heads of a pair][HD + 4]
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(KV8_THREADS, KV8_CTAS) attention_kv8_kernel(co
         const int seq = p.token_seq[p.first_row + r], pos = p.token_pos[p.first_row + r];
         const int lo = p.window > 0 && pos - p.window + 1 > 0 ? pos - p.window + 1 : 0;
         first_unit[r + 1] = seq < 0 ? 0 : units_of(pos, lo);
-        row_info[r] = seq < 0 ? make_int4(0, 0, 0, 0) : make_int4(pos, p.seq_slot[seq], p.seq_len_after[seq] / KV8_BLOCK, lo);
+        row_info[r] = seq < 0 ? make_int4(0, 0, 0, 0) : make_int4(pos, kv8_slot(p.seq_slot[seq], p.n_slots, p.status), p.seq_len_after[seq] / KV8_BLOCK, lo);
     }
     __syncthreads();
     if (warp == 0) {
@@ -531,7 +531,7 @@ extern "C" long long abk_attention_kv8_part_floats(int n_heads, int n_kv_heads, 
 extern "C" int abk_attention_kv8(const void *q, long long q_row, void *out, int n_rows, int n_heads, int n_kv_heads, int head_dim,
                                  int form, float scale, int window, const int *token_seq, const int *token_pos, const int *seq_slot,
                                  const int *seq_len_after, const void *k, const void *v, const float *scales, const void *open,
-                                 const int *page_table, int table_width, int ring_pages, int pool_pages, float *parts,
+                                 const int *page_table, int table_width, int ring_pages, int pool_pages, int n_slots, float *parts,
                                  long long part_floats, int *status, void *stream) {
     if (n_rows <= 0) return 0;
     if (head_dim != 64 && head_dim != 128) ABK_REFUSE("attention_kv8: head_dim %d is not 64 or 128", head_dim);
@@ -554,7 +554,7 @@ extern "C" int abk_attention_kv8(const void *q, long long q_row, void *out, int 
     p.scale_log2 = scale * 1.4426950408889634f, p.window = window, p.token_seq = token_seq, p.token_pos = token_pos;
     p.seq_slot = seq_slot, p.seq_len_after = seq_len_after, p.cache.page_table = page_table, p.cache.table_width = table_width;
     p.cache.ring_pages = ring_pages, p.cache.tokens_per_page = KV8_PAGE, p.scales = scales, p.open = (const __nv_bfloat16 *)open;
-    p.n_pages = pool_pages, p.status = status, p.runs = runs, p.pairs = n_kv_heads * runs, p.parts = parts;
+    p.n_pages = pool_pages, p.n_slots = n_slots, p.status = status, p.runs = runs, p.pairs = n_kv_heads * runs, p.parts = parts;
     void (*kernel)(CUtensorMap, CUtensorMap, AttnKv8) = nullptr;
     auto of_dim = [&](auto hd, auto tiles) {
         constexpr int HD = decltype(hd)::value, NT = decltype(tiles)::value;

@@ -22,7 +22,7 @@ struct Kv8Write {
     uint8_t *k, *v;
     float *scales;
     __nv_bfloat16 *open;
-    int n_pages, *status;
+    int n_pages, n_slots, *status;
 };
 
 // One block of one head's keys or values, held by a warp: token t of the block, elements 8 c .., in piece i of a lane with
@@ -57,6 +57,10 @@ __global__ void __launch_bounds__(32 * KV8_WARPS) kv8_write_kernel(Kv8Write p) {
         const int row = a + first * KV8_BLOCK - o;
         if (row / KV8_BLOCK != q || row >= a + n) return;
     }
+    if ((unsigned)p.seq_slot[s] >= (unsigned)p.n_slots) {  // nothing is written
+        kv8_slot(p.seq_slot[s], p.n_slots, p.status);
+        return;
+    }
     const int slot = p.seq_slot[s];
     const int b0 = start / KV8_BLOCK, last = (after - 1) / KV8_BLOCK;
     // The open block's place holds the first block's earlier tokens until they have been read: where the step also leaves an
@@ -83,24 +87,21 @@ __global__ void __launch_bounds__(32 * KV8_WARPS) kv8_write_kernel(Kv8Write p) {
                 if (pos >= start && pos < after) *(uint4 *)(open + t * HD + 8 * c) = x[i];
             }
         } else if (cache_keeps(p.cache, pos0, after)) {
-            float most = 0.0f;
-            bool odd = false;  // a value that is not finite
+            __nv_bfloat162 top2 = __floats2bfloat162_rn(0.0f, 0.0f);
 #pragma unroll
             for (int i = 0; i < PIECES; i++) {
                 const __nv_bfloat162 *h = (const __nv_bfloat162 *)&x[i];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float2 f = __bfloat1622float2(h[e]);
-                    most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
-                    odd |= !(fabsf(f.x) < INFINITY) || !(fabsf(f.y) < INFINITY);
-                }
+                for (int e = 0; e < 4; e++) top2 = __hmax2_nan(top2, __habs2(h[e]));
             }
-            most = warp_max(most);
-            odd = __any_sync(0xffffffffu, odd);
+            const float2 two = __bfloat1622float2(top2);
+            const bool odd = __any_sync(0xffffffffu, !(two.x < INFINITY) || !(two.y < INFINITY));  // a value that is not finite
+            const float most = warp_max(fmaxf(two.x, two.y));
+            const Kv8Steps steps = kv8_steps<FORM>(odd ? 0.0f : most);
             const int page = kv8_page(p.cache, p.n_pages, slot, pos0, p.status);
             uint8_t *dst = (j == 0 ? p.k : p.v) + cache_offset(p.cache, page, head, p.n_kv_heads, pos0, HD);
 #pragma unroll
-            for (int i = 0; i < PIECES; i++) *(uint2 *)(dst + 8 * (32 * i + lane)) = kv8_pack<FORM>(x[i], odd ? 0.0f : most);
+            for (int i = 0; i < PIECES; i++) *(uint2 *)(dst + 8 * (32 * i + lane)) = kv8_pack<FORM>(x[i], steps);
             if (lane == 0)
                 p.scales[(((long long)page * p.n_kv_heads + head) * 2 + j) * KV8_PAGE_BLOCKS + (pos0 % KV8_PAGE) / KV8_BLOCK] =
                     odd ? __int_as_float(0x7fffffff) : most / kv8_top<FORM>();
@@ -120,14 +121,11 @@ struct Kv8Read {
     const float *scales;
     const __nv_bfloat16 *open;
     void *out_k, *out_v;
-    int n_pages, *status;
+    int n_pages, n_slots, *status;
 };
 
-__device__ __forceinline__ void store8(float *dst, const float *v) {
-    *(float4 *)dst = make_float4(v[0], v[1], v[2], v[3]);
-    *(float4 *)(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
-}
-__device__ __forceinline__ void store8(__nv_bfloat16 *dst, const float *v) {
+__device__ __forceinline__ void store_piece(float *dst, const float *v) { *(float4 *)dst = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void store_piece(__nv_bfloat16 *dst, const float *v) {
     __nv_bfloat162 h[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) h[e] = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
@@ -137,13 +135,13 @@ __device__ __forceinline__ void store8(__nv_bfloat16 *dst, const float *v) {
 // A warp a block of 16 tokens of one head's keys or values: 8 of them to a page and head.
 template <int HD, int FORM, typename T>
 __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8Read p) {
-    constexpr int LPR = HD / 8, PIECES = Kv8Block<HD>::PIECES;
+    constexpr int N = 16 / sizeof(T), PIECES = KV8_BLOCK * HD / (32 * N);  // a lane stores 16 bytes at a time, N elements
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int page_out = blockIdx.x, head = blockIdx.y, j = warp >> 2, block = warp & 3;
     const int s = last_not_above(p.first_page, p.n_seqs, lane, [&](int first, int) { return first <= page_out; });
     if (s < 0 || page_out >= p.first_page[s + 1]) return;
-    const int after = p.seq_len_after[s], slot = p.seq_slot[s];
+    const int after = p.seq_len_after[s], slot = kv8_slot(p.seq_slot[s], p.n_slots, p.status);
     const int pos0 = (page_out - p.first_page[s]) * KV8_PAGE + block * KV8_BLOCK;
     T *dst = (T *)(j == 0 ? p.out_k : p.out_v) +
              (((long long)page_out * p.n_kv_heads + head) * KV8_PAGE + block * KV8_BLOCK) * HD;
@@ -151,32 +149,34 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8Read p) {
         const int page = kv8_page(p.cache, p.n_pages, slot, pos0, p.status);
         const uint8_t *src = (j == 0 ? p.k : p.v) + cache_offset(p.cache, page, head, p.n_kv_heads, pos0, HD);
         const float scale = p.scales[(((long long)page * p.n_kv_heads + head) * 2 + j) * KV8_PAGE_BLOCKS + block];
-        uint2 x[PIECES];
-#pragma unroll
-        for (int i = 0; i < PIECES; i++) x[i] = *(const uint2 *)(src + 8 * (32 * i + lane));
+        uint32_t x[PIECES][N / 4];
 #pragma unroll
         for (int i = 0; i < PIECES; i++) {
-            float v[8];
-            kv8_unpack<FORM>(x[i].x, v), kv8_unpack<FORM>(x[i].y, v + 4);
+            if constexpr (N == 4) {
+                x[i][0] = *(const uint32_t *)(src + N * (32 * i + lane));
+            } else {
+                const uint2 two = *(const uint2 *)(src + N * (32 * i + lane));
+                x[i][0] = two.x, x[i][N / 4 - 1] = two.y;
+            }
+        }
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] *= scale;
-            store8(dst + 8 * (32 * i + lane), v);
+        for (int i = 0; i < PIECES; i++) {
+            float v[N];
+#pragma unroll
+            for (int e = 0; e < N / 4; e++) kv8_unpack<FORM>(x[i][e], v + 4 * e);
+#pragma unroll
+            for (int e = 0; e < N; e++) v[e] *= scale;
+            store_piece(dst + N * (32 * i + lane), v);
         }
     } else {
         const __nv_bfloat16 *open = p.open + (((long long)slot * 2 + j) * p.n_kv_heads + head) * (KV8_BLOCK * HD);
 #pragma unroll
         for (int i = 0; i < PIECES; i++) {
-            const int t = (32 * i + lane) / LPR;
-            uint4 x = make_uint4(0, 0, 0, 0);  // behind the sequence's last token: zeros
-            if (pos0 + t < after) x = *(const uint4 *)(open + 8 * (32 * i + lane));
-            const __nv_bfloat162 *h = (const __nv_bfloat162 *)&x;
-            float v[8];
+            const int at = N * (32 * i + lane);
+            float v[N];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float2 f = __bfloat1622float2(h[e]);
-                v[2 * e] = f.x, v[2 * e + 1] = f.y;
-            }
-            store8(dst + 8 * (32 * i + lane), v);
+            for (int e = 0; e < N; e++) v[e] = pos0 + at / HD < after ? __bfloat162float(open[at + e]) : 0.0f;  // behind the last token: zeros
+            store_piece(dst + at, v);
         }
     }
 }
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8Read p) {
 extern "C" int abk_kv8_write(const void *qkv, long long row, int n_rows, int n_heads, int n_kv_heads, int head_dim, int form,
                              int n_seqs, int one_each, const int *seq_start, const int *seq_pos0, const int *seq_len_after,
                              const int *seq_slot, const int *page_table, int table_width, int ring_pages, void *k, void *v,
-                             float *scales, void *open, int pool_pages, int *status, void *stream) {
+                             float *scales, void *open, int pool_pages, int n_slots, int *status, void *stream) {
     if (n_rows <= 0 || n_seqs <= 0) return 0;
     if (head_dim != 64 && head_dim != 128) ABK_REFUSE("kv8_write: head_dim %d is not 64 or 128", head_dim);
     if (form != KV8_INT8 && form != KV8_E4M3) ABK_REFUSE("kv8_write: no 8-bit form %d", form);
@@ -198,7 +198,7 @@ extern "C" int abk_kv8_write(const void *qkv, long long row, int n_rows, int n_h
     p.one_each = one_each, p.seq_start = seq_start, p.seq_pos0 = seq_pos0, p.seq_len_after = seq_len_after;
     p.seq_slot = seq_slot, p.cache.page_table = page_table, p.cache.table_width = table_width, p.cache.ring_pages = ring_pages;
     p.cache.tokens_per_page = KV8_PAGE, p.k = (uint8_t *)k, p.v = (uint8_t *)v, p.scales = scales, p.open = (__nv_bfloat16 *)open;
-    p.n_pages = pool_pages, p.status = status;
+    p.n_pages = pool_pages, p.n_slots = n_slots, p.status = status;
     const dim3 grid(units, groups), block(32 * KV8_WARPS);
     auto go = [&](auto kernel) { abk_launch(kernel, grid, block, 0, (cudaStream_t)stream, p); };
     if (head_dim == 64) form == KV8_INT8 ? go(kv8_write_kernel<64, KV8_INT8>) : go(kv8_write_kernel<64, KV8_E4M3>);
@@ -209,7 +209,7 @@ extern "C" int abk_kv8_write(const void *qkv, long long row, int n_rows, int n_h
 extern "C" int abk_kv8_read(const void *k, const void *v, const float *scales, const void *open, int n_kv_heads, int head_dim,
                             int form, const int *page_table, int table_width, int n_seqs, const int *seq_len_after,
                             const int *seq_slot, const int *first_page, int n_pages, void *out_k, void *out_v, int out_dtype,
-                            int pool_pages, int *status, void *stream) {
+                            int pool_pages, int n_slots, int *status, void *stream) {
     if (n_pages <= 0 || n_seqs <= 0) return 0;
     if (head_dim != 64 && head_dim != 128) ABK_REFUSE("kv8_read: head_dim %d is not 64 or 128", head_dim);
     if (form != KV8_INT8 && form != KV8_E4M3) ABK_REFUSE("kv8_read: no 8-bit form %d", form);
@@ -220,7 +220,7 @@ extern "C" int abk_kv8_read(const void *k, const void *v, const float *scales, c
     p.first_page = first_page, p.seq_len_after = seq_len_after, p.seq_slot = seq_slot, p.n_seqs = n_seqs, p.n_kv_heads = n_kv_heads;
     p.cache.page_table = page_table, p.cache.table_width = table_width, p.cache.ring_pages = 0, p.cache.tokens_per_page = KV8_PAGE;
     p.k = (const uint8_t *)k, p.v = (const uint8_t *)v, p.scales = scales, p.open = (const __nv_bfloat16 *)open;
-    p.out_k = out_k, p.out_v = out_v, p.n_pages = pool_pages, p.status = status;
+    p.out_k = out_k, p.out_v = out_v, p.n_pages = pool_pages, p.n_slots = n_slots, p.status = status;
     const dim3 grid(n_pages, n_kv_heads), block(256);
     auto go = [&](auto kernel) { abk_launch(kernel, grid, block, 0, (cudaStream_t)stream, p); };
     auto by_form = [&](auto hd) {

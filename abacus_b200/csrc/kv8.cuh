@@ -15,32 +15,48 @@ enum { KV8_INT8 = 0, KV8_E4M3 = 1 };
 
 template <int FORM> __host__ __device__ constexpr float kv8_top() { return FORM == KV8_INT8 ? 127.0f : 448.0f; }
 
-// Eight bfloat16 values in 8 bits each, `most` the largest magnitude of their block (0: all come out as zero).
-template <int FORM> __device__ __forceinline__ uint2 kv8_pack(uint4 x, float most) {
-    const __nv_bfloat162 *h = (const __nv_bfloat162 *)&x;
-    uint32_t out[2] = {0, 0};
-    // x * (top / 128) and most / 128 are exact, and stay below infinity
-    const float top = kv8_top<FORM>() / 512.0f, whole = most / 512.0f;
+// Eight bfloat16 values in 8 bits each; `by` and `inverse` as kv8_steps makes them of the block's largest magnitude.
+// 127 x / most comes as x times a reciprocal, up to 2^-22 off, and is then rounded to 18 bits: where it is halfway between two steps it
+// is exactly that again (8 bits), and where it is not it is 2^-15 or more away (127 x and an odd number times most are whole
+// numbers of 15 bits, at least 1 apart; 448 x likewise). So the rounding to a step is that of the exact quotient, ties to even. A
+// division takes three times as long.
+struct Kv8Steps {
+    float by, inverse;
+};
+template <int FORM> __device__ __forceinline__ Kv8Steps kv8_steps(float most) {
+    const float by = most < 5e-20f ? 1.8446744073709552e19f : 1.0f;  // 2^64: no reciprocal overflows
+    return {by, most > 0.0f ? kv8_top<FORM>() / (most * by) : 0.0f};
+}
+template <int FORM> __device__ __forceinline__ uint2 kv8_pack(uint4 x, Kv8Steps s) {
+    const uint32_t h[4] = {x.x, x.y, x.z, x.w};
+    uint32_t out[2];
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-        float2 f = __bfloat1622float2(h[e]);
-        f.x = whole > 0.0f ? f.x * top / whole : 0.0f, f.y = whole > 0.0f ? f.y * top / whole : 0.0f;
-        uint32_t pair;
-        if constexpr (FORM == KV8_INT8) {
-            const int lo = __float2int_rn(fminf(fmaxf(f.x, -127.0f), 127.0f)) + 128, hi = __float2int_rn(fminf(fmaxf(f.y, -127.0f), 127.0f)) + 128;
-            pair = (uint32_t)lo | (uint32_t)hi << 8;
-        } else {
-            pair = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+    for (int e = 0; e < 2; e++) {
+        float q[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float f = __uint_as_float(i & 1 ? h[2 * e + i / 2] & 0xffff0000u : h[2 * e + i / 2] << 16);
+            const float y = __fmul_rn(__fmul_rn(f, s.by), s.inverse), t = __fmul_rn(y, 65.0f);
+            q[i] = __fsub_rn(t, __fsub_rn(t, y));
         }
-        out[e >> 1] |= pair << (16 * (e & 1));
+        if constexpr (FORM == KV8_INT8) {  // + 1.5 * 2^23: the whole number in the low bits; + 128
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) w[i] = __float_as_uint(__fadd_rn(q[i], 12582912.0f)) + 128u;
+            out[e] = __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
+        } else {
+            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(q[0], q[1]), __NV_SATFINITE, __NV_E4M3);
+            const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(q[2], q[3]), __NV_SATFINITE, __NV_E4M3);
+            out[e] = lo | hi << 16;
+        }
     }
     return make_uint2(out[0], out[1]);
 }
 // Four numbers of a word as float32 (without the scale).
 template <int FORM> __device__ __forceinline__ void kv8_unpack(uint32_t w, float *v) {
-    if constexpr (FORM == KV8_INT8) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = (float)((int)(w >> (8 * e) & 0xff) - 128);
+    if constexpr (FORM == KV8_INT8) {  // 2^23 + b, less 2^23 + 128
+        v[0] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440)) - 8388736.0f, v[1] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7441)) - 8388736.0f;
+        v[2] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7442)) - 8388736.0f, v[3] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7443)) - 8388736.0f;
     } else {
 #pragma unroll
         for (int e = 0; e < 2; e++) {
@@ -54,10 +70,18 @@ template <int FORM> __device__ __forceinline__ void kv8_unpack(uint32_t w, float
 // The page of a position, 0 where the table names one that is not among the pool's n_pages (and a status bit says so: nothing
 // outside the pool is touched).
 #define KV8_BAD_PAGE 2
+#define KV8_BAD_SLOT 4
 __device__ __forceinline__ int kv8_page(const PagedCache &c, int n_pages, int slot, int pos, int *status) {
     const int page = cache_page(c, slot, pos);
     if ((unsigned)page < (unsigned)n_pages) return page;
     atomicOr(status + 2, KV8_BAD_PAGE);
+    return 0;
+}
+
+// The slot, 0 where it is not one of the cache's n_slots (a status bit says so).
+__device__ __forceinline__ int kv8_slot(int slot, int n_slots, int *status) {
+    if ((unsigned)slot < (unsigned)n_slots) return slot;
+    atomicOr(status + 2, KV8_BAD_SLOT);
     return 0;
 }
 

@@ -571,14 +571,20 @@ KV8_FORMS = {"int8": 0, "e4m3": 1}
 
 
 def _kv8_fits(what, batch, cache, n_kv_heads=None, head_dim=None):
-    """The step's sequences have their slots and their positions their places in the cache."""
-    if n_kv_heads is not None and (cache.k.shape[1] != n_kv_heads or cache.k.shape[3] != head_dim):
-        raise KernelRefused(f"{what}: the cache holds {cache.k.shape[1]} kv heads of {cache.k.shape[3]}, not {n_kv_heads} of {head_dim}")
-    slots = cache.open.shape[0]
-    if any(not 0 <= s.slot < slots for s in batch.sequences):
-        raise KernelRefused(f"{what}: a sequence's slot is outside the cache's {slots}")
-    if cache.ring_pages == 0 and batch.max_len_after > cache.table_width * cache.tokens_per_page:
+    """The step's heads are the cache's, its positions have their places there, and the cache is on the current device."""
+    if n_kv_heads is not None and (cache.n_kv_heads != n_kv_heads or cache.head_dim != head_dim):
+        raise KernelRefused(f"{what}: the cache holds {cache.n_kv_heads} kv heads of {cache.head_dim}, not {n_kv_heads} of {head_dim}")
+    if cache.room is not None and batch.max_len_after > cache.room:
         raise KernelRefused(f"{what}: {batch.max_len_after} tokens are more than the page table's {cache.table_width} pages hold")
+    if cache.device_index != torch._C._cuda_getDevice():
+        raise KernelError(f"{what}: the cache is on {cache.k.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+
+
+@functools.lru_cache(maxsize=4096)
+def _kv8_part_floats(n_heads, n_kv_heads, head_dim, device):
+    lib = load_module("attention_kv8")
+    lib.abk_attention_kv8_part_floats.restype = ctypes.c_longlong
+    return lib.abk_attention_kv8_part_floats(n_heads, n_kv_heads, head_dim)
 
 
 def kv8_write(qkv, n_heads, n_kv_heads, head_dim, batch, cache, row=None):
@@ -587,18 +593,19 @@ def kv8_write(qkv, n_heads, n_kv_heads, head_dim, batch, cache, row=None):
     qkv bfloat16 [rows, (n_heads + 2 n_kv_heads) head_dim], prepared (see qkv_prep); what a sequence holds before the
     step (batch.seq_pos0 tokens) must be in the cache. The same step a second time is the same step only for single tokens, and where
     no sequence both completes a block it had begun and begins another."""
-    _here("kv8_write", qkv, cache.k, batch.seq_slot)
+    _here("kv8_write", qkv, batch.seq_slot)
     lib = load_module("kv8")
     heads_size = (n_heads + 2 * n_kv_heads) * head_dim
     row = row or heads_size
-    assert qkv.dtype == torch.bfloat16 and qkv.is_contiguous() and qkv.shape[1] == row >= heads_size and qkv.shape[0] >= batch.n_rows
+    n, width = qkv.shape
+    assert qkv.dtype == torch.bfloat16 and qkv.is_contiguous() and width == row >= heads_size and n >= batch.n_rows
     _kv8_fits("kv8_write", batch, cache, n_kv_heads, head_dim)
-    fn = _typed(lib.abk_kv8_write, "pliiiiiiipppppiippppipp")
-    _check(lib, fn(qkv.data_ptr(), row, batch.n_rows, n_heads, n_kv_heads, head_dim, KV8_FORMS[cache.form], batch.seq_slot.numel(),
+    fn = _typed(lib.abk_kv8_write, "pliiiiiiipppppiippppiipp")
+    slots = batch.seq_slot
+    _check(lib, fn(qkv.data_ptr(), row, batch.n_rows, n_heads, n_kv_heads, head_dim, KV8_FORMS[cache.form], slots.numel(),
                    1 if batch.is_decode else 0, batch.seq_start.data_ptr(), batch.seq_pos0.data_ptr(), batch.seq_len_after.data_ptr(),
-                   batch.seq_slot.data_ptr(), cache.page_table.data_ptr(), cache.table_width, cache.ring_pages, cache.k.data_ptr(),
-                   cache.v.data_ptr(), cache.scales.data_ptr(), cache.open.data_ptr(), cache.k.shape[0],
-                   kernel_status(qkv.device).data_ptr(), _raw_stream()), "kv8_write")
+                   slots.data_ptr(), cache.table_pointer, cache.table_width, cache.ring_pages, *cache.pointers, cache.n_pages,
+                   cache.n_slots, kernel_status(qkv.device).data_ptr(), _raw_stream()), "kv8_write")
 
 
 def kv8_read(cache, batch, first_page, k, v):
@@ -606,39 +613,41 @@ def kv8_read(cache, batch, first_page, k, v):
     first_page[s] + i of k and v, float32 or bfloat16 [pages, kv heads, 64, head_dim], for all first_page[s + 1] - first_page[s]
     pages of it; places behind the sequence's last token become zeros, other pages are left alone. first_page int32
     [sequences + 1], not falling. Not for a cache under a window."""
-    _here("kv8_read", cache.k, batch.seq_slot, first_page, k, v)
+    _here("kv8_read", batch.seq_slot, first_page, k, v)
     lib = load_module("kv8")
     n_seqs = batch.seq_slot.numel()
     assert first_page.dtype == torch.int32 and first_page.is_contiguous() and first_page.numel() >= n_seqs + 1
-    assert k.shape == v.shape and k.dtype == v.dtype and k.is_contiguous() and v.is_contiguous() and k.shape[1:] == cache.k.shape[1:]
+    assert k.shape == v.shape and k.dtype == v.dtype and k.is_contiguous() and v.is_contiguous()
+    assert tuple(k.shape[1:]) == (cache.n_kv_heads, cache.tokens_per_page, cache.head_dim)
     _kv8_fits("kv8_read", batch, cache)
     if cache.ring_pages:
         raise KernelRefused("kv8_read: a cache under a window does not hold a sequence's first tokens")
-    fn = _typed(lib.abk_kv8_read, "ppppiiipiipppippiipp")
-    _check(lib, fn(cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(), cache.open.data_ptr(), cache.k.shape[1],
-                   cache.k.shape[3], KV8_FORMS[cache.form], cache.page_table.data_ptr(), cache.table_width, n_seqs,
-                   batch.seq_len_after.data_ptr(), batch.seq_slot.data_ptr(), first_page.data_ptr(), k.shape[0], k.data_ptr(),
-                   v.data_ptr(), _dt(k), cache.k.shape[0], kernel_status(k.device).data_ptr(), _raw_stream()), "kv8_read")
+    fn = _typed(lib.abk_kv8_read, "ppppiiipiipppippiiipp")
+    _check(lib, fn(*cache.pointers, cache.n_kv_heads, cache.head_dim, KV8_FORMS[cache.form], cache.table_pointer, cache.table_width,
+                   n_seqs, batch.seq_len_after.data_ptr(), batch.seq_slot.data_ptr(), first_page.data_ptr(), k.shape[0], k.data_ptr(),
+                   v.data_ptr(), _dt(k), cache.n_pages, cache.n_slots, kernel_status(k.device).data_ptr(), _raw_stream()), "kv8_read")
 
 
 def attention_kv8(qkv, out, n_heads, n_kv_heads, head_dim, scale, window, batch, cache, ws):
     """Causal grouped-query attention of the step's rows (src/model.c:197-211) over an 8-bit cache that holds the step's own keys
     and values too (kv8_write comes first): each row sees the keys up to its position, within `window` of it if given. Any
     number of new tokens a sequence; meant for one or a few (each row reads its keys itself). q is read from qkv's q columns."""
-    _here("attention_kv8", qkv, out, cache.k, batch.token_seq)
+    _here("attention_kv8", qkv, out, batch.token_seq)
     lib = load_module("attention_kv8")
     n, row = batch.n_rows, (n_heads + 2 * n_kv_heads) * head_dim
-    assert qkv.dtype == torch.bfloat16 and qkv.is_contiguous() and qkv.shape[1] == row and qkv.shape[0] >= n
-    assert out.dtype == torch.bfloat16 and out.is_contiguous() and out.shape[1] == n_heads * head_dim and out.shape[0] >= n
+    rows, width = qkv.shape
+    assert qkv.dtype == torch.bfloat16 and qkv.is_contiguous() and width == row and rows >= n
+    rows, width = out.shape
+    assert out.dtype == torch.bfloat16 and out.is_contiguous() and width == n_heads * head_dim and rows >= n
     _kv8_fits("attention_kv8", batch, cache, n_kv_heads, head_dim)
-    lib.abk_attention_kv8_part_floats.restype = ctypes.c_longlong
-    parts = ws.get("attention_kv8_parts", (lib.abk_attention_kv8_part_floats(n_heads, n_kv_heads, head_dim),), torch.float32)
-    fn = _typed(lib.abk_attention_kv8, "plpiiiiifipppppppppiiiplpp")
+    floats = _kv8_part_floats(n_heads, n_kv_heads, head_dim, cache.device_index)
+    parts = ws.get("attention_kv8_parts", (floats,), torch.float32)
+    fn = _typed(lib.abk_attention_kv8, "plpiiiiifipppppppppiiiiplpp")
     _check(lib, fn(qkv.data_ptr(), row, out.data_ptr(), n, n_heads, n_kv_heads, head_dim, KV8_FORMS[cache.form], scale, window or 0,
                    batch.token_seq.data_ptr(), batch.token_pos.data_ptr(), batch.seq_slot.data_ptr(), batch.seq_len_after.data_ptr(),
-                   cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(), cache.open.data_ptr(), cache.page_table.data_ptr(),
-                   cache.table_width, cache.ring_pages, cache.k.shape[0], parts.data_ptr(), parts.numel(), kernel_status(qkv.device).data_ptr(),
-                   _raw_stream()), "attention_kv8", kernels=2 * -(-n // 512))
+                   *cache.pointers, cache.table_pointer, cache.table_width, cache.ring_pages, cache.n_pages, cache.n_slots,
+                   parts.data_ptr(), floats, kernel_status(qkv.device).data_ptr(), _raw_stream()), "attention_kv8",
+           kernels=2 * -(-n // 512))
 
 
 def attention(qkv, out, n_heads, n_kv_heads, head_dim, scale, window, batch, cache, from_step=False, ws=None, lists=None,
