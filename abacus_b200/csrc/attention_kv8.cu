@@ -36,7 +36,7 @@
 #define KV8_MAX_STAGES 16
 #define KV8_THREADS 160
 #define KV8_ROWS 512  // rows of a launch
-#define KV8_CTAS 2    // CTAs an SM holds
+#define KV8_CTAS 2    // CTAs an SM holds (three of them: two documents of 131,071 and 100,000 tokens 95 us, not 89)
 #define KV8_START 4   // pages that starting a pair costs as much as
 
 struct AttnKv8 {
@@ -74,15 +74,16 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     __half2 t = __floats2half2_rn(lo, hi);
     return *(uint32_t *)&t;
 }
-// Numbers of the bytes of `w` that `select` names, as two float16.
-template <int FORM, int LO, int HI> __device__ __forceinline__ uint32_t f16_of_bytes(uint32_t w) {
+// The numbers of a word's four bytes as float16 in two pairs: of bytes 0, 1 and 2, 3, or (STRIDED) of bytes 0, 2 and 1, 3.
+template <int FORM, bool STRIDED> __device__ __forceinline__ void f16_of_word(uint32_t w, uint32_t &first, uint32_t &second) {
     if constexpr (FORM == KV8_INT8) {
-        const uint32_t biased = __byte_perm(w, 0x64646464u, 0x4040 | LO | HI << 8);
-        const __half2 t = __hsub2(*(const __half2 *)&biased, __half2half2(__ushort_as_half(0x6480)));  // 1152
-        return *(const uint32_t *)&t;
+        const __half2 less = __half2half2(__ushort_as_half(0x6480));  // 1152
+        const uint32_t x = __byte_perm(w, 0x64646464u, STRIDED ? 0x4240 : 0x4140), y = __byte_perm(w, 0x64646464u, STRIDED ? 0x4341 : 0x4342);
+        const __half2 p = __hsub2(*(const __half2 *)&x, less), q = __hsub2(*(const __half2 *)&y, less);
+        first = *(const uint32_t *)&p, second = *(const uint32_t *)&q;
     } else {
-        const __half2_raw t = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(__byte_perm(w, 0, LO | HI << 4) & 0xffff), __NV_E4M3);
-        return (uint32_t)t.x | (uint32_t)t.y << 16;
+        if (STRIDED) w = __byte_perm(w, 0, 0x3120);
+        asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}" : "=r"(first), "=r"(second) : "r"(w));
     }
 }
 // Shared address of 16-byte piece `piece` of token `t` in a page of HD-byte rows, written by TMA as rows of 128 bytes with the
@@ -288,7 +289,7 @@ __global__ void __launch_bounds__(KV8_THREADS, KV8_CTAS) attention_kv8_kernel(co
                         moved |= was[nt][e] != u[nt][e];
                         sc[nt][e] = ex2(sc[nt][e] - n), sc[nt][e + 2] = ex2(sc[nt][e + 2] - n);
                         l[nt][e] += sc[nt][e] + sc[nt][e + 2];
-                        f[nt][e] = v_scale * exp2f(n - u[nt][e]);
+                        f[nt][e] = v_scale * ex2(n - u[nt][e]);
                     }
                 }
                 if (__any_sync(0xffffffffu, moved)) {
@@ -326,8 +327,8 @@ __global__ void __launch_bounds__(KV8_THREADS, KV8_CTAS) attention_kv8_kernel(co
                             ldsm_x4(token_piece<HD>(k_base, KV8_BLOCK * warp + 8 * (j8 & 1) + r8, ks + (j8 >> 1)), w[0], w[1], w[2], w[3]);
 #pragma unroll
                             for (int i = 0; i < 2; i++) {
-                                const uint32_t a[4] = {f16_of_bytes<FORM, 0, 1>(w[2 * i]), f16_of_bytes<FORM, 0, 1>(w[2 * i + 1]),
-                                                       f16_of_bytes<FORM, 2, 3>(w[2 * i]), f16_of_bytes<FORM, 2, 3>(w[2 * i + 1])};
+                                uint32_t a[4];
+                                f16_of_word<FORM, false>(w[2 * i], a[0], a[2]), f16_of_word<FORM, false>(w[2 * i + 1], a[1], a[3]);
 #pragma unroll
                                 for (int nt = 0; nt < NT; nt++) mma_f16(sc[nt], a, qf[nt][ks + i][0], qf[nt][ks + i][1]);
                             }
@@ -350,8 +351,8 @@ __global__ void __launch_bounds__(KV8_THREADS, KV8_CTAS) attention_kv8_kernel(co
                             ldsm_x4_t(token_piece<HD>(v_base, KV8_BLOCK * warp + 8 * (j8 & 1) + r8, c + (j8 >> 1)), w[0], w[1], w[2], w[3]);
 #pragma unroll
                             for (int i = 0; i < 2; i++) {
-                                const uint32_t a[4] = {f16_of_bytes<FORM, 0, 2>(w[2 * i]), f16_of_bytes<FORM, 1, 3>(w[2 * i]),
-                                                       f16_of_bytes<FORM, 0, 2>(w[2 * i + 1]), f16_of_bytes<FORM, 1, 3>(w[2 * i + 1])};
+                                uint32_t a[4];
+                                f16_of_word<FORM, true>(w[2 * i], a[0], a[1]), f16_of_word<FORM, true>(w[2 * i + 1], a[2], a[3]);
 #pragma unroll
                                 for (int nt = 0; nt < NT; nt++) mma_f16(o[nt][c + i], a, pf[nt][0], pf[nt][1]);
                             }
@@ -564,7 +565,7 @@ extern "C" int abk_attention_kv8(const void *q, long long q_row, void *out, int 
     if (head_dim == 64) kernel = heads <= 8 ? of_dim(integral_constant<int, 64>(), integral_constant<int, 1>()) : of_dim(integral_constant<int, 64>(), integral_constant<int, 2>());
     else kernel = heads <= 8 ? of_dim(integral_constant<int, 128>(), integral_constant<int, 1>()) : of_dim(integral_constant<int, 128>(), integral_constant<int, 2>());
     const int stage = 2 * KV8_PAGE * head_dim + 2 * KV8_PAGE_BLOCKS * 4, fold_bytes = 4 * heads * (head_dim + 4) * 4 + 1024;
-    p.stages = ((224 - 24) * 1024 / KV8_CTAS - fold_bytes) / stage;  // (24 KB: the rows' table of each CTA)
+    p.stages = ((226 - 12 * KV8_CTAS) * 1024 / KV8_CTAS - fold_bytes) / stage;  // (12 KB: a CTA's table of rows, and what every CTA takes)
     if (p.stages > KV8_MAX_STAGES) p.stages = KV8_MAX_STAGES;
     const int smem = p.stages * stage + fold_bytes;
     const cudaError_t e = abk_allow_shared_memory((const void *)kernel, smem);
