@@ -468,8 +468,11 @@ template <int HD> __global__ void __launch_bounds__(KV8_FOLD_THREADS) attention_
     const int r = blockIdx.y, pair = blockIdx.x / most_heads, g = blockIdx.x - pair * most_heads, lane = threadIdx.x & 31;
     const int kvh = pair / p.runs, g0 = (pair - kvh * p.runs) * KV8_HEADS;
     if (threadIdx.x == 0) before_s = 0, all_s = 0;
-    pdl_wait();
-    if (g0 + g >= group) return;
+    // (the step's rows are not the kernel above's to write: they are counted while it runs)
+    if (g0 + g >= group) {
+        pdl_wait();
+        return;
+    }
     __syncthreads();
     int before = 0, all = 0;
     for (int i = threadIdx.x; i < p.n_rows; i += KV8_FOLD_THREADS) {
@@ -480,6 +483,7 @@ template <int HD> __global__ void __launch_bounds__(KV8_FOLD_THREADS) attention_
     if (lane == 0) atomicAdd(&before_s, before), atomicAdd(&all_s, all);
     __syncthreads();
     const int mine = row_units(p, r);
+    pdl_wait();
     __nv_bfloat16 *out = p.out + ((long long)(p.first_row + r) * p.n_heads + kvh * group + g0 + g) * HD;
     if (mine == 0) {
         if (threadIdx.x < COLS) *(uint2 *)(out + 4 * threadIdx.x) = make_uint2(0, 0);
@@ -495,7 +499,7 @@ template <int HD> __global__ void __launch_bounds__(KV8_FOLD_THREADS) attention_
     float m = -INFINITY, u = -INFINITY, l = 0.0f;
     for (int c = threadIdx.x; c < n; c += KV8_FOLD_THREADS) {
         const float4 mlu = *(const float4 *)(part(c) + most_heads * HD + 4 * g);
-        m = fmaxf(m, mlu.x), u = fmaxf(u, mlu.z), weight[c] = mlu.z;
+        m = fmaxf(m, mlu.x), u = fmaxf(u, mlu.z);
     }
     m = block_max(m, scratch), u = block_max(u, scratch);
     for (int c = threadIdx.x; c < n; c += KV8_FOLD_THREADS) {

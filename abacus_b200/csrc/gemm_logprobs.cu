@@ -6,6 +6,9 @@
 // the L2 for all but the first; up to LP_GROUP tiles of rows (2,048 rows) are a group, and w is read once a group. A pair takes
 // every pairs-th tile of the line. A thread that reads the accumulator has one row and 128 of a tile's columns; the sums of the
 // group's rows wait in shared memory for the row's next tile, and at the group's end every pair leaves its own for every row.
+// The tensor cores' own sums are cut off, not rounded, at every step of 16 products: over K = 4,096 that leaves log probabilities
+// 1.6e-6 off (against 4e-7 over 1,024), relative to their size. So a long K is multiplied in segments of up to 2,048, each into an
+// accumulator of its own, and the reading threads add them up, in registers, while the tensor cores are on the next one.
 // A second kernel joins the pairs' sums, a warp a row. The eight warps that read need 5.5 instructions and one exponential a logit:
 // at K = 1,024 half of the time that the tensor cores take for it.
 #define ABK_DEFINE_ERROR
@@ -20,10 +23,11 @@
 #define LP_STAGES 6
 #define LP_GROUP 8
 #define LP_THREADS 320   // one warp that loads, one that multiplies, eight that read
+#define LP_SEGMENT 32    // blocks of K to a segment at most
 #define LP_MOST_ROWS 16384  // rows of a launch
 
 struct GemmLogProbs {
-    int rows, vocab, k_blocks, m_tiles, v_tiles, tiles, groups;
+    int rows, vocab, k_blocks, segment_blocks, segments, m_tiles, v_tiles, tiles, groups;
     const int *tokens;
     float *given;  // [rows]: the given token's logit, where there is one
     float4 *parts;  // [pairs][rows]
@@ -46,6 +50,7 @@ __device__ __forceinline__ LpTile tile_at(const GemmLogProbs &g, int t) {
 #define LP_STATE_BYTES (LP_GROUP * 2 * LP_ROWS * 16)
 #define LP_SMEM (LP_STAGES * (LP_A_BYTES + LP_B_BYTES) + LP_STATE_BYTES + 1024 /* alignment */ + 256 /* barriers */)
 
+template <bool SEGMENTS>
 __global__ void __launch_bounds__(LP_THREADS) gemm_logprobs_kernel(const __grid_constant__ CUtensorMap map_x,
                                                                    const __grid_constant__ CUtensorMap map_w, GemmLogProbs g) {
     extern __shared__ uint8_t lp_raw[];
@@ -100,29 +105,29 @@ __global__ void __launch_bounds__(LP_THREADS) gemm_logprobs_kernel(const __grid_
         if (lane == 0 && rank == 0) {
             constexpr uint32_t idesc = tc::idesc_bf16_f32(2 * LP_ROWS, LP_COLS);
             int done = 0, it = 0;
-            for (int t = pair; t < g.tiles && !flags[0]; t += pairs, it++) {
-                const int b = it & 1;
-                if (!tc::mbar_wait(&acc_empty[b], ((it >> 1) & 1) ^ 1)) {  // both CTAs are done with this accumulator
-                    flags[0] = 1;
-                    break;
-                }
-                tc::fence_after_sync();
-                for (int kb = 0; kb < g.k_blocks; kb++, done++) {
-                    const int s = done % LP_STAGES;
-                    if (!tc::mbar_wait(&full[s], (done / LP_STAGES) & 1)) {
+            for (int t = pair; t < g.tiles && !flags[0]; t += pairs) {
+                for (int kb = 0; kb < g.k_blocks && !flags[0]; it++) {
+                    const int b = it & 1, kb_end = SEGMENTS ? min(kb + g.segment_blocks, g.k_blocks) : g.k_blocks;
+                    if (!tc::mbar_wait(&acc_empty[b], ((it >> 1) & 1) ^ 1)) {  // both CTAs are done with this accumulator
                         flags[0] = 1;
                         break;
                     }
                     tc::fence_after_sync();
-                    const uint32_t a = tc::smem_addr(a_tiles + s * LP_A_BYTES), bq = tc::smem_addr(b_tiles + s * LP_B_BYTES);
+                    for (bool more = false; kb < kb_end; kb++, done++) {
+                        const int s = done % LP_STAGES;
+                        if (!tc::mbar_wait(&full[s], (done / LP_STAGES) & 1)) {
+                            flags[0] = 1;
+                            break;
+                        }
+                        tc::fence_after_sync();
+                        const uint32_t a = tc::smem_addr(a_tiles + s * LP_A_BYTES), bq = tc::smem_addr(b_tiles + s * LP_B_BYTES);
 #pragma unroll
-                    for (int k = 0; k < LP_K / 16; k++)
-                        tc::mma_ss_pair(tmem + b * LP_COLS, tc::smem_desc_k_sw128(a + k * 32), tc::smem_desc_k_sw128(bq + k * 32), idesc,
-                                        kb > 0 || k > 0);
-                    tc::mma_commit_pair(&empty[s]);
+                        for (int k = 0; k < LP_K / 16; k++, more = true)
+                            tc::mma_ss_pair(tmem + b * LP_COLS, tc::smem_desc_k_sw128(a + k * 32), tc::smem_desc_k_sw128(bq + k * 32), idesc, more);
+                        tc::mma_commit_pair(&empty[s]);
+                    }
+                    if (!flags[0]) tc::mma_commit_pair(&acc_full[b]);
                 }
-                if (flags[0]) break;
-                tc::mma_commit_pair(&acc_full[b]);
             }
         }
     } else {
@@ -146,63 +151,90 @@ __global__ void __launch_bounds__(LP_THREADS) gemm_logprobs_kernel(const __grid_
         };
         clear();
         int it = 0, group = 0;
+        const int segments = SEGMENTS ? g.segments : 1;
+        float sum[SEGMENTS ? LP_COLS / 2 : 1];  // of the segments so far, this thread's columns
         pdl_wait();
-        for (int t = pair; t < g.tiles; t += pairs, it++) {
-            const int b = it & 1;
+        bool ok = true;
+        for (int t = pair; t < g.tiles && ok; t += pairs) {
             const LpTile at = tile_at(g, t);
             while (group < at.group) leave(group++);
             const int p = at.row0 + rank * LP_ROWS + row, col0 = at.col0 + half * (LP_COLS / 2);
             const bool mine = p < g.rows;
             const int wanted = (mine ? g.tokens[p] : -1) - col0;  // the given token's place among this thread's columns
             float4 &kept = state[(at.in_group * 2 + half) * LP_ROWS + row];
-            float4 s = kept;
-            const bool ok = __all_sync(0xffffffffu, !flags[0] && tc::mbar_wait(&acc_full[b], (it >> 1) & 1));
-            if (!ok) {
-                flags[0] = 1;
-                break;
-            }
-            tc::fence_after_sync();
-            if (__any_sync(0xffffffffu, mine)) {
-                float2 l = make_float2(s.y, 0.0f), tt = make_float2(s.z, 0.0f);
-                float m = s.x;
-                const bool here = __any_sync(0xffffffffu, wanted >= 0 && wanted < LP_COLS / 2 && wanted + col0 < g.vocab);
-#pragma unroll 1
-                for (int c0 = 0; c0 < LP_COLS / 2; c0 += 32) {
-                    if (col0 + c0 >= g.vocab) break;
-                    __align__(8) uint32_t w[32];
-                    const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + b * LP_COLS + half * (LP_COLS / 2) + c0;
-                    tc::tmem_ld16(from, w), tc::tmem_ld16(from + 16, w + 16);
-                    tc::tmem_ld_wait();
-                    float *v = (float *)w;
-                    if (col0 + c0 + 32 > g.vocab) {  // the last tile: columns behind the vocabulary weigh nothing
-#pragma unroll
-                        for (int j = 0; j < 32; j++)
-                            if (col0 + c0 + j >= g.vocab) v[j] = LOGPROBS_FAR;
-                    }
-                    if (here) {
-#pragma unroll
-                        for (int j = 0; j < 32; j++)
-                            if (wanted == c0 + j && col0 + c0 + j < g.vocab) g.given[p] = v[j];
-                    }
-                    float most = v[0];
-#pragma unroll
-                    for (int j = 1; j < 32; j++) most = fmaxf(most, v[j]);
-                    if (most > m) {
-                        const float d = fmaxf(m - most, LOGPROBS_FAR), e = ex2(d * 1.4426950408889634f);
-                        tt = mul2(make_float2(e, e), fma2(l, make_float2(d, d), tt)), l = mul2(make_float2(e, e), l), m = most;
-                    }
-                    const float2 down = make_float2(-m, -m), unit = make_float2(1.4426950408889634f, 1.4426950408889634f);
-#pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        const float2 d = add2(((const float2 *)v)[j], down), y = mul2(d, unit), e = make_float2(ex2(y.x), ex2(y.y));
-                        l = add2(l, e), tt = fma2(e, d, tt);
-                    }
+            const float4 s = kept;
+            const bool any = __any_sync(0xffffffffu, mine);
+            for (int segment = 0; segment < segments; segment++, it++) {
+                const int b = it & 1;
+                ok = __all_sync(0xffffffffu, !flags[0] && tc::mbar_wait(&acc_full[b], (it >> 1) & 1));
+                if (!ok) {
+                    flags[0] = 1;
+                    break;
                 }
-                kept = make_float4(m, l.x + l.y, tt.x + tt.y, 0.0f);
+                tc::fence_after_sync();
+                const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + b * LP_COLS + half * (LP_COLS / 2);
+                if (any && segment < segments - 1) {
+                    if constexpr (SEGMENTS) {
+#pragma unroll
+                        for (int c0 = 0; c0 < LP_COLS / 2; c0 += 16) {
+                            uint32_t w[16];
+                            tc::tmem_ld16(acc + c0, w);
+                            tc::tmem_ld_wait();
+#pragma unroll
+                            for (int j = 0; j < 16; j++) sum[c0 + j] = segment ? sum[c0 + j] + __uint_as_float(w[j]) : __uint_as_float(w[j]);
+                        }
+                    }
+                } else if (any) {
+                    float2 l = make_float2(s.y, 0.0f), tt = make_float2(s.z, 0.0f);
+                    float m = s.x;
+                    const bool here = __any_sync(0xffffffffu, wanted >= 0 && wanted < LP_COLS / 2 && wanted + col0 < g.vocab);
+                    auto columns = [&](int c0) {
+                        __align__(8) uint32_t w[32];
+                        tc::tmem_ld16(acc + c0, w), tc::tmem_ld16(acc + c0 + 16, w + 16);
+                        tc::tmem_ld_wait();
+                        float *v = (float *)w;
+                        if constexpr (SEGMENTS) {
+#pragma unroll
+                            for (int j = 0; j < 32; j++) v[j] += sum[c0 + j];
+                        }
+                        if (col0 + c0 + 32 > g.vocab) {  // the last tile: columns behind the vocabulary weigh nothing
+#pragma unroll
+                            for (int j = 0; j < 32; j++)
+                                if (col0 + c0 + j >= g.vocab) v[j] = LOGPROBS_FAR;
+                        }
+                        if (here) {
+#pragma unroll
+                            for (int j = 0; j < 32; j++)
+                                if (wanted == c0 + j && col0 + c0 + j < g.vocab) g.given[p] = v[j];
+                        }
+                        float most = v[0];
+#pragma unroll
+                        for (int j = 1; j < 32; j++) most = fmaxf(most, v[j]);
+                        if (most > m) {
+                            const float d = fmaxf(m - most, LOGPROBS_FAR), e = ex2(d * 1.4426950408889634f);
+                            tt = mul2(make_float2(e, e), fma2(l, make_float2(d, d), tt)), l = mul2(make_float2(e, e), l), m = most;
+                        }
+                        const float2 down = make_float2(-m, -m), unit = make_float2(1.4426950408889634f, 1.4426950408889634f);
+#pragma unroll
+                        for (int j = 0; j < 16; j++) {
+                            const float2 d = add2(((const float2 *)v)[j], down), y = mul2(d, unit), e = make_float2(ex2(y.x), ex2(y.y));
+                            l = add2(l, e), tt = fma2(e, d, tt);
+                        }
+                    };
+                    if constexpr (SEGMENTS) {  // (the sums are registers: every column by its own number)
+#pragma unroll
+                        for (int c0 = 0; c0 < LP_COLS / 2; c0 += 32)
+                            if (col0 + c0 < g.vocab) columns(c0);
+                    } else {
+#pragma unroll 1
+                        for (int c0 = 0; c0 < LP_COLS / 2 && col0 + c0 < g.vocab; c0 += 32) columns(c0);
+                    }
+                    kept = make_float4(m, l.x + l.y, tt.x + tt.y, 0.0f);
+                }
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive_in_cluster(tc::peer_smem(tc::smem_addr(&acc_empty[b]), 0));
             }
-            tc::fence_before_sync();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive_in_cluster(tc::peer_smem(tc::smem_addr(&acc_empty[b]), 0));
         }
         while (group < g.groups) leave(group++);
     }
@@ -259,7 +291,8 @@ extern "C" int abk_gemm_logprobs(const void *x, const void *w, int M, int V, int
     if (((uintptr_t)x & 15) || ((uintptr_t)w & 15) || ldx % 8 || ldw % 8 || ((uintptr_t)memory & 15))
         ABK_REFUSE("gemm_logprobs: operands must be 16-byte aligned with pitches of a multiple of 8");
     if (floats < abk_gemm_logprobs_floats(M)) ABK_REFUSE("gemm_logprobs: room for %lld floats is too little", floats);
-    if (cudaError_t e = abk_allow_shared_memory((const void *)gemm_logprobs_kernel, LP_SMEM)) return (int)e;
+    auto kernel = (K + LP_K - 1) / LP_K > LP_SEGMENT ? gemm_logprobs_kernel<true> : gemm_logprobs_kernel<false>;
+    if (cudaError_t e = abk_allow_shared_memory((const void *)kernel, LP_SMEM)) return (int)e;
     for (int first = 0; first < M; first += LP_MOST_ROWS) {
         const int rows = M - first < LP_MOST_ROWS ? M - first : LP_MOST_ROWS;
         CUtensorMap mx, mw;
@@ -268,13 +301,15 @@ extern "C" int abk_gemm_logprobs(const void *x, const void *w, int M, int V, int
         if (rc) return rc;
         GemmLogProbs g;
         g.rows = rows, g.vocab = V, g.k_blocks = (K + LP_K - 1) / LP_K, g.m_tiles = (rows + 2 * LP_ROWS - 1) / (2 * LP_ROWS);
+        const int parts = (g.k_blocks + LP_SEGMENT - 1) / LP_SEGMENT;  // segments as equal as whole blocks allow
+        g.segment_blocks = (g.k_blocks + parts - 1) / parts, g.segments = (g.k_blocks + g.segment_blocks - 1) / g.segment_blocks;
         g.v_tiles = (V + LP_COLS - 1) / LP_COLS, g.groups = (g.m_tiles + LP_GROUP - 1) / LP_GROUP;
         if ((long long)g.m_tiles * g.v_tiles > 0x3fffffff) ABK_REFUSE("gemm_logprobs: a vocabulary of %d is too many tiles", V);
         g.tiles = g.m_tiles * g.v_tiles, g.tokens = tokens + first, g.status = status;
         int pairs = abk_sm_count() / 2;
         if (g.tiles < pairs) pairs = g.tiles;
         g.parts = (float4 *)memory, g.given = memory + 4ll * pairs * rows;
-        abk_launch_clusters(gemm_logprobs_kernel, dim3(2 * pairs), dim3(LP_THREADS), LP_SMEM, (cudaStream_t)stream, 2, mx, mw, g);
+        abk_launch_clusters(kernel, dim3(2 * pairs), dim3(LP_THREADS), LP_SMEM, (cudaStream_t)stream, 2, mx, mw, g);
         rc = ABK_LAUNCH_RESULT();
         if (rc) return rc;
         abk_launch(logprobs_join_kernel, dim3((rows + 3) / 4), dim3(128), 0, (cudaStream_t)stream, (const float4 *)g.parts, pairs, rows, V,
