@@ -3,6 +3,7 @@
     from abacus_b200 import LM
     lm = LM("model_dir", dtype="bfloat16", max_tokens=65536)
     outs = lm.generate([[1, 2, 3], [4, 5]], max_new_tokens=32, temperature=0.0)
+    scores = lm.score([[1, 2, 3, 4], [4, 5, 6]], top=5)   # how likely each token was, and the five likeliest in its place
 
 Option names and meanings follow abacus's command line (src/main.c:9-23): max_new_tokens is -n,
 temperature is --temp (0 = greedy, default 0.7), seed is --seed (default: the time, src/main.c:112);
@@ -12,9 +13,10 @@ does not, as --raw).
 """
 import os
 import time
+from dataclasses import dataclass
 
 from .engine import Engine, load_model
-from .engine.generate import Generator
+from .engine.generate import Generator, plan_batches, Request
 from .sampling import Sampler
 
 CHAT_TEMPLATE = "<|im_start|>user\n{}<|im_end|>\n<|im_start|>assistant\n<think>\n\n</think>\n\n"  # src/main.c:168
@@ -22,13 +24,28 @@ DEFAULT_CONTEXT = 4096   # abacus caps a sequence at 4,096 tokens (src/model.c:1
 DEFAULT_SEQUENCES = 8    # the cache's default room: this many sequences of that length
 
 
+@dataclass
+class Score:
+    """What a model makes of a text: for every token but the first, its log probability after those before it (natural logarithm),
+    the entropy of the distribution it was taken from, and that distribution's most likely tokens, [(token, log probability)]."""
+    tokens: list
+    logprobs: list
+    entropies: list
+    top: list = None
+
+    @property
+    def total(self):
+        return sum(self.logprobs)
+
+
 class LM:
-    def __init__(self, folder, dtype="bfloat16", max_tokens=None, max_slots=None, max_context=None):
+    def __init__(self, folder, dtype="bfloat16", max_tokens=None, max_slots=None, max_context=None, cache=None):
+        """cache: "int8" or "e4m3" keeps keys and values in 8 bits (see Engine); None: in the model's type."""
         self.model = load_model(folder, dtype)
         spec = self.model.spec
         if max_tokens is None:
             max_tokens = min(spec.max_positions, DEFAULT_CONTEXT) * DEFAULT_SEQUENCES
-        self.engine = Engine(self.model, max_tokens=max_tokens, max_slots=max_slots, max_context=max_context)
+        self.engine = Engine(self.model, max_tokens=max_tokens, max_slots=max_slots, max_context=max_context, cache=cache)
         self.tokenizer = None
         if os.path.exists(os.path.join(folder, "tokenizer.json")):
             from .tokenizer import Tokenizer
@@ -47,17 +64,19 @@ class LM:
         return self.tokenizer.encode(prompt if raw else CHAT_TEMPLATE.format(prompt))
 
     def generate(self, prompts, max_new_tokens=512, temperature=0.7, top_k=20, seed=None, stop_tokens=None,
-                 batch_size=None, raw=False, return_requests=False, on_token=None):
+                 batch_size=None, raw=False, return_requests=False, on_token=None, logprobs=None):
         """Returns one list of new token ids per prompt (strings instead, if the prompts were strings).
         seed None: the time, as abacus's command line does; give a seed to draw the same tokens again.
-        on_token(request, token) is called for every kept token as soon as the host has it."""
+        on_token(request, token) is called for every kept token as soon as the host has it.
+        logprobs: a number k from 0 on gives every kept token its log probability (at temperature 1, before any cut) and the k most
+        likely tokens in its place, in the requests' `logprobs` and `top` (see return_requests)."""
         if seed is None:
             seed = int(time.time())
         as_text = bool(prompts) and isinstance(prompts[0], str)
         ids = [self.encode(p, raw) for p in prompts] if as_text else [list(p) for p in prompts]
         sampler = Sampler(self.model.ctx.device, temperature=temperature, top_k=top_k, seed=seed)
         stops = self.stop_tokens() if stop_tokens is None else list(stop_tokens)
-        gen = Generator(self.engine, sampler, stops, on_token=on_token)
+        gen = Generator(self.engine, sampler, stops, on_token=on_token, logprobs=logprobs)
         requests = gen.generate(ids, max_new_tokens, batch_size=batch_size)
         self.last_stats = gen.stats
         if return_requests:
@@ -67,6 +86,36 @@ class LM:
         return [r.output for r in requests]
 
 
-def generate(folder, prompts, dtype="bfloat16", max_tokens=None, **options):
+    def score(self, texts, top=0, raw=True):
+        """A Score for each text (token-id lists, or strings, which raw=False wraps as generate does): the log probability of every
+        token after the first, and with top > 0 the `top` most likely tokens in its place. Texts go through in batches that
+        fit the cache, and leave nothing there."""
+        as_text = bool(texts) and isinstance(texts[0], str)
+        ids = [self.encode(t, raw) for t in texts] if as_text else [[int(t) for t in text] for text in texts]
+        cache = self.engine.cache
+        scores = [None] * len(ids)
+        requests = [Request(i, tokens, 0) for i, tokens in enumerate(ids)]
+        for batch in plan_batches(requests, self.engine.cache_tokens, cache.max_slots, self.engine.max_context):
+            slots = []
+            try:
+                for r in batch:
+                    slots.append(self.engine.open())
+                entries = [(slot, r.prompt, list(range(len(r.prompt) - 1))) for slot, r in zip(slots, batch)]
+                logprob, entropy, top_ids, top_logprobs = self.engine.score(entries, [t for r in batch for t in r.prompt[1:]], top)
+                logprob, entropy = logprob.tolist(), entropy.tolist()
+                best = [list(zip(i, v)) for i, v in zip(top_ids.tolist(), top_logprobs.tolist())] if top else None
+            finally:
+                for slot in slots:
+                    self.engine.close(slot)
+            at = 0
+            for r in batch:
+                n = len(r.prompt) - 1
+                scores[r.index] = Score(r.prompt, logprob[at:at + n], entropy[at:at + n], best[at:at + n] if top else None)
+                at += n
+        self.engine.check_status()
+        return scores
+
+
+def generate(folder, prompts, dtype="bfloat16", max_tokens=None, cache=None, **options):
     """One call: load `folder` and generate for `prompts` (see LM.generate for the options)."""
-    return LM(folder, dtype=dtype, max_tokens=max_tokens).generate(prompts, **options)
+    return LM(folder, dtype=dtype, max_tokens=max_tokens, cache=cache).generate(prompts, **options)

@@ -16,6 +16,7 @@ from dataclasses import dataclass
 import torch
 
 from ..kernels import guards
+from . import kv8
 from .need import CacheNeed
 from .pages import CacheFull, FreeList, PageBook
 
@@ -39,13 +40,13 @@ class LayerKV:
 @dataclass
 class EntryView:
     owns_storage: bool  # False: the entry reads the cache of another entry
-    kv: object  # LayerKV or None
+    kv: object  # LayerKV (kv8.LayerKV8 in an 8-bit cache) or None
     state: object  # float32 [slots, *state_shape] or None
     states: dict = None  # further states by name, [slots, *shape] each
 
 
 class _Group:
-    def __init__(self, need, entries, n_pages, max_slots, max_context, dtype, device):
+    def __init__(self, need, entries, n_pages, max_slots, max_context, dtype, device, form=None):
         tpp = TOKENS_PER_PAGE
         self.need, self.entries = need, entries
         self.ring_pages = 0 if need.window is None else (need.window + tpp - 2) // tpp + 1
@@ -57,11 +58,23 @@ class _Group:
         self.table_width = max(1, min(per_seq, n_pages))
         self.book = PageBook(n_pages, tpp, self.ring_pages, self.pinned_pages)
         shape = (len(entries), n_pages, need.n_kv_heads, tpp, need.head_dim)
+        self.scales = self.open = None
+        if form is not None:  # keys and values in 8 bits
+            if (need.v_head_dim or need.head_dim) != need.head_dim or need.values_in_keys or self.pinned_pages or need.head_dim not in (64, 128):
+                raise ValueError(f"an 8-bit cache holds plain heads of 64 or 128, not {need}")
+            self.k, self.v, self.scales, self.open = kv8.pools(len(entries), n_pages, max_slots, need.n_kv_heads, need.head_dim, form, device)
+        else:
+            self._pools(shape, need, dtype, device)
+        self._tables(max_slots, device)
+
+    def _pools(self, shape, need, dtype, device):
         self.k = guards.zeros(shape, dtype, device, what="cache keys")  # guard words around the pools
         if need.values_in_keys:  # one pool: a value is the first v_head_dim elements of its key row
             self.v = self.k
         else:
             self.v = guards.zeros(shape[:-1] + (need.v_head_dim or need.head_dim,), dtype, device, what="cache values")
+
+    def _tables(self, max_slots, device):
         # the tables as the host has them; what changes goes to the device as arguments of a kernel (no copy from a host
         # buffer, which would have to be kept as it is, or waited for, while earlier steps are in flight)
         self.table_host = torch.zeros((max_slots, self.table_width), dtype=torch.int32)
@@ -95,11 +108,12 @@ _STATE_TYPES = {"float32": torch.float32, "int32": torch.int32}
 
 class SequenceCache:
     """needs: one CacheNeed (or None) per schedule entry; sources: per entry, None or the entry it reads.
-    frame_need: what the model's frame keeps per sequence (a CacheNeed with states only), or None."""
+    frame_need: what the model's frame keeps per sequence (a CacheNeed with states only), or None.
+    form: "int8" or "e4m3" for keys and values in 8 bits with scales (cache/kv8.py); None: in `dtype`."""
 
-    def __init__(self, needs, sources, max_tokens, dtype, device, max_slots=None, max_context=None, frame_need=None):
+    def __init__(self, needs, sources, max_tokens, dtype, device, max_slots=None, max_context=None, frame_need=None, form=None):
         tpp = TOKENS_PER_PAGE
-        self.device, self.dtype = torch.device(device), dtype
+        self.device, self.dtype, self.form = torch.device(device), dtype, form
         self.n_pages = max(1, -(-max_tokens // tpp))
         self.max_slots = max_slots or min(self.n_pages, 4096)
         self.max_context = min(max_context or self.n_pages * tpp, self.n_pages * tpp)
@@ -123,7 +137,7 @@ class SequenceCache:
         self.frame = EntryView(True, None, None, self._named(frame_need, "the frame") if frame_need is not None else {})
         for (hkv, hd, window, vd, keep_first, in_keys), entries in by_need.items():
             g = _Group(CacheNeed(hkv, hd, window, v_head_dim=vd, keep_first=keep_first, values_in_keys=in_keys), entries, self.n_pages,
-                       self.max_slots, self.max_context, dtype, self.device)
+                       self.max_slots, self.max_context, dtype, self.device, form)
             self.groups.append(g)
             for i, e in enumerate(entries):
                 self._of_entry[e] = (g, i)
@@ -144,8 +158,11 @@ class SequenceCache:
         kv = None
         if owner in self._of_entry:
             g, i = self._of_entry[owner]
-            kv = LayerKV(g.k[i], g.v[i], g.table, g.table_width, g.ring_pages, TOKENS_PER_PAGE, g.need.window,
-                         g.pinned_pages, g.need.values_in_keys)
+            if self.form is not None:
+                kv = kv8.LayerKV8(g.k[i], g.v[i], g.scales[i], g.open[i], g.table, g.table_width, g.ring_pages, g.need.window)
+            else:
+                kv = LayerKV(g.k[i], g.v[i], g.table, g.table_width, g.ring_pages, TOKENS_PER_PAGE, g.need.window,
+                             g.pinned_pages, g.need.values_in_keys)
         return EntryView(self.sources[e] is None, kv, self.states.get(owner), self.named_states.get(owner, {}))
 
     # ------------------------------------------------------------ slots
@@ -220,4 +237,5 @@ class SequenceCache:
 
     def bytes(self):
         total = sum((g.k.numel() + (0 if g.need.values_in_keys else g.v.numel())) * g.k.element_size() for g in self.groups)
+        total += sum(t.numel() * t.element_size() for g in self.groups for t in (g.scales, g.open) if t is not None)
         return total + sum(s.numel() * 4 for s in self._all_states())

@@ -4,9 +4,10 @@
 
 MODEL is a folder with config.json, *.safetensors and, for text, tokenizer.json (abacus takes the
 model.bin its converter makes of such a folder). Options keep abacus's names and meanings; -t and
---q4 have nothing to do here (GPU; no quantized weights) and say so. New: --fp32, --top-k, --batch.
+--q4 have nothing to do here (GPU; no quantized weights) and say so. New: --fp32, --top-k, --batch, --score, --kv8.
 """
 import json
+import math
 import sys
 import time
 
@@ -25,6 +26,8 @@ USAGE = """usage: abacus MODEL [options]
   --fp32           run everything in true 32-bit floating point (default: bfloat16)
   --top-k K        sample among the K most likely tokens (default 20, at most 64; 0: all tokens)
   --batch B        with --bench: B sequences at once (default 1)
+  --score TEXT     print how likely the text is (JSON); with --ids: the ids instead, TEXT may be empty
+  --kv8 FORM       keep keys and values in 8 bits, int8 or e4m3 (plain attention, bfloat16)
   -t N, --q4       abacus's CPU threads and 4-bit weights: not built here
 """
 
@@ -38,6 +41,7 @@ class Options:
         self.pp = self.tg = 0
         self.text = self.ids = self.dump = None
         self.start, self.chunk, self.top_k, self.batch = 1, 0, 20, 1
+        self.score = self.kv8 = None
 
 
 class UsageError(Exception):
@@ -95,6 +99,12 @@ def parse(argv):
             o.top_k = int(value())
         elif a == "--batch" and more:
             o.batch = int(value())
+        elif a == "--score" and more:
+            o.score = value()
+        elif a == "--kv8" and more:
+            o.kv8 = value()
+            if o.kv8 not in ("int8", "e4m3"):
+                raise UsageError(f"abacus: --kv8 {o.kv8}: the forms are int8 and e4m3\n")
         else:
             raise UsageError(USAGE)
         i += 1
@@ -163,7 +173,7 @@ def main(argv=None):
         return 1
     from .api import LM
     need = max(o.pp + o.tg + 64, 4096) * max(o.batch, 1) if (o.pp or o.tg) else None
-    lm = LM(o.model, dtype="float32" if o.fp32 else "bfloat16", max_tokens=need)
+    lm = LM(o.model, dtype="float32" if o.fp32 else "bfloat16", max_tokens=need, cache=o.kv8)
     if o.info:
         print(info_line(lm.model))
     elif o.text is not None:
@@ -173,6 +183,14 @@ def main(argv=None):
         print(" ".join(str(t) for t in lm.tokenizer.encode(o.text)))
     elif o.pp > 0 or o.tg > 0:
         print(json.dumps(bench(lm, o.pp, o.tg, o.batch)))
+    elif o.score is not None:
+        if o.ids is None and lm.tokenizer is None:
+            sys.stderr.write("abacus: this model folder has no tokenizer.json; use --ids\n")
+            return 1
+        s = lm.score([o.ids if o.ids is not None else lm.encode(o.score, raw=True)])[0]
+        n = max(len(s.logprobs), 1)
+        print(json.dumps({"tokens": len(s.tokens), "logprob": round(s.total, 4), "perplexity": round(math.exp(-s.total / n), 4),
+                          "mean_entropy": round(sum(s.entropies) / n, 4)}))
     elif o.ids is not None:
         if o.dump:
             dump_logits(lm, o.ids, o.start, o.chunk, o.dump)

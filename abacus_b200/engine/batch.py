@@ -94,6 +94,7 @@ class StepBatch:
         self.longest = 0  # tokens of the sequence that brings most
         self.is_decode = False
         self.any_continuation = False
+        self.scoring = None  # a step that scores: where its numbers go (engine.engine.Scoring)
         self._sent, self._sent_on = None, set()
 
     def fill(self, sequences, pad_logits=False, exact=False):

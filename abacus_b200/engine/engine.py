@@ -7,12 +7,13 @@ sequence. This is abacus's forward(tokens, n, pos, logits, n_logits)
 (src/model.c:315-327) for a batch of sequences instead of one.
 """
 import os
+from dataclasses import dataclass
 
 import numpy as np
 
 import torch
 
-from ..cache import SequenceCache
+from ..cache import TOKENS_PER_PAGE, SequenceCache
 from ..config.registry import load_config
 from ..models.model import Model
 from ..weights.loader import load_folder
@@ -50,6 +51,17 @@ def load_model(folder, dtype="bfloat16", device=None):
     return model
 
 
+@dataclass
+class Scoring:
+    """Where a step that scores leaves its numbers, for its wanted rows in order (ops.token_logprobs says what they are)."""
+    tokens: torch.Tensor      # int32: the token whose log probability is wanted (-1: none)
+    logprob: torch.Tensor     # float32
+    entropy: torch.Tensor     # float32
+    top_ids: torch.Tensor = None       # int32 [rows, k], or None
+    top_logprobs: torch.Tensor = None  # float32 [rows, k]
+    done: bool = False        # the model's frame has seen to it
+
+
 _ONE_TOKEN, _WANT_IT = np.zeros(1, dtype=np.int64), [0]
 
 
@@ -70,30 +82,51 @@ def capturable(model):
 
 
 class Engine:
-    def __init__(self, model, max_tokens, max_slots=None, max_context=None, use_graphs=True):
+    def __init__(self, model, max_tokens, max_slots=None, max_context=None, use_graphs=True, cache=None):
+        """cache: "int8" or "e4m3" keeps keys and values in 8 bits with scales (cache/kv8.py; models whose mixers are all plain attention
+        in bfloat16, heads of 64 or 128): half the bytes a token. None: in the model's type."""
         self.model = model
+        if cache is not None:
+            self._check_kv8(model, cache)
         spec = model.spec
         context = min(max_context or spec.max_positions, spec.max_positions)
         self.cache = SequenceCache(model.cache_needs(), model.cache_sources(), max_tokens, model.ctx.dtype,
                                    model.ctx.device, max_slots=max_slots, max_context=context,
-                                   frame_need=model.frame_need())
+                                   frame_need=model.frame_need(), form=cache)
         self.max_context = self.cache.max_context
         model.prepare(self.max_context)
         self.vocab = spec.vocab
         # the step function in C where the model is made of the library's own parts, else the parts' forward()
-        self.cstep = CStep(model, self.cache) if CStep.serves(model) else None
+        self.cstep = CStep(model, self.cache) if cache is None and CStep.serves(model) else None
         decode_graphs, prompt_graphs = capturable(model)
+        if cache is not None and prompt_graphs:  # a sequence that goes on has its pages counted on the host
+            prompt_graphs = "from_start"
         self.graphs = DecodeGraphs(self) if use_graphs and decode_graphs else None
         prompts = use_graphs and prompt_graphs and os.environ.get("ABACUS_PROMPT_GRAPHS", "1") != "0"
         self.prompt_graphs = PromptGraphs(self, from_start_only=prompt_graphs == "from_start") if prompts else None
         self._step_batch = None
         self._graph_memory = None
 
+    @staticmethod
+    def _check_kv8(model, form):
+        from ..cache.kv8 import FORMS
+        from ..parts.attention import Attention
+        if form not in FORMS:
+            raise ValueError(f"cache {form!r}: keys and values are kept in the model's type (None) or as {' or '.join(FORMS)}")
+        plain = all(type(b.mixer) is Attention and not b.mixer.general and b.mixer.spec.head_dim in (64, 128) for b in model.blocks)
+        if not plain or model.ctx.dtype != torch.bfloat16:
+            raise ValueError("an 8-bit cache serves bfloat16 models whose mixers are all plain attention with heads of 64 or 128")
+
     def graph_memory(self):
         """The memory pool of the engine's captured steps, by its id."""
         if self._graph_memory is None:
             self._graph_memory = torch.cuda.MemPool()
         return self._graph_memory.id
+
+    @property
+    def cache_tokens(self):
+        """Tokens the cache has room for."""
+        return self.cache.n_pages * TOKENS_PER_PAGE
 
     # ------------------------------------------------------------ sequences
     def open(self):
@@ -147,6 +180,35 @@ class Engine:
         for s in seqs:
             self.cache.advance(s.slot, len(s.tokens))
         return logits
+
+    def score(self, entries, tokens, top=0):
+        """A step (see step) that gives, for every wanted row, the log probability of the given token, the entropy and the `top` most
+        likely tokens instead of logits, which are not kept. tokens: a token a wanted row, in the order of the entries and of each
+        entry's `want` (-1: none). Returns (logprob, entropy, top_ids, top_logprobs) on the device, the last two None for top=0."""
+        rows = sum(len(want) for _, _, want in entries)
+        if len(tokens) != rows:
+            raise StepError(f"{len(tokens)} tokens to score at {rows} wanted places")
+        if not 0 <= top <= min(64, self.vocab):
+            raise StepError(f"{top} most likely tokens: 0 to {min(64, self.vocab)} can be had")
+        seqs = self.plan(entries)
+        device = self.model.ctx.device
+        batch = self._room_for(sum(len(s.tokens) for s in seqs), len(seqs), rows)
+        batch.fill(seqs, exact=True)
+        number = lambda *shape: torch.empty(shape, dtype=torch.float32, device=device)
+        given = torch.tensor(list(tokens), dtype=torch.int32).to(device)
+        batch.scoring = Scoring(given, number(rows), number(rows), torch.empty((rows, top), dtype=torch.int32, device=device) if top else None,
+                                number(rows, top) if top else None)
+        try:
+            self.model.forward(batch, self.cache)
+            scoring = batch.scoring
+        finally:
+            batch.scoring = None
+        if not scoring.done:
+            raise StepError(f"the model's frame {self.model.spec.frame!r} makes logits of its own and cannot score")
+        self.last_batch = batch
+        for s in seqs:
+            self.cache.advance(s.slot, len(s.tokens))
+        return scoring.logprob, scoring.entropy, scoring.top_ids, scoring.top_logprobs
 
     def forward(self, batch):
         """The model's forward pass over a filled step: in one call to C where that serves the model."""

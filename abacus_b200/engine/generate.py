@@ -29,6 +29,8 @@ class Request:
     max_new_tokens: int
     output: list = field(default_factory=list)
     finish_reason: str = ""  # "stop", "length" or "context"
+    logprobs: list = field(default_factory=list)  # of the output's tokens, where they were asked for
+    top: list = field(default_factory=list)       # [(token, log probability)] of the most likely ones in each one's place
     slot: int = -1
 
 
@@ -106,10 +108,12 @@ class Generator:
     """Runs requests through an engine. `engine` needs open(), close(slot), step(entries) -> logits,
     max_context and a cache with n_pages and max_slots; `sampler` needs states() and sample()."""
 
-    def __init__(self, engine, sampler, stop_tokens=(), on_token=None):
+    def __init__(self, engine, sampler, stop_tokens=(), on_token=None, logprobs=None):
         """on_token(request, token): called for every token a request keeps, as soon as the host has it (the chat
-        loop prints each piece as it comes, src/main.c:177-180)."""
+        loop prints each piece as it comes, src/main.c:177-180). logprobs: None, or how many most likely tokens a request keeps beside each of
+        its own and its log probability."""
         self.engine, self.sampler, self.stop_tokens, self.on_token = engine, sampler, tuple(stop_tokens), on_token
+        self.logprobs = logprobs
         self.stats = {"prefill_steps": 0, "decode_steps": 0, "batches": 0}
         self.rng = None
 
@@ -156,6 +160,16 @@ class Generator:
             return self._landing[:n].tolist()
         return read
 
+    def _score(self, logits, drawn):
+        """The drawn tokens' log probabilities and the most likely tokens (launched at once: a step that runs ahead takes the logits'
+        place). Returns a function that gives them, [(log probability, [(token, log probability)])] by row."""
+        from ..kernels import ops
+        n, k, device = drawn.numel(), self.logprobs, logits.device
+        logprob = torch.empty(n, dtype=torch.float32, device=device)
+        ids, values = torch.empty((n, k), dtype=torch.int32, device=device), torch.empty((n, k), dtype=torch.float32, device=device)
+        ops.token_logprobs(logits, drawn, logprob, top_ids=ids if k else None, top_logprobs=values if k else None, n_rows=n)
+        return lambda: [(p, list(zip(i, v))) for p, i, v in zip(logprob.tolist(), ids.tolist(), values.tolist())]
+
     def run_batch(self, batch):
         engine = self.engine
         for r in batch:
@@ -174,6 +188,7 @@ class Generator:
             while True:
                 rows = list(live.live)
                 drawn = self.sampler.sample(logits, self.rng, index=index)
+                scored = self._score(logits, drawn) if self.logprobs is not None else None
                 ahead = None
                 if self._may_run_ahead(rows, engine, live.max_context):
                     read = self._read_beside(drawn)
@@ -186,6 +201,11 @@ class Generator:
                 self.stats["t_end"] = now
                 kept = [len(r.output) for r in rows]
                 finished, entries = live.take(sampled)
+                if scored is not None:
+                    for r, n, (logprob, top) in zip(rows, kept, scored()):
+                        if len(r.output) > n:
+                            r.logprobs.append(logprob)
+                            r.top.append(top)
                 if self.on_token is not None:
                     for r, n in zip(rows, kept):
                         for token in r.output[n:]:

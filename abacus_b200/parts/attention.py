@@ -17,6 +17,8 @@ import os
 
 import torch
 
+from ..cache.kv import LayerKV
+from ..cache.kv8 import LayerKV8
 from ..cache.need import CacheNeed
 from ..kernels import ops
 from .attention_plan import AttentionLists, AttentionStepPlan
@@ -27,6 +29,9 @@ from .linear import Linear
 # A decode step's attention kernel can norm and rotate q and k and write the new key and value to the cache itself: a
 # launch less in every layer. ABACUS_DECODE_PREPARES=0 keeps the preparation a kernel of its own (for comparison).
 DECODE_PREPARES = os.environ.get("ABACUS_DECODE_PREPARES", "1") != "0"
+# Tokens a sequence brings up to which a step that goes on with it attends to an 8-bit cache row by row, each row reading all its keys;
+# beyond that the sequences' keys and values are read back into 16-bit pages first, for the prompt kernel.
+KV8_ROWS_UP_TO = 8
 # The q/k/v product of a long prompt step can do the same in its epilogue (heads of 128): a kernel and a pass over
 # q, k and v less. ABACUS_PRODUCT_PREPARES=0 keeps the preparation a kernel of its own (for comparison).
 PRODUCT_PREPARES = os.environ.get("ABACUS_PRODUCT_PREPARES", "1") != "0"
@@ -175,7 +180,63 @@ class Attention:
         if self.position is not None:
             self.cos, self.sin = self.position.tables(max_positions, device)
 
+    def forward_kv8(self, xn, out, batch, cache, ws):
+        """The same over an 8-bit cache: whole prompts attend to their own keys as they came, everything else to what the cache
+        holds (cache/kv8.py)."""
+        s, n, writes = self.spec, batch.n_rows, cache.owns_storage
+        if self.general or self.ctx.dtype != torch.bfloat16:
+            raise ops.KernelRefused("an 8-bit cache serves plain attention in bfloat16")
+        qkv = ws.get("qkv", (n, self.row), self.ctx.dtype)
+        att = ws.get("att", (n, s.n_heads * self.v_dim), self.ctx.dtype)
+        (self.qkv_proj if writes else self.q_proj).forward(xn, qkv if writes else qkv[:, :self.q_size], n)
+        rotary_dim = self.position.rotary_dim if self.position else 0
+        ops.qkv_prep(qkv, s.n_heads, s.n_kv_heads, s.head_dim, batch, self.q_norm, self.k_norm, s.qk_norm_eps, self.cos, self.sin, rotary_dim,
+                     self.position.interleaved if self.position else False, None, q_only=not writes)
+        if writes:
+            ops.kv8_write(qkv, s.n_heads, s.n_kv_heads, s.head_dim, batch, cache.kv)
+        heads = (s.n_heads, s.n_kv_heads, s.head_dim, s.scale)
+        if writes and not batch.is_decode and not batch.any_continuation:
+            if ops.attention_window_takes(qkv, s.head_dim, s.head_dim, s.n_heads, s.n_kv_heads):
+                ops.attention_window(qkv, att, *heads, s.window, batch)
+            else:
+                ops.attention_generic(qkv, att, *heads, s.window, batch, None, from_step=True)
+        elif s.window is not None and not batch.is_decode:
+            raise ops.KernelRefused("windowed attention takes several tokens of a sequence only at its start, "
+                                    "and only with keys of its own")
+        elif batch.longest <= KV8_ROWS_UP_TO or batch.plan.get(self.lists.name) is None:
+            ops.attention_kv8(qkv, att, *heads, s.window, batch, cache.kv, ws)
+        else:
+            first_page, pages = self._kv8_pages(batch, cache.kv, ws)
+            ops.kv8_read(cache.kv, batch, first_page, pages.k, pages.v)
+            ops.attention_prefill(qkv, att, *heads, batch, pages, AttentionLists(batch.plan[self.lists.name]))
+        self.o_proj.forward(att, out, n)
+        return out
+
+    @staticmethod
+    def _kv8_pages(batch, kv, ws):
+        """Where an 8-bit cache's sequences are read back to, made once a step for all layers with the same heads: their first pages,
+        and the pages as a 16-bit cache with a table of its own (a row a slot)."""
+        key = (kv.n_kv_heads, kv.head_dim, kv.n_slots)
+        made = batch.__dict__.setdefault("kv8_pages", {})
+        if made.get("step") is not batch.sequences:
+            made.clear()
+            made["step"] = batch.sequences
+        if key not in made:
+            counts = [-(-(s.start + len(s.tokens)) // kv.tokens_per_page) for s in batch.sequences]
+            first = [sum(counts[:i]) for i in range(len(counts) + 1)]
+            table = torch.zeros((kv.n_slots, max(counts)), dtype=torch.int32)
+            for s, at, count in zip(batch.sequences, first, counts):
+                table[s.slot, :count] = torch.arange(at, at + count, dtype=torch.int32)
+            device = batch.seq_slot.device
+            shape = (first[-1], kv.n_kv_heads, kv.tokens_per_page, kv.head_dim)
+            k, v = (ws.get(f"kv8_{name}", shape, torch.bfloat16) for name in ("keys", "values"))
+            made[key] = (torch.tensor(first + first[-1:] * (batch.seq_slot.numel() - len(counts)), dtype=torch.int32).to(device),
+                         LayerKV(k, v, table.to(device), table.shape[1], 0, kv.tokens_per_page, None))
+        return made[key]
+
     def forward(self, xn, out, batch, cache, ws):
+        if isinstance(cache.kv, LayerKV8):
+            return self.forward_kv8(xn, out, batch, cache, ws)
         s = self.spec
         n = batch.n_rows
         qkv = ws.get("qkv", (n, self.row), self.ctx.dtype)

@@ -10,7 +10,8 @@ A frame has
   param_shapes(tied) -> {slot: shape}     slots "embed", "final_norm", and "head" unless tied
   bind(params, ctx)
   embed(batch, ws, status) -> x           float32 [rows, hidden], the residual stream
-  logits(x, y, batch, ws) -> float32 [batch.n_logit_rows, vocab]
+  logits(x, y, batch, ws) -> float32 [batch.n_logit_rows, vocab], or nothing of them for a step that scores (batch.scoring):
+                                          `end` does either behind the frame's last norm
   step_weights() -> tensors a step reads once whatever its size
 """
 import torch
@@ -19,6 +20,39 @@ from ..kernels import ops
 from .base import FRAMES, NORMS, to_device
 from .linear import Linear
 from .position import Sinusoids
+
+
+LOGIT_ROWS = 512  # rows whose logits a step that scores keeps at a time, where it needs them
+
+
+def end(frame, batch, ws, norm):
+    """The end of a frame: norm(xn, rows, r) puts the wanted rows into xn, and the output matrix makes their logits of them. A step
+    that scores (batch.scoring, engine.Scoring) leaves the given tokens' log probabilities there instead: by the product that
+    keeps no logits where that takes the matrix and no other tokens are asked for, else from some rows' logits at a time."""
+    r, scoring = batch.n_logit_rows, batch.scoring
+    if scoring is None:
+        out = ws.get("logits", (max(r, 1), frame.vocab), torch.float32)[:r]
+    else:
+        out = ws.get("logits", (1, frame.vocab), torch.float32)[:0]
+        scoring.done = True
+    if not r:
+        return out
+    xn = ws.get("xn_final", (r, frame.hidden), frame.ctx.dtype)
+    norm(xn, batch.logit_rows, r)
+    if scoring is None:
+        frame.head.forward(xn, out, r)
+    elif scoring.top_ids is None and ops.gemm_tc_logprobs_takes(xn, frame.head.weight):
+        ops.gemm_tc_logprobs(xn, frame.head.weight, scoring.tokens, scoring.logprob, scoring.entropy, ws, r)
+    else:
+        part = ws.get("logits", (min(r, LOGIT_ROWS), frame.vocab), torch.float32)
+        for lo in range(0, r, LOGIT_ROWS):
+            rows = slice(lo, min(r, lo + LOGIT_ROWS))
+            n = rows.stop - lo
+            frame.head.forward(xn[rows], part[:n], n)
+            ops.token_logprobs(part[:n], scoring.tokens[rows], scoring.logprob[rows], entropy=scoring.entropy[rows],
+                               top_ids=scoring.top_ids[rows] if scoring.top_ids is not None else None,
+                               top_logprobs=scoring.top_logprobs[rows] if scoring.top_ids is not None else None)
+    return out
 
 
 @FRAMES.register("plain")
@@ -53,13 +87,7 @@ class PlainFrame:
         return x
 
     def logits(self, x, y, batch, ws):
-        r = batch.n_logit_rows
-        out = ws.get("logits", (max(r, 1), self.vocab), torch.float32)[:r]
-        if r:
-            xn = ws.get("xn_final", (r, self.hidden), self.ctx.dtype)
-            self.final_norm.forward(x, y, xn, rows=batch.logit_rows, n_rows=r)
-            self.head.forward(xn, out, r)
-        return out
+        return end(self, batch, ws, lambda xn, rows, r: self.final_norm.forward(x, y, xn, rows=rows, n_rows=r))
 
 
 @FRAMES.register("scaled_pairs")
@@ -111,13 +139,7 @@ class PairsFrame:
 
     def logits(self, x, pending, batch, ws):
         from .streams import read_streams
-        r = batch.n_logit_rows
-        out = ws.get("logits", (max(r, 1), self.vocab), torch.float32)[:r]
-        if r:
-            xn = ws.get("xn_final", (r, self.hidden), self.ctx.dtype)
-            read_streams(x, pending, self.ones, self.final_norm, xn, rows=batch.logit_rows, n_rows=r)
-            self.head.forward(xn, out, r)
-        return out
+        return end(self, batch, ws, lambda xn, rows, r: read_streams(x, pending, self.ones, self.final_norm, xn, rows=rows, n_rows=r))
 
 
 @FRAMES.register("positions")
@@ -168,13 +190,7 @@ class PositionsFrame:
 
     def logits(self, x, pending, batch, ws):
         from .streams import read_streams
-        r = batch.n_logit_rows
-        out = ws.get("logits", (max(r, 1), self.vocab), torch.float32)[:r]
-        if r:
-            xn = ws.get("xn_final", (r, self.hidden), self.ctx.dtype)
-            read_streams(x, pending, self.ones, self.final_norm, xn, rows=batch.logit_rows, n_rows=r)
-            self.head.forward(xn, out, r)
-        return out
+        return end(self, batch, ws, lambda xn, rows, r: read_streams(x, pending, self.ones, self.final_norm, xn, rows=rows, n_rows=r))
 
 
 @FRAMES.register("loop_input")
@@ -238,13 +254,7 @@ class LoopInputFrame:
 
     def logits(self, x, pending, batch, ws):
         from .streams import read_streams
-        r = batch.n_logit_rows
-        out = ws.get("logits", (max(r, 1), self.vocab), torch.float32)[:r]
-        if r:
-            xn = ws.get("xn_final", (r, self.hidden), self.ctx.dtype)
-            read_streams(x, pending, self.ones, self.final_norm, xn, rows=batch.logit_rows, n_rows=r)
-            self.head.forward(xn, out, r)
-        return out
+        return end(self, batch, ws, lambda xn, rows, r: read_streams(x, pending, self.ones, self.final_norm, xn, rows=rows, n_rows=r))
 
 
 class NormedEndFrame(PlainFrame):
@@ -256,13 +266,7 @@ class NormedEndFrame(PlainFrame):
         self.options = spec.frame_spec
 
     def logits(self, x, pending, batch, ws):
-        r = batch.n_logit_rows
-        out = ws.get("logits", (max(r, 1), self.vocab), torch.float32)[:r]
-        if r:
-            xn = ws.get("xn_final", (r, self.hidden), self.ctx.dtype)
-            self.final_norm.forward_normed(x, pending, xn, rows=batch.logit_rows, n_rows=r)
-            self.head.forward(xn, out, r)
-        return out
+        return end(self, batch, ws, lambda xn, rows, r: self.final_norm.forward_normed(x, pending, xn, rows=rows, n_rows=r))
 
 
 @FRAMES.register("scaled")
