@@ -11,6 +11,12 @@
 // accumulator of its own, and the reading threads add them up, in registers, while the tensor cores are on the next one.
 // A second kernel joins the pairs' sums, a warp a row. The eight warps that read need 5.5 instructions and one exponential a logit:
 // at K = 1,024 half of the time that the tensor cores take for it.
+//
+// Few rows (up to LP_FEW): w is all there is to read, and a tile of 256 rows of x of which a few are there costs the tensor cores as much
+// time as w takes to come. So the operands change sides: a CTA's tile is up to 128 rows of w, the rows of x are its 16 to 64 columns, and
+// a thread that reads the accumulator has one token of the vocabulary and keeps the sums of 32 rows of x in registers over all of its
+// CTA's tiles. The tiles are as high as makes all CTAs take the same number of full ones (115 for 151,936 on 148 SMs). 37 rows of 1,024
+// against 151,936: 64 us, with the tiles above 83 (the matrix at the copy rate: 48).
 #define ABK_DEFINE_ERROR
 #include "common.cuh"
 #include "tc_common.cuh"
@@ -253,6 +259,166 @@ __global__ void __launch_bounds__(LP_THREADS) gemm_logprobs_kernel(const __grid_
     }
 }
 
+// ------------------------------------------------------------------ few rows
+#define LP_FEW 64
+#define LP_FEW_STAGES 8
+#define LP_FEW_SMEM (LP_FEW_STAGES * (LP_A_BYTES + LP_FEW * LP_K * 2) + 1024 /* alignment */ + 256 /* barriers */)
+
+struct FewLogProbs {
+    int rows, columns, vocab, high, tiles, k_blocks, segment_blocks, segments;  // columns: the rows of x, up to a multiple of 16; high: rows of w a tile
+    const int *tokens;
+    float *given;
+    float4 *parts;  // [CTAs][rows]
+    int *status;
+};
+
+__global__ void __launch_bounds__(LP_THREADS) gemm_logprobs_few_kernel(const __grid_constant__ CUtensorMap map_w,
+                                                                       const __grid_constant__ CUtensorMap map_x, FewLogProbs g) {
+    extern __shared__ uint8_t lp_raw[];
+    uint8_t *smem = (uint8_t *)(((uintptr_t)lp_raw + 1023) & ~(uintptr_t)1023);
+    const int b_bytes = g.columns * LP_K * 2;
+    uint8_t *a_tiles = smem, *b_tiles = smem + LP_FEW_STAGES * LP_A_BYTES;
+    uint64_t *full = (uint64_t *)(b_tiles + LP_FEW_STAGES * LP_FEW * LP_K * 2);
+    uint64_t *empty = full + LP_FEW_STAGES, *acc_full = empty + LP_FEW_STAGES, *acc_empty = acc_full + 2;
+    uint32_t *tmem_holder = (uint32_t *)(acc_empty + 2);
+    volatile int *flags = (volatile int *)(tmem_holder + 1);  // [0]: a wait ran out
+    __shared__ int token_s[LP_FEW];
+    __shared__ float4 sums_s[4][LP_FEW];
+    constexpr uint32_t TMEM_COLS = 2 * LP_FEW;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < LP_FEW_STAGES; s++) tc::mbar_init(&full[s], 1), tc::mbar_init(&empty[s], 1);
+        for (int b = 0; b < 2; b++) tc::mbar_init(&acc_full[b], 1), tc::mbar_init(&acc_empty[b], 8);
+        flags[0] = 0;
+        tc::mbar_init_fence();
+        tc::tma_prefetch_map(&map_x), tc::tma_prefetch_map(&map_w);
+    }
+    if (warp == 1) tc::tmem_alloc(tmem_holder, TMEM_COLS);
+    pdl_wait();
+    if (threadIdx.x < g.rows) token_s[threadIdx.x] = g.tokens[threadIdx.x];
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = *tmem_holder;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int issued = 0;
+            for (int t = blockIdx.x; t < g.tiles && !flags[0]; t += gridDim.x) {
+                for (int kb = 0; kb < g.k_blocks; kb++, issued++) {
+                    const int s = issued % LP_FEW_STAGES;
+                    if (!tc::mbar_wait(&empty[s], ((issued / LP_FEW_STAGES) & 1) ^ 1)) {
+                        flags[0] = 1;
+                        break;
+                    }
+                    tc::mbar_expect_tx(&full[s], g.high * LP_K * 2 + b_bytes);
+                    tc::tma_load_2d(a_tiles + s * LP_A_BYTES, &map_w, kb * LP_K, t * g.high, &full[s]);
+                    tc::tma_load_2d(b_tiles + s * b_bytes, &map_x, kb * LP_K, 0, &full[s]);
+                }
+            }
+            if (flags[0])  // let the copies still in flight land before the CTA's memory goes away
+                for (int i = max(0, issued - LP_FEW_STAGES); i < issued; i++) tc::mbar_wait(&full[i % LP_FEW_STAGES], (i / LP_FEW_STAGES) & 1);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const uint32_t idesc = tc::idesc_bf16_f32(LP_ROWS, g.columns);
+            int done = 0, it = 0;
+            for (int t = blockIdx.x; t < g.tiles && !flags[0]; t += gridDim.x) {
+                for (int kb = 0; kb < g.k_blocks && !flags[0]; it++) {
+                    const int b = it & 1, kb_end = min(kb + g.segment_blocks, g.k_blocks);
+                    if (!tc::mbar_wait(&acc_empty[b], ((it >> 1) & 1) ^ 1)) {
+                        flags[0] = 1;
+                        break;
+                    }
+                    tc::fence_after_sync();
+                    for (bool more = false; kb < kb_end; kb++, done++) {
+                        const int s = done % LP_FEW_STAGES;
+                        if (!tc::mbar_wait(&full[s], (done / LP_FEW_STAGES) & 1)) {
+                            flags[0] = 1;
+                            break;
+                        }
+                        tc::fence_after_sync();
+                        const uint32_t a = tc::smem_addr(a_tiles + s * LP_A_BYTES), bq = tc::smem_addr(b_tiles + s * b_bytes);
+#pragma unroll
+                        for (int k = 0; k < LP_K / 16; k++, more = true)
+                            tc::mma_ss(tmem + b * LP_FEW, tc::smem_desc_k_sw128(a + k * 32), tc::smem_desc_k_sw128(bq + k * 32), idesc, more);
+                        tc::mma_commit(&empty[s]);
+                    }
+                    if (!flags[0]) tc::mma_commit(&acc_full[b]);
+                }
+            }
+        }
+    } else {
+        // warp w reads lanes 32 * (w % 4) .. + 31 of the accumulator, tokens of the vocabulary, and 32 of the rows of x
+        constexpr int COLS = LP_FEW / 2;
+        const int quarter = warp & 3, half = (warp - 2) >> 2, col0 = half * COLS;
+        float m[COLS], l[COLS], tt[COLS];
+#pragma unroll
+        for (int j = 0; j < COLS; j++) m[j] = -3.402823466e38f, l[j] = 0.0f, tt[j] = 0.0f;
+        bool ok = true;
+        int it = 0;
+        for (int t = blockIdx.x; t < g.tiles && ok; t += gridDim.x) {
+            const int in_tile = quarter * 32 + lane, token = t * g.high + in_tile;
+            const bool mine = in_tile < g.high && token < g.vocab;
+            float sum[COLS];
+            for (int segment = 0; segment < g.segments; segment++, it++) {
+                const int b = it & 1;
+                ok = __all_sync(0xffffffffu, !flags[0] && tc::mbar_wait(&acc_full[b], (it >> 1) & 1));
+                if (!ok) {
+                    flags[0] = 1;
+                    break;
+                }
+                tc::fence_after_sync();
+#pragma unroll
+                for (int c0 = 0; c0 < COLS; c0 += 16) {
+                    if (col0 + c0 >= g.columns) continue;
+                    uint32_t w[16];
+                    tc::tmem_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + b * LP_FEW + col0 + c0, w);
+                    tc::tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 16; j++) sum[c0 + j] = segment ? sum[c0 + j] + __uint_as_float(w[j]) : __uint_as_float(w[j]);
+                }
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&acc_empty[b]);
+            }
+            if (ok && mine) {
+#pragma unroll
+                for (int j = 0; j < COLS; j++) {
+                    if (col0 + j >= g.rows) continue;
+                    const float v = sum[j], n = fmaxf(m[j], v), dm = m[j] - n, dv = v - n;
+                    const float a = ex2(dm * 1.4426950408889634f), e = ex2(dv * 1.4426950408889634f);
+                    tt[j] = fmaf(a, fmaf(l[j], dm, tt[j]), e * dv);
+                    l[j] = fmaf(l[j], a, e), m[j] = n;
+                    if (token_s[col0 + j] == token) g.given[col0 + j] = v;
+                }
+            }
+            __syncwarp();
+        }
+#pragma unroll
+        for (int j = 0; j < COLS; j++) {
+            if (col0 + j >= g.rows) continue;
+            const RowSums s = joined_lanes({m[j], l[j], tt[j], 0.0f}, 16);
+            if (lane == 0) sums_s[quarter][col0 + j] = make_float4(s.m, s.l, s.t, 0.0f);
+        }
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    if (threadIdx.x < g.rows) {
+        RowSums s = {-3.402823466e38f, 0.0f, 0.0f, 0.0f};
+        for (int q = 0; q < 4; q++) {
+            const float4 x = sums_s[q][threadIdx.x];
+            s = joined(s, {x.x, x.y, x.z, 0.0f});
+        }
+        g.parts[(long long)blockIdx.x * g.rows + threadIdx.x] = make_float4(s.m, s.l, s.t, 0.0f);
+    }
+    if (flags[0] && threadIdx.x == 0) atomicOr(g.status + 1, 1);
+    if (warp == 1) {
+        tc::fence_after_sync();
+        tc::tmem_free(tmem, TMEM_COLS);
+    }
+}
+
 // A warp a row: the pairs' sums joined.
 __global__ void __launch_bounds__(128) logprobs_join_kernel(const float4 *__restrict__ parts, int pairs, int rows, int vocab,
                                                             const int *__restrict__ tokens, const float *__restrict__ given,
@@ -273,7 +439,7 @@ __global__ void __launch_bounds__(128) logprobs_join_kernel(const float4 *__rest
     if (lane == 0) {
         const int token = tokens[row];
         const float log_l = logf(s.l), nan = __int_as_float(0x7fffffff);
-        const bool none = !(s.l > 0.0f);  // (a NaN or an infinity among the logits)
+        const bool none = !(s.l > 0.0f) || !(s.t == s.t);  // (a NaN or an infinity among the logits)
         logprob[row] = none || token < 0 || token >= vocab ? nan : given[row] - s.m - log_l;
         if (entropy) entropy[row] = none ? nan : log_l - s.t / s.l;
     }
@@ -282,7 +448,7 @@ __global__ void __launch_bounds__(128) logprobs_join_kernel(const float4 *__rest
 // Floats of memory for the sums of `rows` rows: 4 a row and pair of CTAs, and the given tokens' logits.
 extern "C" long long abk_gemm_logprobs_floats(int rows) {
     const long long most = rows < LP_MOST_ROWS ? rows : LP_MOST_ROWS;
-    return most * (4 * (abk_sm_count() / 2) + 1) + 4;
+    return most * (4 * (rows <= LP_FEW ? abk_sm_count() : abk_sm_count() / 2) + 1) + 4;
 }
 extern "C" int abk_gemm_logprobs(const void *x, const void *w, int M, int V, int K, long long ldx, long long ldw, const int *tokens,
                                  float *logprob, float *entropy, float *memory, long long floats, int *status, void *stream) {
@@ -291,7 +457,31 @@ extern "C" int abk_gemm_logprobs(const void *x, const void *w, int M, int V, int
     if (((uintptr_t)x & 15) || ((uintptr_t)w & 15) || ldx % 8 || ldw % 8 || ((uintptr_t)memory & 15))
         ABK_REFUSE("gemm_logprobs: operands must be 16-byte aligned with pitches of a multiple of 8");
     if (floats < abk_gemm_logprobs_floats(M)) ABK_REFUSE("gemm_logprobs: room for %lld floats is too little", floats);
-    auto kernel = (K + LP_K - 1) / LP_K > LP_SEGMENT ? gemm_logprobs_kernel<true> : gemm_logprobs_kernel<false>;
+    const int k_blocks = (K + LP_K - 1) / LP_K, pieces = (k_blocks + LP_SEGMENT - 1) / LP_SEGMENT;  // segments as equal as whole blocks allow
+    const int segment_blocks = (k_blocks + pieces - 1) / pieces, segments = (k_blocks + segment_blocks - 1) / segment_blocks;
+    if (M <= LP_FEW) {
+        const int ctas = abk_sm_count();
+        FewLogProbs g;
+        const long long waves = (V + (long long)ctas * LP_ROWS - 1) / ((long long)ctas * LP_ROWS);
+        g.high = (int)((V + waves * ctas - 1) / (waves * ctas));
+        if (g.high < 16) g.high = 16;
+        g.rows = M, g.columns = (M + 15) / 16 * 16, g.vocab = V, g.tiles = (V + g.high - 1) / g.high;
+        g.k_blocks = k_blocks, g.segment_blocks = segment_blocks, g.segments = segments, g.tokens = tokens, g.status = status;
+        const int grid = g.tiles < ctas ? g.tiles : ctas;
+        g.parts = (float4 *)memory, g.given = memory + 4ll * grid * M;
+        CUtensorMap mx, mw;
+        int rc = tmap::bf16_rows_of_128_bytes(x, M, K, ldx, g.columns, &mx);
+        if (!rc) rc = tmap::bf16_rows_of_128_bytes(w, V, K, ldw, g.high, &mw);
+        if (rc) return rc;
+        if (cudaError_t e = abk_allow_shared_memory((const void *)gemm_logprobs_few_kernel, LP_FEW_SMEM)) return (int)e;
+        abk_launch(gemm_logprobs_few_kernel, dim3(grid), dim3(LP_THREADS), LP_FEW_SMEM, (cudaStream_t)stream, mw, mx, g);
+        rc = ABK_LAUNCH_RESULT();
+        if (rc) return rc;
+        abk_launch(logprobs_join_kernel, dim3((M + 3) / 4), dim3(128), 0, (cudaStream_t)stream, (const float4 *)g.parts, grid, M, V, tokens,
+                   (const float *)g.given, logprob, entropy);
+        return ABK_LAUNCH_RESULT();
+    }
+    auto kernel = k_blocks > LP_SEGMENT ? gemm_logprobs_kernel<true> : gemm_logprobs_kernel<false>;
     if (cudaError_t e = abk_allow_shared_memory((const void *)kernel, LP_SMEM)) return (int)e;
     for (int first = 0; first < M; first += LP_MOST_ROWS) {
         const int rows = M - first < LP_MOST_ROWS ? M - first : LP_MOST_ROWS;
@@ -300,9 +490,7 @@ extern "C" int abk_gemm_logprobs(const void *x, const void *w, int M, int V, int
         if (!rc) rc = tmap::bf16_rows_of_128_bytes(w, V, K, ldw, LP_COLS / 2, &mw);
         if (rc) return rc;
         GemmLogProbs g;
-        g.rows = rows, g.vocab = V, g.k_blocks = (K + LP_K - 1) / LP_K, g.m_tiles = (rows + 2 * LP_ROWS - 1) / (2 * LP_ROWS);
-        const int parts = (g.k_blocks + LP_SEGMENT - 1) / LP_SEGMENT;  // segments as equal as whole blocks allow
-        g.segment_blocks = (g.k_blocks + parts - 1) / parts, g.segments = (g.k_blocks + g.segment_blocks - 1) / g.segment_blocks;
+        g.rows = rows, g.vocab = V, g.k_blocks = k_blocks, g.segment_blocks = segment_blocks, g.segments = segments, g.m_tiles = (rows + 2 * LP_ROWS - 1) / (2 * LP_ROWS);
         g.v_tiles = (V + LP_COLS - 1) / LP_COLS, g.groups = (g.m_tiles + LP_GROUP - 1) / LP_GROUP;
         if ((long long)g.m_tiles * g.v_tiles > 0x3fffffff) ABK_REFUSE("gemm_logprobs: a vocabulary of %d is too many tiles", V);
         g.tiles = g.m_tiles * g.v_tiles, g.tokens = tokens + first, g.status = status;
