@@ -87,17 +87,96 @@ __device__ __noinline__ int cut_to_best(Ranked *list, Ranked *spare, int n, int 
     return n;
 }
 
+// What the warps of a CTA know of the most likely elements, in shared memory.
+struct Bounds {
+    volatile float of_warp[LOGPROBS_WARPS];  // what ceil(k / 8) of a warp's elements reach
+    volatile float common;                   // what k elements of the slice reach, as of some moment
+};
+// A warp's bound: the in_warp-th largest of its lanes' numbers.
+__device__ __forceinline__ void leave_bound(Bounds *b, float of_lane, int in_warp, int warp, int lane) {
+    float x = -INFINITY;
+    for (int r = 0; r < in_warp; r++) {
+        x = largest_of_lanes(of_lane);
+        const unsigned holders = __ballot_sync(0xffffffffu, of_lane == x);
+        if (lane == __ffs(holders) - 1) of_lane = -INFINITY;  // one of them is taken out
+    }
+    if (lane == 0) b->of_warp[warp] = x;
+}
+// What k elements of the slice reach: ceil(k / in_warp) warps have in_warp of them that reach it. The bounds of this moment or earlier
+// ones, either will do.
+__device__ __forceinline__ float common_bound(const Bounds *bounds, int top, int in_warp, int lane) {
+    const float b = bounds->of_warp[lane & (LOGPROBS_WARPS - 1)];
+    int above = 0;  // (equals in the order of the warps)
+#pragma unroll
+    for (int w = 0; w < LOGPROBS_WARPS; w++) {
+        const float o = __shfl_sync(0xffffffffu, b, w);
+        above += o > b || (o == b && w < (lane & (LOGPROBS_WARPS - 1)));
+    }
+    const unsigned at = __ballot_sync(0xffffffffu, above == (top + in_warp - 1) / in_warp - 1);
+    return __shfl_sync(0xffffffffu, b, __ffs(at) - 1);
+}
+// A warp's list: n elements, and what an element has to reach to be noted.
+struct Noted {
+    int n;
+    float cut;
+};
+// An element of every lane.
+__device__ __forceinline__ void note(Noted &noted, Ranked *list, float v, int at, bool real, int lane) {
+    const bool hit = real && v >= noted.cut;
+    const unsigned hits = __ballot_sync(0xffffffffu, hit);
+    if (hits) {
+        if (hit) list[noted.n + __popc(hits & ((1u << lane) - 1))] = {v, at};
+        noted.n += __popc(hits);
+    }
+}
+// Room for an element of every lane's next piece.
+__device__ __forceinline__ void make_room(Noted &noted, Ranked *list, Ranked *spare, int top, int lane) {
+    if (noted.n <= LOGPROBS_NOTED) return;
+    __syncwarp();
+    noted.n = cut_to_best(list, spare, noted.n, top, lane);
+    if (noted.n == top) noted.cut = fmaxf(noted.cut, next_up(list[noted.n - 1].v));
+}
+// The elements of a warp's 32 * U pieces from j0 on that reach the cut, read again behind their sums (the walk's own copies would have
+// to stay in registers for this: 512 rows of 151,936 with the 5 most likely take 71 us so, not 66).
+template <typename T> __device__ __forceinline__ Noted note_pieces(const uint4 *src, int j0, int pieces, int body, Noted noted, Ranked *list,
+                                                                Ranked *spare, int top, int lane) {
+    constexpr int N = Piece<T>::N, U = 16 / N;
+    uint4 w[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) w[u] = j0 + 32 * u + lane < pieces ? __ldg(src + j0 + 32 * u + lane) : Piece<T>::nothing();
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        float v[N];
+        Piece<T>::floats(w[u], v);
+        float of_piece = v[0];
+#pragma unroll
+        for (int e = 1; e < N; e++) of_piece = fmaxf(of_piece, v[e]);
+        if (!__any_sync(0xffffffffu, of_piece >= noted.cut)) continue;
+        make_room(noted, list, spare, top, lane);
+#pragma unroll
+        for (int e = 0; e < N; e++) note(noted, list, v[e], body + (j0 + 32 * u + lane) * N + e, j0 + 32 * u + lane < pieces, lane);
+    }
+    return noted;
+}
+// The bound moves with a thread's maximum that counts.
+__device__ __forceinline__ void move_bound(Bounds *b, float of_lane, int top, int in_warp, int warp, int lane) {
+    leave_bound(b, of_lane, in_warp, warp, lane);
+    __syncwarp();
+    const float x = common_bound(b, top, in_warp, lane);
+    if (lane == 0) b->common = x;
+}
+
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(LOGPROBS_THREADS, 4) logprobs_kernel(LogProbs p) {
+__global__ void __launch_bounds__(LOGPROBS_THREADS, sizeof(T) == 4 ? 4 : 3) logprobs_kernel(LogProbs p) {
     constexpr int N = Piece<T>::N, U = 16 / N, ROOM = LOGPROBS_NOTED + 32 * N;  // elements of a piece, pieces a thread takes at a time
-    __shared__ Ranked noted[TOP ? LOGPROBS_WARPS : 1][TOP ? ROOM : 1], best[TOP ? LOGPROBS_MAX_TOP : 1];
+    __shared__ Ranked lists[TOP ? LOGPROBS_WARPS : 1][TOP ? ROOM : 1], best[TOP ? LOGPROBS_MAX_TOP : 1];
     __shared__ Ranked cand[TOP ? LOGPROBS_MAX_SPLITS * LOGPROBS_MAX_TOP : 1];  // in turn: room to sort a list, all lists, the cluster's
-    __shared__ volatile float bounds[LOGPROBS_WARPS], common_s;
+    __shared__ Bounds bounds;
     __shared__ RowSums warp_sums[LOGPROBS_WARPS], cta_sums;
     __shared__ int count, in_cta, in_row, have[LOGPROBS_MAX_SPLITS];
     const int split = (int)tc::cluster_rank(), splits = (int)tc::cluster_size(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int row = blockIdx.y;
-    if (threadIdx.x == 0) count = 0, common_s = -INFINITY;
+    if (threadIdx.x == 0) count = 0, bounds.common = -INFINITY;
     pdl_wait();
     const T *x = (const T *)p.logits + row * p.stride;
     // slices start on a 16-byte boundary of memory; slice 0 also takes the elements before the first one
@@ -124,52 +203,15 @@ __global__ void __launch_bounds__(LOGPROBS_THREADS, 4) logprobs_kernel(LogProbs 
             l = add2(l, w), t = fma2(w, make_float2(fmaxf(d.x, LOGPROBS_FAR), fmaxf(d.y, LOGPROBS_FAR)), t);
         }
     };
-    Ranked *list = noted[TOP ? warp : 0];
-    int n = 0;                        // elements in the warp's list
-    float cut = -3.402823466e38f;     // what an element has to reach to be noted
-    auto note = [&](float v, int at, bool real) {  // (the whole warp, an element a lane)
-        const bool hit = real && v >= cut;
-        const unsigned hits = __ballot_sync(0xffffffffu, hit);
-        if (hits) {
-            if (hit) list[n + __popc(hits & ((1u << lane) - 1))] = {v, at};
-            n += __popc(hits);
-        }
-    };
-    auto make_room = [&]() {  // for an element of every lane's next piece
-        if (n <= LOGPROBS_NOTED) return;
-        __syncwarp();
-        n = cut_to_best(list, cand + warp * LOGPROBS_MAX_TOP, n, p.top, lane);
-        if (n == p.top) cut = fmaxf(cut, next_up(list[n - 1].v));
-    };
+    Ranked *list = lists[TOP ? warp : 0], *spare = cand + (TOP ? warp * LOGPROBS_MAX_TOP : 0);
+    Noted noted = {0, -3.402823466e38f};
     const int in_warp = (p.top + LOGPROBS_WARPS - 1) / LOGPROBS_WARPS;
-    auto bound = [&](float of_lane) {  // the warp's in_warp-th largest of its lanes' numbers
-        float b = -INFINITY;
-        for (int r = 0; r < in_warp; r++) {
-            b = largest_of_lanes(of_lane);
-            const unsigned holders = __ballot_sync(0xffffffffu, of_lane == b);
-            if (lane == __ffs(holders) - 1) of_lane = -INFINITY;  // one of them is taken out
-        }
-        if (lane == 0) bounds[warp] = b;
-    };
-    // What k elements of the slice reach: ceil(k / in_warp) warps have in_warp of them that reach it. The bounds of this moment or earlier
-    // ones, either will do.
-    auto common = [&]() {
-        const float b = bounds[lane & (LOGPROBS_WARPS - 1)];
-        int above = 0;  // (equals in the order of the warps)
-#pragma unroll
-        for (int w = 0; w < LOGPROBS_WARPS; w++) {
-            const float o = __shfl_sync(0xffffffffu, b, w);
-            above += o > b || (o == b && w < (lane & (LOGPROBS_WARPS - 1)));
-        }
-        const unsigned at = __ballot_sync(0xffffffffu, above == (p.top + in_warp - 1) / in_warp - 1);
-        return __shfl_sync(0xffffffffu, b, __ffs(at) - 1);
-    };
     auto loose = [&](int from, int to) {  // elements outside the pieces, a lane each
         const int at = from + lane;
         const float v = at < to ? to_float(x[at]) : -INFINITY;
         const float2 alone = make_float2(v, -INFINITY);
         if (at < to) sum(&alone, 1, v);
-        if (TOP) make_room(), note(v, at, at < to);
+        if (TOP) make_room(noted, list, spare, p.top, lane), note(noted, list, v, at, at < to, lane);
     };
     auto load = [&](int j0, uint4 *w) {
         if (j0 + 32 * U <= pieces) {
@@ -193,42 +235,31 @@ __global__ void __launch_bounds__(LOGPROBS_THREADS, 4) logprobs_kernel(LogProbs 
         for (int e = 1; e < 16; e++) most = fmaxf(most, v[e]);
         if (TOP) {
             if (first) {  // the first bounds
-                bound(most);
+                leave_bound(&bounds, most, in_warp, warp, lane);
                 __syncthreads();
-                cut = fmaxf(cut, common());
+                noted.cut = fmaxf(noted.cut, common_bound(&bounds, p.top, in_warp, lane));
+            } else {
+                noted.cut = fmaxf(noted.cut, bounds.common);
             }
-            else cut = fmaxf(cut, common_s);
         }
         if (first && warp == 0) loose(lo, body);
-        if (TOP && __any_sync(0xffffffffu, most >= cut)) {
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                float of_piece = v[u * N];
-#pragma unroll
-                for (int e = 1; e < N; e++) of_piece = fmaxf(of_piece, v[u * N + e]);
-                if (!__any_sync(0xffffffffu, of_piece >= cut)) continue;
-                make_room();
-#pragma unroll
-                for (int e = 0; e < N; e++) note(v[u * N + e], body + (j0 + 32 * u + lane) * N + e, j0 + 32 * u + lane < pieces);
-            }
-            if (!first && __any_sync(0xffffffffu, most >= cut && most > m)) {  // (else no thread's maximum that counts has moved)
-                bound(fmaxf(m, most));
-                __syncwarp();
-                const float b = common();
-                if (lane == 0) common_s = b;
-            }
-        }
+        const bool risen = most > m;
         sum((const float2 *)v, 8, most);
+        if (TOP && __any_sync(0xffffffffu, most >= noted.cut)) {
+            const bool moves = __any_sync(0xffffffffu, most >= noted.cut && risen);  // (else no thread's maximum that counts does)
+            noted = note_pieces<T>(src, j0, pieces, body, noted, list, spare, p.top, lane);
+            if (!first && moves) move_bound(&bounds, m, p.top, in_warp, warp, lane);
+        }
         first = false;
     }
     if (warp == LOGPROBS_WARPS - 1) loose(tail, hi);
     const RowSums mine = joined_lanes({m, l.x + l.y, t.x + t.y, 0.0f}, 16);
     if (lane == 0) warp_sums[warp] = mine;
-    if (TOP) make_room();
+    if (TOP) make_room(noted, list, spare, p.top, lane);
     __syncthreads();
     if (TOP) {
-        const float b = common();
-        for (int i = lane; i < n; i += 32)
+        const float b = common_bound(&bounds, p.top, in_warp, lane);
+        for (int i = lane; i < noted.n; i += 32)
             if (list[i].v >= b) cand[atomicAdd(&count, 1)] = list[i];
     }
     if (warp == 0) {
@@ -286,10 +317,10 @@ __global__ void __launch_bounds__(LOGPROBS_THREADS, 4) logprobs_kernel(LogProbs 
                         have[lane] = n_c, kth = n_c == p.top ? v : -INFINITY, all_have = n_c >= few ? w : -INFINITY;
                     }
                     found = __reduce_add_sync(0xffffffffu, n_c), kth = fmaxf(warp_max(kth), -warp_max(-all_have));
-                    if (lane == 0) common_s = kth, in_row = found;
+                    if (lane == 0) bounds.common = kth, in_row = found;
                 }
                 __syncthreads();
-                const float kth = common_s;
+                const float kth = bounds.common;
                 for (int j = threadIdx.x; j < splits * p.top; j += LOGPROBS_THREADS) {
                     const int c = j / p.top, i = j - c * p.top;
                     if (i >= have[c]) continue;
