@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8Read p) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int page_out = blockIdx.x, head = blockIdx.y, j = warp >> 2, block = warp & 3;
     const int s = last_not_above(p.first_page, p.n_seqs, lane, [&](int first, int) { return first <= page_out; });
-    if (s < 0 || page_out >= p.first_page[s + 1]) return;
+    if (s < 0 || page_out < p.first_page[s] || page_out >= p.first_page[s + 1]) return;
     const int after = p.seq_len_after[s], slot = kv8_slot(p.seq_slot[s], p.n_slots, p.status);
     const int pos0 = (page_out - p.first_page[s]) * KV8_PAGE + block * KV8_BLOCK;
     T *dst = (T *)(j == 0 ? p.out_k : p.out_v) +

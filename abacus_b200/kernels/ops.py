@@ -553,6 +553,7 @@ def gemm_tc_logprobs(x, w, tokens, logprob, entropy, ws, m=None):
         raise KernelRefused("gemm_tc_logprobs: bfloat16 rows of a multiple of 8, 16-byte aligned")
     lib = load_module("gemm_logprobs")
     memory = ws.get("logprobs_sums", (_gemm_logprobs_floats(m),), torch.float32)
+    _here("gemm_tc_logprobs", memory)
     fn = _typed(lib.abk_gemm_logprobs, "ppiiillpppplpp")
     _check(lib, fn(x.data_ptr(), w.data_ptr(), m, vocab, k, x.stride(0), w.stride(0), tokens.data_ptr(), logprob.data_ptr(), _at(entropy),
                    memory.data_ptr(), memory.numel(), kernel_status(x.device).data_ptr(), _raw_stream()), "gemm_tc_logprobs",
@@ -591,7 +592,7 @@ def kv8_write(qkv, n_heads, n_kv_heads, head_dim, batch, cache, row=None):
     """The keys and values of the step's rows go into an 8-bit cache (cache.LayerKV8): blocks of 16 tokens that the step
     completes into 8 bits with their scales, the last tokens of a sequence that do not fill a block into its open block.
     qkv bfloat16 [rows, (n_heads + 2 n_kv_heads) head_dim], prepared (see qkv_prep); what a sequence holds before the
-    step (batch.seq_pos0 tokens) must be in the cache. The same step a second time is the same step only for single tokens, and where
+    step (batch.seq_pos0 tokens) must be in the cache, and no slot may be in the step twice. The same step a second time is the same step only for single tokens, and where
     no sequence both completes a block it had begun and begins another."""
     _here("kv8_write", qkv, batch.seq_slot)
     lib = load_module("kv8")
@@ -612,7 +613,7 @@ def kv8_read(cache, batch, first_page, k, v):
     """What an 8-bit cache holds of the step's sequences, behind the step, as pages: logical page i of sequence s becomes page
     first_page[s] + i of k and v, float32 or bfloat16 [pages, kv heads, 64, head_dim], for all first_page[s + 1] - first_page[s]
     pages of it; places behind the sequence's last token become zeros, other pages are left alone. first_page int32
-    [sequences + 1], not falling. Not for a cache under a window."""
+    [sequences + 1], not falling (of one that falls, some pages are left alone). Not for a cache under a window."""
     _here("kv8_read", batch.seq_slot, first_page, k, v)
     lib = load_module("kv8")
     n_seqs = batch.seq_slot.numel()
@@ -631,7 +632,8 @@ def kv8_read(cache, batch, first_page, k, v):
 def attention_kv8(qkv, out, n_heads, n_kv_heads, head_dim, scale, window, batch, cache, ws):
     """Causal grouped-query attention of the step's rows (src/model.c:197-211) over an 8-bit cache that holds the step's own keys
     and values too (kv8_write comes first): each row sees the keys up to its position, within `window` of it if given. Any
-    number of new tokens a sequence; meant for one or a few (each row reads its keys itself). q is read from qkv's q columns."""
+    number of new tokens a sequence; meant for one or a few (each row reads its keys itself). q is read from qkv's q columns.
+    ws: a Workspace for the parts of rows that several CTAs share. A block with a value that is not finite is NaN in all that see it."""
     _here("attention_kv8", qkv, out, batch.token_seq)
     lib = load_module("attention_kv8")
     n, row = batch.n_rows, (n_heads + 2 * n_kv_heads) * head_dim
@@ -640,8 +642,12 @@ def attention_kv8(qkv, out, n_heads, n_kv_heads, head_dim, scale, window, batch,
     rows, width = out.shape
     assert out.dtype == torch.bfloat16 and out.is_contiguous() and width == n_heads * head_dim and rows >= n
     _kv8_fits("attention_kv8", batch, cache, n_kv_heads, head_dim)
+    if cache.ring_pages and (not window or window + batch.longest - 1 > cache.ring_pages * cache.tokens_per_page):
+        raise KernelRefused(f"attention_kv8: a ring of {cache.ring_pages} pages does not hold the keys that {batch.longest} new tokens of a "
+                            f"sequence see under a window of {window}")
     floats = _kv8_part_floats(n_heads, n_kv_heads, head_dim, cache.device_index)
     parts = ws.get("attention_kv8_parts", (floats,), torch.float32)
+    _here("attention_kv8", parts)
     fn = _typed(lib.abk_attention_kv8, "plpiiiiifipppppppppiiiiplpp")
     _check(lib, fn(qkv.data_ptr(), row, out.data_ptr(), n, n_heads, n_kv_heads, head_dim, KV8_FORMS[cache.form], scale, window or 0,
                    batch.token_seq.data_ptr(), batch.token_pos.data_ptr(), batch.seq_slot.data_ptr(), batch.seq_len_after.data_ptr(),

@@ -195,6 +195,10 @@ def test_attention_under_a_window_with_a_ring_of_pages(ops, window):
         batch = run.write(ops, [(a, 1), (b, 1)], qkv)
         if i % 7 == 0:
             run.attend(ops, batch, qkv)
+    out = torch.zeros((2, 6 * 64), dtype=torch.bfloat16, device="cuda")
+    for too_wide in (None, run.kv.ring_pages * 64 + 1):
+        with pytest.raises(ops.KernelRefused, match="ring"):
+            ops.attention_kv8(qkv.cuda(), out, 6, 2, 64, 0.125, too_wide, batch, run.kv, run.ws)
     with pytest.raises(ops.KernelRefused):
         ops.kv8_read(run.kv, batch, torch.zeros(3, dtype=torch.int32, device="cuda"), *(torch.zeros((1, 2, 64, 64), device="cuda") for _ in range(2)))
 
@@ -387,6 +391,30 @@ def test_models_through_the_engine(tmp_path, ops, form):
     s, w = lm.score([first])[0], plain_lm.score([first])[0]
     assert np.abs(np.array(s.logprobs) - np.array(w.logprobs)).max() < 0.05 * float(want.abs().max())
     engine.check_status()
+
+
+def test_first_pages_that_fall_and_models_that_have_other_mixers(tmp_path, ops):
+    """kv8_read with a list that is not rising stays inside; an engine of another architecture, or in float32, refuses an 8-bit cache."""
+    import abacus_b200
+    import temetar_models
+    run = Run(2, 1, 64, "int8", slots=3, pages=8)
+    slots = [run.open() for _ in range(3)]
+    batch = run.write(ops, [(s, 70) for s in slots], run.rows(210))
+    k, v = (torch.full((6, 1, 64, 64), 7.0, device="cuda") for _ in range(2))
+    for first in ([4, 2, 6, 0], [0, -5, 3, 2], [6, 5, 4, 3], [0, 100, 200, 300], [-3, -2, -1, 0]):
+        ops.kv8_read(run.kv, batch, torch.tensor(first, dtype=torch.int32, device="cuda"), k, v)
+    torch.cuda.synchronize()
+    assert not any(ops.kernel_status(k.device).tolist())
+    (tmp_path / "t").mkdir()
+    (tmp_path / "q").mkdir()
+    other = temetar_models.write_folder(tmp_path / "t", "P")[0]
+    with pytest.raises(ValueError, match="8-bit"):
+        abacus_b200.LM(other, cache="int8", max_tokens=256)
+    folder = make_model_folder(tmp_path / "q", "D")
+    with pytest.raises(ValueError, match="8-bit"):
+        abacus_b200.LM(folder, dtype="float32", cache="int8", max_tokens=256)
+    with pytest.raises(ValueError, match="int8 or e4m3"):
+        abacus_b200.LM(folder, cache="fp8", max_tokens=256)
 
 
 def test_windowed_layers_through_the_engine(tmp_path):
