@@ -15,7 +15,7 @@
 // floats with the query heads as the 8 columns (two tiles of them from 9 heads on): scores are keys x heads, the
 // output columns x heads, so nothing is spent on heads that are not there beyond the eighth. An 8-bit number is a float16 number exactly,
 // and q is one too once each head's row is brought below 1 by a power of two (what of a head lies 2^-14 below its largest
-// element keeps an absolute error of 2^-25 of that). The softmax weights are p_j s_b 2^-u in float16, 2^-12 off at most, u
+// element keeps an absolute error of 2^-25 of that). The softmax weights are p_j s_b 2^-u in float16, 2^-11 off at most, u
 // chosen per head so that the largest ever seen is about 1: a block of small values with large weights counts as precisely
 // as one of large values. Scores, maximum, sum and output are float32. The open block's keys and values go through the same products
 // in bfloat16, its weights as two bfloat16 parts.
@@ -25,6 +25,11 @@
 // inner dimension is free as long as both operands follow it: a thread's four neighbouring bytes of a key row are the pairs
 // that the instruction calls (2c, 2c + 1) and (2c + 8, 2c + 9), and q is read in that order. Values come transposed, two
 // tokens and two columns to a word: even columns are the upper eight rows of a tile and odd columns the lower eight.
+//
+// Measured (attention and fold, without the write): 32 rows over 128 to 4,096 tokens, 32 query and 8 kv heads of 128, int8, in 35 us
+// (139 MB; the first page lands after 5, pieces end between 24 and 34, the fold takes 3); 8 rows over 32,768 in 91 (5.9 TB/s); two
+// rows over 131,071 and 100,000 e4m3 tokens in 87; one row over 2,176 in 10. A page's block takes a warp some 260 instructions (int8),
+// half of them the way from bytes to float16: at the copy rate 0.4 of what an SM issues.
 #define ABK_DEFINE_ERROR
 #include "common.cuh"
 #include "tc_common.cuh"

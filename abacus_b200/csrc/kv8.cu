@@ -7,6 +7,8 @@
 // zero; a block with a value that is not finite reads back as NaN.
 // A block is put into 8 bits when its last token comes; until then its tokens lie as they came in the slot's open block,
 // so that no value is ever rounded twice and a token's place in the 8-bit pages is written once.
+// A warp takes one block of one head's keys or values, 16 rows of the step in 16-byte pieces, in registers from load to store. Measured:
+// prompts of 5,745 tokens, 8 heads of 128, 35 MB in and out, in 10 us, read back as float32 in 13 (59 MB); single tokens of 32 sequences in 3.
 #define ABK_DEFINE_ERROR
 #include "common.cuh"
 #include "kv8.cuh"
@@ -25,16 +27,10 @@ struct Kv8Write {
     int n_pages, n_slots, *status;
 };
 
-// One block of one head's keys or values, held by a warp: token t of the block, elements 8 c .., in piece i of a lane with
-// 32 i + lane = t * HD / 8 + c.
-template <int HD> struct Kv8Block {
-    static constexpr int PIECES = KV8_BLOCK * HD / 256;
-    uint4 x[PIECES];
-};
-
+// A warp holds a block in pieces of 8 elements: token t, elements 8 c .., in piece i of a lane with 32 i + lane = t * HD / 8 + c.
 template <int HD, int FORM>
 __global__ void __launch_bounds__(32 * KV8_WARPS) kv8_write_kernel(Kv8Write p) {
-    constexpr int LPR = HD / 8, PIECES = Kv8Block<HD>::PIECES;  // lanes to a row of 16-byte pieces
+    constexpr int LPR = HD / 8, PIECES = KV8_BLOCK * HD / 256;  // lanes to a row of 16-byte pieces
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int which = blockIdx.y * KV8_WARPS + warp;  // keys of the heads, then values of the heads

@@ -9,11 +9,15 @@
 // A row is read once, by a CTA or, where there are few rows, by a cluster of up to 16 CTAs, a slice each. Every thread keeps a
 // running maximum and the two sums over its elements, 16 at a time, the next 16 on their way; nothing in the walk waits for
 // another warp. The most likely tokens: an element is noted, in the warp's own list in shared memory, only where it reaches a bound
-// that at least k elements of the slice reach: the smallest of the warps' ceil(k / 8)-th largest thread maxima, which the warps
-// leave in shared memory as they go (a bound that is out of date is only lower). A list that fills up is cut to its best k; a
+// that at least k elements of the slice reach: every warp leaves its ceil(k / 8)-th largest thread maximum in shared memory as it goes,
+// and of these the one that enough warps reach is the bound (one that is out of date is only lower). A list that fills up is cut to its best k; a
 // warp meets its elements by rising index, so from then on an equal of the k-th need not be noted. At the end the elements that
 // reach the last bound, some tens, are ranked by counting those before each, and once more those of a cluster's CTAs. Elements of -inf are
 // never noted: where a row has fewer than k others, the first of them fill its places.
+//
+// Measured: 512 rows of 151,936 float32 logits with 5 alternatives in 66 us, 4.7 TB/s (53 without); 8 rows with 20 in 12.7 (9.4 without), a
+// chain of three turns of loads, bounds, ranks and the cluster's fold; 200 rows of 50,261 bfloat16 logits, a twentieth not -inf, with 64
+// in 26 (10 without): there every turn of 512 elements has some to note.
 #define ABK_DEFINE_ERROR
 #include "common.cuh"
 #include "tc_common.cuh"
