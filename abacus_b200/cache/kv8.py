@@ -51,8 +51,7 @@ class LayerKV8:
                 raise ValueError(f"{name} of an 8-bit cache is on {t.device}, its keys on {self.k.device}")
 
         known = dict(form="int8" if self.k.dtype == torch.uint8 else "e4m3", n_pages=pages, n_kv_heads=heads, head_dim=dim,
-                     n_slots=self.open.shape[0], device_index=self.k.get_device(),
-                     pointers=tuple(t.data_ptr() for t in (self.k, self.v, self.scales, self.open)), table_pointer=self.page_table.data_ptr(),
+                     n_slots=self.open.shape[0], device_index=self.k.get_device(), record=None,  # (ops.Kv8Cache, at the first call)
                      room=None if self.ring_pages else self.table_width * PAGE)
         for name, value in known.items():
             object.__setattr__(self, name, value)

@@ -538,33 +538,33 @@ extern "C" long long abk_attention_kv8_part_floats(int n_heads, int n_kv_heads, 
     const int group = n_kv_heads > 0 ? n_heads / n_kv_heads : 1;
     return 2ll * KV8_CTAS * abk_sm_count() * (group < KV8_HEADS ? group : KV8_HEADS) * (head_dim + 4);
 }
-extern "C" int abk_attention_kv8(const void *q, long long q_row, void *out, int n_rows, int n_heads, int n_kv_heads, int head_dim,
-                                 int form, float scale, int window, const int *token_seq, const int *token_pos, const int *seq_slot,
-                                 const int *seq_len_after, const void *k, const void *v, const float *scales, const void *open,
-                                 const int *page_table, int table_width, int ring_pages, int pool_pages, int n_slots, float *parts,
-                                 long long part_floats, int *status, void *stream) {
+extern "C" int abk_attention_kv8(const void *q, long long q_row, void *out, int n_rows, int n_heads, float scale, int window,
+                                 const int *token_seq, const int *token_pos, const int *seq_slot, const int *seq_len_after,
+                                 const Kv8Cache *cache, float *parts, long long part_floats, void *stream) {
+    const Kv8Cache &c = *cache;
+    const int head_dim = c.head_dim, n_kv_heads = c.n_kv_heads, form = c.form;
     if (n_rows <= 0) return 0;
     if (head_dim != 64 && head_dim != 128) ABK_REFUSE("attention_kv8: head_dim %d is not 64 or 128", head_dim);
     if (form != KV8_INT8 && form != KV8_E4M3) ABK_REFUSE("attention_kv8: no 8-bit form %d", form);
     if (n_kv_heads < 1 || n_heads < 1 || n_heads % n_kv_heads) ABK_REFUSE("attention_kv8: %d heads do not divide into %d kv heads", n_heads, n_kv_heads);
     const int group = n_heads / n_kv_heads, runs = (group + KV8_HEADS - 1) / KV8_HEADS, heads = group < KV8_HEADS ? group : KV8_HEADS;
-    if ((((uintptr_t)q | (uintptr_t)out) & 7) || (q_row & 3) || (((uintptr_t)scales | (uintptr_t)open | (uintptr_t)parts) & 15))
+    if ((((uintptr_t)q | (uintptr_t)out) & 7) || (q_row & 3) || (((uintptr_t)c.scales | (uintptr_t)c.open | (uintptr_t)parts) & 15))
         ABK_REFUSE("attention_kv8: q and out must be 8-byte aligned, scales, open blocks and parts 16-byte aligned");
     const int grid = KV8_CTAS * abk_sm_count();
     if (grid > KV8_MAX_GRID) ABK_REFUSE("attention_kv8: %d CTAs are more than the fold has room for", grid);
     if (part_floats < abk_attention_kv8_part_floats(n_heads, n_kv_heads, head_dim))
         ABK_REFUSE("attention_kv8: room for %lld floats of parts is too little", part_floats);
     CUtensorMap km, vm;
-    const long long pool_rows = (long long)pool_pages * n_kv_heads * KV8_PAGE * head_dim / 128;
-    int rc = tmap::bytes_in_rows_of_128(k, pool_rows, KV8_PAGE * head_dim / 128, &km);
-    if (!rc) rc = tmap::bytes_in_rows_of_128(v, pool_rows, KV8_PAGE * head_dim / 128, &vm);
+    const long long pool_rows = (long long)c.n_pages * n_kv_heads * KV8_PAGE * head_dim / 128;
+    int rc = tmap::bytes_in_rows_of_128(c.k, pool_rows, KV8_PAGE * head_dim / 128, &km);
+    if (!rc) rc = tmap::bytes_in_rows_of_128(c.v, pool_rows, KV8_PAGE * head_dim / 128, &vm);
     if (rc) return rc;
     AttnKv8 p;
     p.q = (const __nv_bfloat16 *)q, p.q_row = q_row, p.out = (__nv_bfloat16 *)out, p.n_heads = n_heads, p.n_kv_heads = n_kv_heads;
     p.scale_log2 = scale * 1.4426950408889634f, p.window = window, p.token_seq = token_seq, p.token_pos = token_pos;
-    p.seq_slot = seq_slot, p.seq_len_after = seq_len_after, p.cache.page_table = page_table, p.cache.table_width = table_width;
-    p.cache.ring_pages = ring_pages, p.cache.tokens_per_page = KV8_PAGE, p.scales = scales, p.open = (const __nv_bfloat16 *)open;
-    p.n_pages = pool_pages, p.n_slots = n_slots, p.status = status, p.runs = runs, p.pairs = n_kv_heads * runs, p.parts = parts;
+    p.seq_slot = seq_slot, p.seq_len_after = seq_len_after, p.cache.page_table = c.page_table, p.cache.table_width = c.table_width;
+    p.cache.ring_pages = c.ring_pages, p.cache.tokens_per_page = KV8_PAGE, p.scales = c.scales, p.open = (const __nv_bfloat16 *)c.open;
+    p.n_pages = c.n_pages, p.n_slots = c.n_slots, p.status = c.status, p.runs = runs, p.pairs = n_kv_heads * runs, p.parts = parts;
     void (*kernel)(CUtensorMap, CUtensorMap, AttnKv8) = nullptr;
     auto of_dim = [&](auto hd, auto tiles) {
         constexpr int HD = decltype(hd)::value, NT = decltype(tiles)::value;

@@ -177,54 +177,53 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8Read p) {
     }
 }
 
-extern "C" int abk_kv8_write(const void *qkv, long long row, int n_rows, int n_heads, int n_kv_heads, int head_dim, int form,
-                             int n_seqs, int one_each, const int *seq_start, const int *seq_pos0, const int *seq_len_after,
-                             const int *seq_slot, const int *page_table, int table_width, int ring_pages, void *k, void *v,
-                             float *scales, void *open, int pool_pages, int n_slots, int *status, void *stream) {
+extern "C" int abk_kv8_cache_bytes() { return (int)sizeof(Kv8Cache); }
+extern "C" int abk_kv8_write(const void *qkv, long long row, int n_rows, int n_heads, int n_seqs, int one_each, const int *seq_start,
+                             const int *seq_pos0, const int *seq_len_after, const int *seq_slot, const Kv8Cache *cache, void *stream) {
+    const Kv8Cache &c = *cache;
     if (n_rows <= 0 || n_seqs <= 0) return 0;
-    if (head_dim != 64 && head_dim != 128) ABK_REFUSE("kv8_write: head_dim %d is not 64 or 128", head_dim);
-    if (form != KV8_INT8 && form != KV8_E4M3) ABK_REFUSE("kv8_write: no 8-bit form %d", form);
-    if ((((uintptr_t)qkv | (uintptr_t)k | (uintptr_t)v | (uintptr_t)open) & 15) || (row & 7) || ((uintptr_t)scales & 3))
+    if (c.head_dim != 64 && c.head_dim != 128) ABK_REFUSE("kv8_write: head_dim %d is not 64 or 128", c.head_dim);
+    if (c.form != KV8_INT8 && c.form != KV8_E4M3) ABK_REFUSE("kv8_write: no 8-bit form %d", c.form);
+    if ((((uintptr_t)qkv | (uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)c.open) & 15) || (row & 7) || ((uintptr_t)c.scales & 3))
         ABK_REFUSE("kv8_write: rows, pools and open blocks must be 16-byte aligned");
     const int units = one_each ? n_seqs : n_rows / KV8_BLOCK + 2 * n_seqs + 1;
-    const int groups = (2 * n_kv_heads + KV8_WARPS - 1) / KV8_WARPS;
-    if (n_kv_heads < 1 || groups > 65535) ABK_REFUSE("kv8_write: %d kv heads", n_kv_heads);
+    const int groups = (2 * c.n_kv_heads + KV8_WARPS - 1) / KV8_WARPS;
+    if (c.n_kv_heads < 1 || groups > 65535) ABK_REFUSE("kv8_write: %d kv heads", c.n_kv_heads);
     Kv8Write p;
-    p.qkv = (const __nv_bfloat16 *)qkv, p.row = row, p.n_heads = n_heads, p.n_kv_heads = n_kv_heads, p.n_seqs = n_seqs;
+    p.qkv = (const __nv_bfloat16 *)qkv, p.row = row, p.n_heads = n_heads, p.n_kv_heads = c.n_kv_heads, p.n_seqs = n_seqs;
     p.one_each = one_each, p.seq_start = seq_start, p.seq_pos0 = seq_pos0, p.seq_len_after = seq_len_after;
-    p.seq_slot = seq_slot, p.cache.page_table = page_table, p.cache.table_width = table_width, p.cache.ring_pages = ring_pages;
-    p.cache.tokens_per_page = KV8_PAGE, p.k = (uint8_t *)k, p.v = (uint8_t *)v, p.scales = scales, p.open = (__nv_bfloat16 *)open;
-    p.n_pages = pool_pages, p.n_slots = n_slots, p.status = status;
+    p.seq_slot = seq_slot, p.cache.page_table = c.page_table, p.cache.table_width = c.table_width, p.cache.ring_pages = c.ring_pages;
+    p.cache.tokens_per_page = KV8_PAGE, p.k = (uint8_t *)c.k, p.v = (uint8_t *)c.v, p.scales = c.scales, p.open = (__nv_bfloat16 *)c.open;
+    p.n_pages = c.n_pages, p.n_slots = c.n_slots, p.status = c.status;
     const dim3 grid(units, groups), block(32 * KV8_WARPS);
     auto go = [&](auto kernel) { abk_launch(kernel, grid, block, 0, (cudaStream_t)stream, p); };
-    if (head_dim == 64) form == KV8_INT8 ? go(kv8_write_kernel<64, KV8_INT8>) : go(kv8_write_kernel<64, KV8_E4M3>);
-    else form == KV8_INT8 ? go(kv8_write_kernel<128, KV8_INT8>) : go(kv8_write_kernel<128, KV8_E4M3>);
+    if (c.head_dim == 64) c.form == KV8_INT8 ? go(kv8_write_kernel<64, KV8_INT8>) : go(kv8_write_kernel<64, KV8_E4M3>);
+    else c.form == KV8_INT8 ? go(kv8_write_kernel<128, KV8_INT8>) : go(kv8_write_kernel<128, KV8_E4M3>);
     return ABK_LAUNCH_RESULT();
 }
 
-extern "C" int abk_kv8_read(const void *k, const void *v, const float *scales, const void *open, int n_kv_heads, int head_dim,
-                            int form, const int *page_table, int table_width, int n_seqs, const int *seq_len_after,
-                            const int *seq_slot, const int *first_page, int n_pages, void *out_k, void *out_v, int out_dtype,
-                            int pool_pages, int n_slots, int *status, void *stream) {
+extern "C" int abk_kv8_read(const Kv8Cache *cache, int n_seqs, const int *seq_len_after, const int *seq_slot, const int *first_page,
+                            int n_pages, void *out_k, void *out_v, int out_dtype, void *stream) {
+    const Kv8Cache &c = *cache;
     if (n_pages <= 0 || n_seqs <= 0) return 0;
-    if (head_dim != 64 && head_dim != 128) ABK_REFUSE("kv8_read: head_dim %d is not 64 or 128", head_dim);
-    if (form != KV8_INT8 && form != KV8_E4M3) ABK_REFUSE("kv8_read: no 8-bit form %d", form);
-    if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)open | (uintptr_t)out_k | (uintptr_t)out_v) & 15)
+    if (c.head_dim != 64 && c.head_dim != 128) ABK_REFUSE("kv8_read: head_dim %d is not 64 or 128", c.head_dim);
+    if (c.form != KV8_INT8 && c.form != KV8_E4M3) ABK_REFUSE("kv8_read: no 8-bit form %d", c.form);
+    if (((uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)c.open | (uintptr_t)out_k | (uintptr_t)out_v) & 15)
         ABK_REFUSE("kv8_read: pools, open blocks and copies must be 16-byte aligned");
-    if (n_kv_heads < 1 || n_kv_heads > 65535) ABK_REFUSE("kv8_read: %d kv heads", n_kv_heads);
+    if (c.n_kv_heads < 1 || c.n_kv_heads > 65535) ABK_REFUSE("kv8_read: %d kv heads", c.n_kv_heads);
     Kv8Read p;
-    p.first_page = first_page, p.seq_len_after = seq_len_after, p.seq_slot = seq_slot, p.n_seqs = n_seqs, p.n_kv_heads = n_kv_heads;
-    p.cache.page_table = page_table, p.cache.table_width = table_width, p.cache.ring_pages = 0, p.cache.tokens_per_page = KV8_PAGE;
-    p.k = (const uint8_t *)k, p.v = (const uint8_t *)v, p.scales = scales, p.open = (const __nv_bfloat16 *)open;
-    p.out_k = out_k, p.out_v = out_v, p.n_pages = pool_pages, p.n_slots = n_slots, p.status = status;
-    const dim3 grid(n_pages, n_kv_heads), block(256);
+    p.first_page = first_page, p.seq_len_after = seq_len_after, p.seq_slot = seq_slot, p.n_seqs = n_seqs, p.n_kv_heads = c.n_kv_heads;
+    p.cache.page_table = c.page_table, p.cache.table_width = c.table_width, p.cache.ring_pages = 0, p.cache.tokens_per_page = KV8_PAGE;
+    p.k = (const uint8_t *)c.k, p.v = (const uint8_t *)c.v, p.scales = c.scales, p.open = (const __nv_bfloat16 *)c.open;
+    p.out_k = out_k, p.out_v = out_v, p.n_pages = c.n_pages, p.n_slots = c.n_slots, p.status = c.status;
+    const dim3 grid(n_pages, c.n_kv_heads), block(256);
     auto go = [&](auto kernel) { abk_launch(kernel, grid, block, 0, (cudaStream_t)stream, p); };
     auto by_form = [&](auto hd) {
         constexpr int HD = decltype(hd)::value;
-        if (out_dtype == ABK_F32) form == KV8_INT8 ? go(kv8_read_kernel<HD, KV8_INT8, float>) : go(kv8_read_kernel<HD, KV8_E4M3, float>);
-        else form == KV8_INT8 ? go(kv8_read_kernel<HD, KV8_INT8, __nv_bfloat16>) : go(kv8_read_kernel<HD, KV8_E4M3, __nv_bfloat16>);
+        if (out_dtype == ABK_F32) c.form == KV8_INT8 ? go(kv8_read_kernel<HD, KV8_INT8, float>) : go(kv8_read_kernel<HD, KV8_E4M3, float>);
+        else c.form == KV8_INT8 ? go(kv8_read_kernel<HD, KV8_INT8, __nv_bfloat16>) : go(kv8_read_kernel<HD, KV8_E4M3, __nv_bfloat16>);
     };
-    if (head_dim == 64) by_form(std::integral_constant<int, 64>());
+    if (c.head_dim == 64) by_form(std::integral_constant<int, 64>());
     else by_form(std::integral_constant<int, 128>());
     return ABK_LAUNCH_RESULT();
 }

@@ -13,6 +13,16 @@
 #define KV8_PAGE_BLOCKS (KV8_PAGE / KV8_BLOCK)
 enum { KV8_INT8 = 0, KV8_E4M3 = 1 };
 
+// An 8-bit cache of one schedule entry, as the launchers get it (kernels/ops.py: Kv8Cache has the same fields in the same order).
+struct Kv8Cache {
+    void *k, *v;        // [pages, kv heads, 64, head_dim]
+    float *scales;      // [pages, kv heads, 2 (keys, values), 4]
+    void *open;         // bfloat16 [slots, 2, kv heads, 16, head_dim]
+    const int *page_table;
+    int *status;
+    int table_width, ring_pages, n_pages, n_slots, n_kv_heads, head_dim, form, pad;
+};
+
 template <int FORM> __host__ __device__ constexpr float kv8_top() { return FORM == KV8_INT8 ? 127.0f : 448.0f; }
 
 // Eight bfloat16 values in 8 bits each; `by` and `inverse` as kv8_steps makes them of the block's largest magnitude.

@@ -147,6 +147,9 @@ def compile_module(module, verbose=True, extra_flags=()):
 
 def load_module(module):
     """The ctypes library of csrc/<module>.cu, compiled first if it is missing or stale."""
+    lib = _loaded.get(module)
+    if lib is not None:
+        return lib
     with _lock:
         if module in _loaded:
             return _loaded[module]

@@ -495,13 +495,11 @@ def sample_all(logits, temperature, rng_state, out, n_rows=None, rng_index=None)
 # ------------------------------------------------------------------ log probabilities (csrc/logprobs.cu)
 def _here(what, *tensors):
     """The tensors are on the current device, whose stream the kernel goes to."""
-    for t in tensors:
-        if t is not None and not t.is_cuda:
-            _need_cuda(t)
-    device = torch._C._cuda_getDevice()
+    device = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2
     for t in tensors:
         if t is not None and t.get_device() != device:
-            raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{device}")
+            _need_cuda(t)
+            raise KernelError(f"{what}: a tensor is on {t.device}, the current device is another one (cuda:{torch.cuda.current_device()})")
 
 
 LOGPROBS_MAX_TOP = 64
@@ -571,14 +569,29 @@ def _gemm_logprobs_floats(m):
 KV8_FORMS = {"int8": 0, "e4m3": 1}
 
 
-def _kv8_fits(what, batch, cache, n_kv_heads=None, head_dim=None):
-    """The step's heads are the cache's, its positions have their places there, and the cache is on the current device."""
+class Kv8Cache(ctypes.Structure):
+    """A cache.LayerKV8 as the launchers get it (csrc/kv8.cuh): put together at the first call and kept with it."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "scales", "open", "page_table", "status")]
+    _fields_ += [(n, ctypes.c_int) for n in ("table_width", "ring_pages", "n_pages", "n_slots", "n_kv_heads", "head_dim", "form", "pad")]
+
+
+def _kv8_record(what, batch, cache, n_kv_heads=None, head_dim=None):
+    """The address of the cache's record, if the step's heads are the cache's, its positions have their places there, and the cache is
+    on the current device."""
     if n_kv_heads is not None and (cache.n_kv_heads != n_kv_heads or cache.head_dim != head_dim):
         raise KernelRefused(f"{what}: the cache holds {cache.n_kv_heads} kv heads of {cache.head_dim}, not {n_kv_heads} of {head_dim}")
     if cache.room is not None and batch.max_len_after > cache.room:
         raise KernelRefused(f"{what}: {batch.max_len_after} tokens are more than the page table's {cache.table_width} pages hold")
-    if cache.device_index != torch._C._cuda_getDevice():
-        raise KernelError(f"{what}: the cache is on {cache.k.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+    record = cache.record
+    if record is None:
+        _need_cuda(cache.k)
+        made = Kv8Cache(cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(), cache.open.data_ptr(), cache.page_table.data_ptr(),
+                        kernel_status(cache.k.device).data_ptr(), cache.table_width, cache.ring_pages, cache.n_pages, cache.n_slots,
+                        cache.n_kv_heads, cache.head_dim, KV8_FORMS[cache.form], 0)
+        assert load_module("kv8").abk_kv8_cache_bytes() == ctypes.sizeof(made)
+        record = (made, ctypes.addressof(made))
+        object.__setattr__(cache, "record", record)
+    return record[1]
 
 
 @functools.lru_cache(maxsize=4096)
@@ -600,13 +613,12 @@ def kv8_write(qkv, n_heads, n_kv_heads, head_dim, batch, cache, row=None):
     row = row or heads_size
     n, width = qkv.shape
     assert qkv.dtype == torch.bfloat16 and qkv.is_contiguous() and width == row >= heads_size and n >= batch.n_rows
-    _kv8_fits("kv8_write", batch, cache, n_kv_heads, head_dim)
-    fn = _typed(lib.abk_kv8_write, "pliiiiiiipppppiippppiipp")
+    record = _kv8_record("kv8_write", batch, cache, n_kv_heads, head_dim)
+    _here("kv8_write", cache.k)
+    fn = _typed(lib.abk_kv8_write, "pliiiipppppp")
     slots = batch.seq_slot
-    _check(lib, fn(qkv.data_ptr(), row, batch.n_rows, n_heads, n_kv_heads, head_dim, KV8_FORMS[cache.form], slots.numel(),
-                   1 if batch.is_decode else 0, batch.seq_start.data_ptr(), batch.seq_pos0.data_ptr(), batch.seq_len_after.data_ptr(),
-                   slots.data_ptr(), cache.table_pointer, cache.table_width, cache.ring_pages, *cache.pointers, cache.n_pages,
-                   cache.n_slots, kernel_status(qkv.device).data_ptr(), _raw_stream()), "kv8_write")
+    _check(lib, fn(qkv.data_ptr(), row, batch.n_rows, n_heads, slots.numel(), 1 if batch.is_decode else 0, batch.seq_start.data_ptr(),
+                   batch.seq_pos0.data_ptr(), batch.seq_len_after.data_ptr(), slots.data_ptr(), record, _raw_stream()), "kv8_write")
 
 
 def kv8_read(cache, batch, first_page, k, v):
@@ -620,13 +632,13 @@ def kv8_read(cache, batch, first_page, k, v):
     assert first_page.dtype == torch.int32 and first_page.is_contiguous() and first_page.numel() >= n_seqs + 1
     assert k.shape == v.shape and k.dtype == v.dtype and k.is_contiguous() and v.is_contiguous()
     assert tuple(k.shape[1:]) == (cache.n_kv_heads, cache.tokens_per_page, cache.head_dim)
-    _kv8_fits("kv8_read", batch, cache)
+    record = _kv8_record("kv8_read", batch, cache)
+    _here("kv8_read", cache.k)
     if cache.ring_pages:
         raise KernelRefused("kv8_read: a cache under a window does not hold a sequence's first tokens")
-    fn = _typed(lib.abk_kv8_read, "ppppiiipiipppippiiipp")
-    _check(lib, fn(*cache.pointers, cache.n_kv_heads, cache.head_dim, KV8_FORMS[cache.form], cache.table_pointer, cache.table_width,
-                   n_seqs, batch.seq_len_after.data_ptr(), batch.seq_slot.data_ptr(), first_page.data_ptr(), k.shape[0], k.data_ptr(),
-                   v.data_ptr(), _dt(k), cache.n_pages, cache.n_slots, kernel_status(k.device).data_ptr(), _raw_stream()), "kv8_read")
+    fn = _typed(lib.abk_kv8_read, "pipppippip")
+    _check(lib, fn(record, n_seqs, batch.seq_len_after.data_ptr(), batch.seq_slot.data_ptr(), first_page.data_ptr(), k.shape[0],
+                   k.data_ptr(), v.data_ptr(), _dt(k), _raw_stream()), "kv8_read")
 
 
 def attention_kv8(qkv, out, n_heads, n_kv_heads, head_dim, scale, window, batch, cache, ws):
@@ -641,19 +653,17 @@ def attention_kv8(qkv, out, n_heads, n_kv_heads, head_dim, scale, window, batch,
     assert qkv.dtype == torch.bfloat16 and qkv.is_contiguous() and width == row and rows >= n
     rows, width = out.shape
     assert out.dtype == torch.bfloat16 and out.is_contiguous() and width == n_heads * head_dim and rows >= n
-    _kv8_fits("attention_kv8", batch, cache, n_kv_heads, head_dim)
+    record = _kv8_record("attention_kv8", batch, cache, n_kv_heads, head_dim)
     if cache.ring_pages and (not window or window + batch.longest - 1 > cache.ring_pages * cache.tokens_per_page):
         raise KernelRefused(f"attention_kv8: a ring of {cache.ring_pages} pages does not hold the keys that {batch.longest} new tokens of a "
                             f"sequence see under a window of {window}")
     floats = _kv8_part_floats(n_heads, n_kv_heads, head_dim, cache.device_index)
     parts = ws.get("attention_kv8_parts", (floats,), torch.float32)
-    _here("attention_kv8", parts)
-    fn = _typed(lib.abk_attention_kv8, "plpiiiiifipppppppppiiiiplpp")
-    _check(lib, fn(qkv.data_ptr(), row, out.data_ptr(), n, n_heads, n_kv_heads, head_dim, KV8_FORMS[cache.form], scale, window or 0,
-                   batch.token_seq.data_ptr(), batch.token_pos.data_ptr(), batch.seq_slot.data_ptr(), batch.seq_len_after.data_ptr(),
-                   *cache.pointers, cache.table_pointer, cache.table_width, cache.ring_pages, cache.n_pages, cache.n_slots,
-                   parts.data_ptr(), floats, kernel_status(qkv.device).data_ptr(), _raw_stream()), "attention_kv8",
-           kernels=2 * -(-n // 512))
+    _here("attention_kv8", parts, cache.k)
+    fn = _typed(lib.abk_attention_kv8, "plpiifipppppplp")
+    _check(lib, fn(qkv.data_ptr(), row, out.data_ptr(), n, n_heads, scale, window or 0, batch.token_seq.data_ptr(), batch.token_pos.data_ptr(),
+                   batch.seq_slot.data_ptr(), batch.seq_len_after.data_ptr(), record, parts.data_ptr(), floats, _raw_stream()),
+           "attention_kv8", kernels=2 * -(-n // 512))
 
 
 def attention(qkv, out, n_heads, n_kv_heads, head_dim, scale, window, batch, cache, from_step=False, ws=None, lists=None,
