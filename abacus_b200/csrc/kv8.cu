@@ -12,6 +12,7 @@
 #define ABK_DEFINE_ERROR
 #include "common.cuh"
 #include "kv8.cuh"
+#include "qkv_prep.cuh"
 
 #define KV8_WARPS 4
 
@@ -28,6 +29,30 @@ struct Kv8Write {
 };
 
 // A warp holds a block in pieces of 8 elements: token t, elements 8 c .., in piece i of a lane with 32 i + lane = t * HD / 8 + c.
+// A whole block into 8 bits, by a warp.
+template <int HD, int FORM>
+__device__ __forceinline__ void close_block(const Kv8Write &p, const uint4 *x, int slot, int head, int j, int pos0, int lane) {
+    constexpr int PIECES = KV8_BLOCK * HD / 256;
+    __nv_bfloat162 top2 = __floats2bfloat162_rn(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < PIECES; i++) {
+        const __nv_bfloat162 *h = (const __nv_bfloat162 *)&x[i];
+#pragma unroll
+        for (int e = 0; e < 4; e++) top2 = __hmax2_nan(top2, __habs2(h[e]));
+    }
+    const float2 two = __bfloat1622float2(top2);
+    const bool odd = __any_sync(0xffffffffu, !(two.x < INFINITY) || !(two.y < INFINITY));  // a value that is not finite
+    const float most = warp_max(fmaxf(two.x, two.y));
+    const Kv8Steps steps = kv8_steps<FORM>(odd ? 0.0f : most);
+    const int page = kv8_page(p.cache, p.n_pages, slot, pos0, p.status);
+    uint8_t *dst = (j == 0 ? p.k : p.v) + cache_offset(p.cache, page, head, p.n_kv_heads, pos0, HD);
+#pragma unroll
+    for (int i = 0; i < PIECES; i++) *(uint2 *)(dst + 8 * (32 * i + lane)) = kv8_pack<FORM>(x[i], steps);
+    if (lane == 0)
+        p.scales[(((long long)page * p.n_kv_heads + head) * 2 + j) * KV8_PAGE_BLOCKS + (pos0 % KV8_PAGE) / KV8_BLOCK] =
+            odd ? __int_as_float(0x7fffffff) : most / kv8_top<FORM>();
+}
+
 template <int HD, int FORM>
 __global__ void __launch_bounds__(32 * KV8_WARPS) kv8_write_kernel(Kv8Write p) {
     constexpr int LPR = HD / 8, PIECES = KV8_BLOCK * HD / 256;  // lanes to a row of 16-byte pieces
@@ -83,29 +108,68 @@ __global__ void __launch_bounds__(32 * KV8_WARPS) kv8_write_kernel(Kv8Write p) {
                 if (pos >= start && pos < after) *(uint4 *)(open + t * HD + 8 * c) = x[i];
             }
         } else if (cache_keeps(p.cache, pos0, after)) {
-            __nv_bfloat162 top2 = __floats2bfloat162_rn(0.0f, 0.0f);
-#pragma unroll
-            for (int i = 0; i < PIECES; i++) {
-                const __nv_bfloat162 *h = (const __nv_bfloat162 *)&x[i];
-#pragma unroll
-                for (int e = 0; e < 4; e++) top2 = __hmax2_nan(top2, __habs2(h[e]));
-            }
-            const float2 two = __bfloat1622float2(top2);
-            const bool odd = __any_sync(0xffffffffu, !(two.x < INFINITY) || !(two.y < INFINITY));  // a value that is not finite
-            const float most = warp_max(fmaxf(two.x, two.y));
-            const Kv8Steps steps = kv8_steps<FORM>(odd ? 0.0f : most);
-            const int page = kv8_page(p.cache, p.n_pages, slot, pos0, p.status);
-            uint8_t *dst = (j == 0 ? p.k : p.v) + cache_offset(p.cache, page, head, p.n_kv_heads, pos0, HD);
-#pragma unroll
-            for (int i = 0; i < PIECES; i++) *(uint2 *)(dst + 8 * (32 * i + lane)) = kv8_pack<FORM>(x[i], steps);
-            if (lane == 0)
-                p.scales[(((long long)page * p.n_kv_heads + head) * 2 + j) * KV8_PAGE_BLOCKS + (pos0 % KV8_PAGE) / KV8_BLOCK] =
-                    odd ? __int_as_float(0x7fffffff) : most / kv8_top<FORM>();
+            close_block<HD, FORM>(p, x, slot, head, j, pos0, lane);
         }
         if (!both || b != b0) return;
         __syncwarp();  // every lane has read its pieces of the old open block
         b = last;
     }
+}
+
+// A step of one token a sequence with its preparation (qkv_prep.cuh) taken in: q normed and rotated in place, the new token's key and value
+// into the open block, or, the sixteenth of its block, with the fifteen before it into 8 bits. A warp takes 256 / HD query heads of a
+// row, or one key or value head.
+struct Kv8Prepare {
+    __nv_bfloat16 *qkv;
+    const int *token_seq, *token_pos;
+    const float *q_norm, *k_norm;  // [HD]; null: no norm
+    const float *cos, *sin;        // [positions, HD / 2]; null: no rotation
+    float eps;
+};
+template <int HD, int FORM>
+__global__ void __launch_bounds__(32 * KV8_WARPS) kv8_prepare_write_kernel(Kv8Write p, Kv8Prepare e) {
+    constexpr int LPH = HD / 8, HPW = 32 / LPH, PIECES = KV8_BLOCK * HD / 256;
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.x, sub = lane / LPH, l = lane % LPH;
+    const int q_warps = (p.n_heads + HPW - 1) / HPW, unit = blockIdx.y * KV8_WARPS + warp;
+    if (unit >= q_warps + 2 * p.n_kv_heads) return;
+    const int seq = e.token_seq[r];
+    if (seq < 0) return;
+    const int pos = e.token_pos[r];
+    const bool upper = l >= LPH / 2;
+    float cs[8], sn[8];
+    if (e.cos) {
+        const int at = (upper ? l - LPH / 2 : l) * 8;
+        const float4 *c4 = (const float4 *)(e.cos + (long long)pos * (HD / 2) + at), *s4 = (const float4 *)(e.sin + (long long)pos * (HD / 2) + at);
+        const float4 c0 = c4[0], c1 = c4[1], s0 = s4[0], s1 = s4[1];
+        cs[0] = c0.x, cs[1] = c0.y, cs[2] = c0.z, cs[3] = c0.w, cs[4] = c1.x, cs[5] = c1.y, cs[6] = c1.z, cs[7] = c1.w;
+        sn[0] = s0.x, sn[1] = s0.y, sn[2] = s0.z, sn[3] = s0.w, sn[4] = s1.x, sn[5] = s1.y, sn[6] = s1.z, sn[7] = s1.w;
+    }
+    __nv_bfloat16 *row = e.qkv + (long long)r * p.row + 8 * l;
+    if (unit < q_warps) {
+        const int h = unit * HPW + sub;
+        const uint4 raw = h < p.n_heads ? *(const uint4 *)(row + (long long)h * HD) : make_uint4(0, 0, 0, 0);
+        const uint4 done = prep_head_values<HD>(raw, true, e.q_norm, e.eps, e.cos != nullptr, l, upper, cs, sn);
+        if (h < p.n_heads) *(uint4 *)(row + (long long)h * HD) = done;
+        return;
+    }
+    const int which = unit - q_warps, j = which / p.n_kv_heads, head = which - j * p.n_kv_heads;
+    const uint4 raw = *(const uint4 *)(row + (long long)(p.n_heads + which) * HD);
+    const uint4 mine = prep_head_values<HD>(raw, j == 0, e.k_norm, e.eps, e.cos != nullptr, l, upper, cs, sn);  // (the same in every run of LPH lanes)
+    if ((unsigned)p.seq_slot[seq] >= (unsigned)p.n_slots) {  // nothing is written
+        kv8_slot(p.seq_slot[seq], p.n_slots, p.status);
+        return;
+    }
+    const int slot = p.seq_slot[seq], t = pos % KV8_BLOCK;
+    __nv_bfloat16 *open = p.open + (((long long)slot * 2 + j) * p.n_kv_heads + head) * (KV8_BLOCK * HD);
+    if (t < KV8_BLOCK - 1) {
+        if (sub == 0) *(uint4 *)(open + t * HD + 8 * l) = mine;
+        return;
+    }
+    uint4 x[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; i++) x[i] = (32 * i + lane) / LPH < KV8_BLOCK - 1 ? *(const uint4 *)(open + 8 * (32 * i + lane)) : mine;
+    close_block<HD, FORM>(p, x, slot, head, j, pos - t, lane);
 }
 
 struct Kv8Read {
@@ -178,6 +242,34 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8Read p) {
 }
 
 extern "C" int abk_kv8_cache_bytes() { return (int)sizeof(Kv8Cache); }
+static Kv8Write kv8_write_args(const void *qkv, long long row, int n_heads, const int *seq_slot, const Kv8Cache &c) {
+    Kv8Write p = {};
+    p.qkv = (const __nv_bfloat16 *)qkv, p.row = row, p.n_heads = n_heads, p.n_kv_heads = c.n_kv_heads, p.seq_slot = seq_slot;
+    p.cache.page_table = c.page_table, p.cache.table_width = c.table_width, p.cache.ring_pages = c.ring_pages;
+    p.cache.tokens_per_page = KV8_PAGE, p.k = (uint8_t *)c.k, p.v = (uint8_t *)c.v, p.scales = c.scales, p.open = (__nv_bfloat16 *)c.open;
+    p.n_pages = c.n_pages, p.n_slots = c.n_slots, p.status = c.status;
+    return p;
+}
+// Rows of one token each. q_norm, k_norm, cos and sin may be null (no norm, no rotation).
+extern "C" int abk_kv8_prepare_write(void *qkv, long long row, int n_rows, int n_heads, const int *token_seq, const int *token_pos,
+                                     const int *seq_slot, const float *q_norm, const float *k_norm, float eps, const float *cos,
+                                     const float *sin, const Kv8Cache *cache, void *stream) {
+    const Kv8Cache &c = *cache;
+    if (n_rows <= 0) return 0;
+    if (c.head_dim != 64 && c.head_dim != 128) ABK_REFUSE("kv8_write: head_dim %d is not 64 or 128", c.head_dim);
+    if (c.form != KV8_INT8 && c.form != KV8_E4M3) ABK_REFUSE("kv8_write: no 8-bit form %d", c.form);
+    if ((((uintptr_t)qkv | (uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)c.open | (uintptr_t)q_norm | (uintptr_t)k_norm | (uintptr_t)cos |
+          (uintptr_t)sin) & 15) || (row & 7) || ((uintptr_t)c.scales & 3) || !cos != !sin)
+        ABK_REFUSE("kv8_write: rows, norms, angles, pools and open blocks must be 16-byte aligned");
+    const int warps = (n_heads + 256 / c.head_dim - 1) / (256 / c.head_dim) + 2 * c.n_kv_heads, groups = (warps + KV8_WARPS - 1) / KV8_WARPS;
+    if (c.n_kv_heads < 1 || n_heads < 1 || groups > 65535) ABK_REFUSE("kv8_write: %d heads, %d kv heads", n_heads, c.n_kv_heads);
+    const Kv8Write p = kv8_write_args(qkv, row, n_heads, seq_slot, c);
+    const Kv8Prepare e = {(__nv_bfloat16 *)qkv, token_seq, token_pos, q_norm, k_norm, cos, sin, eps};
+    auto go = [&](auto kernel) { abk_launch(kernel, dim3(n_rows, groups), dim3(32 * KV8_WARPS), 0, (cudaStream_t)stream, p, e); };
+    if (c.head_dim == 64) c.form == KV8_INT8 ? go(kv8_prepare_write_kernel<64, KV8_INT8>) : go(kv8_prepare_write_kernel<64, KV8_E4M3>);
+    else c.form == KV8_INT8 ? go(kv8_prepare_write_kernel<128, KV8_INT8>) : go(kv8_prepare_write_kernel<128, KV8_E4M3>);
+    return ABK_LAUNCH_RESULT();
+}
 extern "C" int abk_kv8_write(const void *qkv, long long row, int n_rows, int n_heads, int n_seqs, int one_each, const int *seq_start,
                              const int *seq_pos0, const int *seq_len_after, const int *seq_slot, const Kv8Cache *cache, void *stream) {
     const Kv8Cache &c = *cache;
@@ -189,12 +281,8 @@ extern "C" int abk_kv8_write(const void *qkv, long long row, int n_rows, int n_h
     const int units = one_each ? n_seqs : n_rows / KV8_BLOCK + 2 * n_seqs + 1;
     const int groups = (2 * c.n_kv_heads + KV8_WARPS - 1) / KV8_WARPS;
     if (c.n_kv_heads < 1 || groups > 65535) ABK_REFUSE("kv8_write: %d kv heads", c.n_kv_heads);
-    Kv8Write p;
-    p.qkv = (const __nv_bfloat16 *)qkv, p.row = row, p.n_heads = n_heads, p.n_kv_heads = c.n_kv_heads, p.n_seqs = n_seqs;
-    p.one_each = one_each, p.seq_start = seq_start, p.seq_pos0 = seq_pos0, p.seq_len_after = seq_len_after;
-    p.seq_slot = seq_slot, p.cache.page_table = c.page_table, p.cache.table_width = c.table_width, p.cache.ring_pages = c.ring_pages;
-    p.cache.tokens_per_page = KV8_PAGE, p.k = (uint8_t *)c.k, p.v = (uint8_t *)c.v, p.scales = c.scales, p.open = (__nv_bfloat16 *)c.open;
-    p.n_pages = c.n_pages, p.n_slots = c.n_slots, p.status = c.status;
+    Kv8Write p = kv8_write_args(qkv, row, n_heads, seq_slot, c);
+    p.n_seqs = n_seqs, p.one_each = one_each, p.seq_start = seq_start, p.seq_pos0 = seq_pos0, p.seq_len_after = seq_len_after;
     const dim3 grid(units, groups), block(32 * KV8_WARPS);
     auto go = [&](auto kernel) { abk_launch(kernel, grid, block, 0, (cudaStream_t)stream, p); };
     if (c.head_dim == 64) c.form == KV8_INT8 ? go(kv8_write_kernel<64, KV8_INT8>) : go(kv8_write_kernel<64, KV8_E4M3>);

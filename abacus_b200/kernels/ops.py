@@ -601,12 +601,22 @@ def _kv8_part_floats(n_heads, n_kv_heads, head_dim, device):
     return lib.abk_attention_kv8_part_floats(n_heads, n_kv_heads, head_dim)
 
 
-def kv8_write(qkv, n_heads, n_kv_heads, head_dim, batch, cache, row=None):
+def kv8_write_prepares(qkv, cos, sin, q_norm, k_norm, rotary_dim, interleaved, head_dim):
+    """Whether kv8_write takes the q/k/v preparation of a decode step into its own kernel: the rotation over the whole head in halves
+    (or none), norms and angles in float32, everything 16-byte aligned."""
+    tensors = [t for t in (qkv, cos, sin, q_norm, k_norm) if t is not None]
+    return ((cos is None or (rotary_dim == head_dim and not interleaved)) and all(t.data_ptr() % 16 == 0 for t in tensors)
+            and all(t is None or t.dtype == torch.float32 for t in (q_norm, k_norm, cos, sin)))
+
+
+def kv8_write(qkv, n_heads, n_kv_heads, head_dim, batch, cache, row=None, prepare=None):
     """The keys and values of the step's rows go into an 8-bit cache (cache.LayerKV8): blocks of 16 tokens that the step
     completes into 8 bits with their scales, the last tokens of a sequence that do not fill a block into its open block.
     qkv bfloat16 [rows, (n_heads + 2 n_kv_heads) head_dim], prepared (see qkv_prep); what a sequence holds before the
     step (batch.seq_pos0 tokens) must be in the cache, and no slot may be in the step twice. The same step a second time is the same step only for single tokens, and where
-    no sequence both completes a block it had begun and begins another."""
+    no sequence both completes a block it had begun and begins another.
+    prepare (a step of single tokens): dict(q_norm, k_norm, eps, cos, sin) where kv8_write_prepares() says so: qkv is as the product left it,
+    and the kernel norms and rotates q in place, and the keys on their way (src/model.c:247-259)."""
     _here("kv8_write", qkv, batch.seq_slot)
     lib = load_module("kv8")
     heads_size = (n_heads + 2 * n_kv_heads) * head_dim
@@ -615,6 +625,17 @@ def kv8_write(qkv, n_heads, n_kv_heads, head_dim, batch, cache, row=None):
     assert qkv.dtype == torch.bfloat16 and qkv.is_contiguous() and width == row >= heads_size and n >= batch.n_rows
     record = _kv8_record("kv8_write", batch, cache, n_kv_heads, head_dim)
     _here("kv8_write", cache.k)
+    if prepare is not None:
+        cos = prepare["cos"]
+        if not batch.is_decode:
+            raise KernelRefused("kv8_write: only a step of single tokens is prepared on the way")
+        if cos is not None and batch.max_position >= cos.shape[0]:
+            raise KernelError(f"position {batch.max_position} is beyond the rotary table of {cos.shape[0]} positions")
+        fn = _typed(lib.abk_kv8_prepare_write, "pliipppppfpppp")
+        _check(lib, fn(qkv.data_ptr(), row, batch.n_rows, n_heads, batch.token_seq.data_ptr(), batch.token_pos.data_ptr(),
+                       batch.seq_slot.data_ptr(), _at(prepare["q_norm"]), _at(prepare["k_norm"]), prepare["eps"] or 0.0, _at(cos),
+                       _at(prepare["sin"]), record, _raw_stream()), "kv8_write")
+        return
     fn = _typed(lib.abk_kv8_write, "pliiiipppppp")
     slots = batch.seq_slot
     _check(lib, fn(qkv.data_ptr(), row, batch.n_rows, n_heads, slots.numel(), 1 if batch.is_decode else 0, batch.seq_start.data_ptr(),

@@ -189,11 +189,16 @@ class Attention:
         qkv = ws.get("qkv", (n, self.row), self.ctx.dtype)
         att = ws.get("att", (n, s.n_heads * self.v_dim), self.ctx.dtype)
         (self.qkv_proj if writes else self.q_proj).forward(xn, qkv if writes else qkv[:, :self.q_size], n)
-        rotary_dim = self.position.rotary_dim if self.position else 0
-        ops.qkv_prep(qkv, s.n_heads, s.n_kv_heads, s.head_dim, batch, self.q_norm, self.k_norm, s.qk_norm_eps, self.cos, self.sin, rotary_dim,
-                     self.position.interleaved if self.position else False, None, q_only=not writes)
+        rotary_dim, interleaved = (self.position.rotary_dim, self.position.interleaved) if self.position else (0, False)
+        prepare = None
+        if (DECODE_PREPARES and writes and batch.is_decode
+                and ops.kv8_write_prepares(qkv, self.cos, self.sin, self.q_norm, self.k_norm, rotary_dim, interleaved, s.head_dim)):
+            prepare = dict(q_norm=self.q_norm, k_norm=self.k_norm, eps=s.qk_norm_eps, cos=self.cos, sin=self.sin)
+        else:
+            ops.qkv_prep(qkv, s.n_heads, s.n_kv_heads, s.head_dim, batch, self.q_norm, self.k_norm, s.qk_norm_eps, self.cos, self.sin,
+                         rotary_dim, interleaved, None, q_only=not writes)
         if writes:
-            ops.kv8_write(qkv, s.n_heads, s.n_kv_heads, s.head_dim, batch, cache.kv)
+            ops.kv8_write(qkv, s.n_heads, s.n_kv_heads, s.head_dim, batch, cache.kv, prepare=prepare)
         heads = (s.n_heads, s.n_kv_heads, s.head_dim, s.scale)
         if writes and not batch.is_decode and not batch.any_continuation:
             if ops.attention_window_takes(qkv, s.head_dim, s.head_dim, s.n_heads, s.n_kv_heads):

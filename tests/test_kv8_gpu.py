@@ -234,6 +234,58 @@ def test_numbers_of_every_size(ops, form):
                 assert torch.equal(blocks[i], wanted[i]), i
 
 
+@pytest.mark.parametrize("form", ["int8", "e4m3"])
+@pytest.mark.parametrize("heads, kv_heads, dim, norms, angles", [(4, 2, 128, True, True), (5, 1, 64, True, False), (7, 7, 64, False, True), (2, 1, 128, False, False)])
+def test_a_decode_step_prepared_on_its_way(ops, heads, kv_heads, dim, norms, angles, form):
+    """kv8_write(prepare=..) leaves the bits that qkv_prep and kv8_write leave, through whole blocks, padded rows alone; several tokens a
+    sequence and positions beyond the table are refused."""
+    from abacus_b200.engine.batch import Sequence, StepBatch
+    runs = [Run(heads, kv_heads, dim, form, slots=3, pages=12) for _ in range(2)]
+    g = torch.Generator(device="cuda").manual_seed(dim + heads)
+    q_norm, k_norm = (1.0 + 0.2 * torch.randn(dim, generator=g, device="cuda") for _ in range(2)) if norms else (None, None)
+    cos = sin = None
+    if angles:
+        a = torch.rand((256, dim // 2), generator=g, device="cuda") * 6.0
+        cos, sin = a.cos(), a.sin()
+    prepare = dict(q_norm=q_norm, k_norm=k_norm, eps=1e-6, cos=cos, sin=sin)
+    assert ops.kv8_write_prepares(torch.zeros(8, dtype=torch.bfloat16, device="cuda"), cos, sin, q_norm, k_norm, dim, False, dim)
+    width = (heads + 2 * kv_heads) * dim
+    starts = (0, 9, 15)
+    for run in runs:
+        for s in starts:
+            slot = run.open()
+            if s:
+                run.g.manual_seed(s)
+                run.write(ops, [(slot, s)], run.rows(s))
+    for i in range(40):
+        qkv = torch.randn((4, width), generator=g, device="cuda").to(torch.bfloat16)
+        rows = []
+        for run, fused in zip(runs, (True, False)):
+            batch = StepBatch(4, 4, 1, "cuda").fill([Sequence(j, [0], s + i, []) for j, s in enumerate(starts)])
+            for j, s in enumerate(starts):
+                run.cache.reserve(j, s + i + 1)
+            x = qkv.clone()
+            if fused:
+                ops.kv8_write(x, heads, kv_heads, dim, batch, run.kv, prepare=prepare)
+            else:
+                ops.qkv_prep(x, heads, kv_heads, dim, batch, q_norm, k_norm, 1e-6, cos, sin, dim if angles else 0, False, None)
+                ops.kv8_write(x, heads, kv_heads, dim, batch, run.kv)
+            rows.append(x)
+        assert torch.equal(rows[0][:3, :heads * dim], rows[1][:3, :heads * dim]) and torch.equal(rows[0][3], qkv[3])
+        bits = [(r.kv.k.view(torch.uint8), r.kv.v.view(torch.uint8), r.kv.scales.view(torch.int32)) for r in runs]
+        assert all(torch.equal(x, y) for x, y in zip(*bits))
+        for j, s in enumerate(starts):  # the open block's tokens (behind its end anything may lie)
+            n = (s + i + 1) % 16
+            assert torch.equal(runs[0].kv.open[j, :, :, :n].view(torch.int16), runs[1].kv.open[j, :, :, :n].view(torch.int16))
+    with pytest.raises(ops.KernelRefused, match="single tokens"):
+        several = StepBatch(2, 1, 1, "cuda").fill([Sequence(0, [0, 0], 40, [])], exact=True)
+        ops.kv8_write(qkv, heads, kv_heads, dim, several, runs[0].kv, prepare=prepare)
+    if angles:
+        with pytest.raises(ops.KernelError, match="rotary table"):
+            far = StepBatch(1, 1, 1, "cuda").fill([Sequence(0, [0], 256, [])], exact=True)
+            ops.kv8_write(qkv, heads, kv_heads, dim, far, runs[0].kv, prepare=prepare)
+
+
 def test_padding_streams_and_graphs(ops):
     """A captured decode step of more rows than it brings: padded rows become zeros and write nothing; replayed for a step that closes
     blocks, with a second graph captured between; the attention call on another stream."""
