@@ -51,7 +51,7 @@ struct AttnKv8 {
     int n_heads, n_kv_heads, runs;
     float scale_log2;
     int window;
-    const int *token_seq, *token_pos, *seq_slot, *seq_len_after;
+    const int *token_seq, *token_pos, *seq_slot, *seq_pos0, *seq_len_after;
     PagedCache cache;
     const float *scales;
     const __nv_bfloat16 *open;
@@ -144,6 +144,7 @@ __global__ void __launch_bounds__(KV8_THREADS, KV8_CTAS) attention_kv8_kernel(co
     __shared__ uint64_t full[KV8_MAX_STAGES], empty[KV8_MAX_STAGES];
     __shared__ int first_unit[KV8_ROWS + 1];  // of a pair of the rows before a row
     __shared__ int4 row_info[KV8_ROWS];       // position, slot, blocks in 8 bits, first visible key
+    __shared__ int fresh_page[KV8_ROWS];      // the first page that the step itself writes to
     __shared__ int failed;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -153,11 +154,13 @@ __global__ void __launch_bounds__(KV8_THREADS, KV8_CTAS) attention_kv8_kernel(co
         tc::mbar_init_fence();
         tc::tma_prefetch_map(&k_map), tc::tma_prefetch_map(&v_map);
     }
-    pdl_wait();
+    // Before pdl_wait() only what kernels further back than the one just before this wrote is read: the step's index arrays and
+    // the page table, and (by the copy warp) the pages that the step's own tokens, which that kernel may still be writing, are not in.
     for (int r = threadIdx.x; r < p.n_rows; r += KV8_THREADS) {
         const int seq = p.token_seq[p.first_row + r], pos = p.token_pos[p.first_row + r];
         const int lo = p.window > 0 && pos - p.window + 1 > 0 ? pos - p.window + 1 : 0;
         first_unit[r + 1] = seq < 0 ? 0 : units_of(pos, lo);
+        fresh_page[r] = seq < 0 ? 0 : p.seq_pos0[seq] / KV8_PAGE;
         row_info[r] = seq < 0 ? make_int4(0, 0, 0, 0) : make_int4(pos, kv8_slot(p.seq_slot[seq], p.n_slots, p.status), p.seq_len_after[seq] / KV8_BLOCK, lo);
     }
     __syncthreads();
@@ -178,7 +181,10 @@ __global__ void __launch_bounds__(KV8_THREADS, KV8_CTAS) attention_kv8_kernel(co
     __syncthreads();
     const long long units = (long long)p.pairs * first_unit[p.n_rows], per = (units + gridDim.x - 1) / gridDim.x;
     const long long begin = per * blockIdx.x, end = min(units, begin + per);
-    if (begin >= end) return;
+    if (begin >= end) {
+        pdl_wait();
+        return;
+    }
     // the run of pages that starts at `unit`
     auto segment_at = [&](long long unit) {
         int lo = 0, hi = p.n_rows;  // the last row that starts at or before the unit (rows without pages start where the next one does)
@@ -197,7 +203,7 @@ __global__ void __launch_bounds__(KV8_THREADS, KV8_CTAS) attention_kv8_kernel(co
 
     if (warp == 4) {
         int issued = 0;
-        bool go = true;
+        bool go = true, waited = false;
         for (long long unit = begin; unit < end && go;) {
             const Kv8Segment seg = segment_at(unit);
             const int4 info = row_info[seg.row];
@@ -209,6 +215,7 @@ __global__ void __launch_bounds__(KV8_THREADS, KV8_CTAS) attention_kv8_kernel(co
                 for (int i = 0; i < n && go; i++, issued++) {
                     const long long tile = (long long)__shfl_sync(0xffffffffu, page_lane, i) * p.n_kv_heads + kvh;
                     int bad = 0;
+                    if (!waited && first + base + i >= fresh_page[seg.row]) pdl_wait(), waited = true;
                     if (lane == 0) {
                         const int s = issued % stages;
                         if (!tc::mbar_wait(&empty[s], ((issued / stages) & 1) ^ 1)) {
@@ -225,6 +232,7 @@ __global__ void __launch_bounds__(KV8_THREADS, KV8_CTAS) attention_kv8_kernel(co
             }
             unit += seg.units;
         }
+        pdl_wait();
         if (!go && lane == 0) {  // let the copies in flight land before the CTA's memory goes away
             failed = 1;
             issued--;  // the copy that was not issued
@@ -234,6 +242,7 @@ __global__ void __launch_bounds__(KV8_THREADS, KV8_CTAS) attention_kv8_kernel(co
         const int i8 = lane >> 2, c4 = 4 * (lane & 3), j8 = lane >> 3, r8 = lane & 7;
         bool ok = true;
         int s = 0, phase = 0, done = 0;
+        pdl_wait();
         for (long long unit = begin; unit < end && ok;) {
             const Kv8Segment seg = segment_at(unit);
             unit += seg.units;
@@ -539,8 +548,8 @@ extern "C" long long abk_attention_kv8_part_floats(int n_heads, int n_kv_heads, 
     return 2ll * KV8_CTAS * abk_sm_count() * (group < KV8_HEADS ? group : KV8_HEADS) * (head_dim + 4);
 }
 extern "C" int abk_attention_kv8(const void *q, long long q_row, void *out, int n_rows, int n_heads, float scale, int window,
-                                 const int *token_seq, const int *token_pos, const int *seq_slot, const int *seq_len_after,
-                                 const Kv8Cache *cache, float *parts, long long part_floats, void *stream) {
+                                 const int *token_seq, const int *token_pos, const int *seq_slot, const int *seq_pos0,
+                                 const int *seq_len_after, const Kv8Cache *cache, float *parts, long long part_floats, void *stream) {
     const Kv8Cache &c = *cache;
     const int head_dim = c.head_dim, n_kv_heads = c.n_kv_heads, form = c.form;
     if (n_rows <= 0) return 0;
@@ -562,7 +571,7 @@ extern "C" int abk_attention_kv8(const void *q, long long q_row, void *out, int 
     AttnKv8 p;
     p.q = (const __nv_bfloat16 *)q, p.q_row = q_row, p.out = (__nv_bfloat16 *)out, p.n_heads = n_heads, p.n_kv_heads = n_kv_heads;
     p.scale_log2 = scale * 1.4426950408889634f, p.window = window, p.token_seq = token_seq, p.token_pos = token_pos;
-    p.seq_slot = seq_slot, p.seq_len_after = seq_len_after, p.cache.page_table = c.page_table, p.cache.table_width = c.table_width;
+    p.seq_slot = seq_slot, p.seq_pos0 = seq_pos0, p.seq_len_after = seq_len_after, p.cache.page_table = c.page_table, p.cache.table_width = c.table_width;
     p.cache.ring_pages = c.ring_pages, p.cache.tokens_per_page = KV8_PAGE, p.scales = c.scales, p.open = (const __nv_bfloat16 *)c.open;
     p.n_pages = c.n_pages, p.n_slots = c.n_slots, p.status = c.status, p.runs = runs, p.pairs = n_kv_heads * runs, p.parts = parts;
     void (*kernel)(CUtensorMap, CUtensorMap, AttnKv8) = nullptr;
@@ -574,7 +583,7 @@ extern "C" int abk_attention_kv8(const void *q, long long q_row, void *out, int 
     if (head_dim == 64) kernel = heads <= 8 ? of_dim(integral_constant<int, 64>(), integral_constant<int, 1>()) : of_dim(integral_constant<int, 64>(), integral_constant<int, 2>());
     else kernel = heads <= 8 ? of_dim(integral_constant<int, 128>(), integral_constant<int, 1>()) : of_dim(integral_constant<int, 128>(), integral_constant<int, 2>());
     const int stage = 2 * KV8_PAGE * head_dim + 2 * KV8_PAGE_BLOCKS * 4, fold_bytes = 4 * heads * (head_dim + 4) * 4 + 1024;
-    p.stages = ((226 - 12 * KV8_CTAS) * 1024 / KV8_CTAS - fold_bytes) / stage;  // (12 KB: a CTA's table of rows, and what every CTA takes)
+    p.stages = ((226 - 14 * KV8_CTAS) * 1024 / KV8_CTAS - fold_bytes) / stage;  // (14 KB: a CTA's table of rows, and what every CTA takes)
     if (p.stages > KV8_MAX_STAGES) p.stages = KV8_MAX_STAGES;
     const int smem = p.stages * stage + fold_bytes;
     const cudaError_t e = abk_allow_shared_memory((const void *)kernel, smem);

@@ -681,9 +681,9 @@ def attention_kv8(qkv, out, n_heads, n_kv_heads, head_dim, scale, window, batch,
     floats = _kv8_part_floats(n_heads, n_kv_heads, head_dim, cache.device_index)
     parts = ws.get("attention_kv8_parts", (floats,), torch.float32)
     _here("attention_kv8", parts, cache.k)
-    fn = _typed(lib.abk_attention_kv8, "plpiifipppppplp")
+    fn = _typed(lib.abk_attention_kv8, "plpiifippppppplp")
     _check(lib, fn(qkv.data_ptr(), row, out.data_ptr(), n, n_heads, scale, window or 0, batch.token_seq.data_ptr(), batch.token_pos.data_ptr(),
-                   batch.seq_slot.data_ptr(), batch.seq_len_after.data_ptr(), record, parts.data_ptr(), floats, _raw_stream()),
+                   batch.seq_slot.data_ptr(), batch.seq_pos0.data_ptr(), batch.seq_len_after.data_ptr(), record, parts.data_ptr(), floats, _raw_stream()),
            "attention_kv8", kernels=2 * -(-n // 512))
 
 
