@@ -13,11 +13,11 @@
 // sustains 1,377 under the power cap); 4,999 rows of 4,096 in 5,035, 1,236 TFLOP/s (4,849 in one segment). The eight warps that read need 5.5 instructions and one exponential a logit:
 // at K = 1,024 half of the time that the tensor cores take for it.
 //
-// Few rows (up to LP_FEW): w is all there is to read, and a tile of 256 rows of x of which a few are there costs the tensor cores as much
+// Few rows (up to LP_FEW, few_wins): w is all there is to read, and a tile of 256 rows of x of which a few are there costs the tensor cores as much
 // time as w takes to come. So the operands change sides: a CTA's tile is up to 128 rows of w, the rows of x are its 16 to 64 columns, and
 // a thread that reads the accumulator has one token of the vocabulary and keeps the sums of 32 rows of x in registers over all of its
 // CTA's tiles. The tiles are as high as makes all CTAs take the same number of full ones (115 for 151,936 on 148 SMs). 37 rows of 1,024
-// against 151,936: 64 us, with the tiles above 83 (the matrix at the copy rate: 48).
+// against 151,936: 61 us, with the tiles above 77 (the matrix at the copy rate: 48).
 #define ABK_DEFINE_ERROR
 #include "common.cuh"
 #include "tc_common.cuh"
@@ -352,6 +352,7 @@ __global__ void __launch_bounds__(LP_THREADS) gemm_logprobs_few_kernel(const __g
     } else {
         // warp w reads lanes 32 * (w % 4) .. + 31 of the accumulator, tokens of the vocabulary, and 32 of the rows of x
         constexpr int COLS = LP_FEW / 2;
+        static_assert(COLS == 32, "a column a lane at the end");
         const int quarter = warp & 3, half = (warp - 2) >> 2, col0 = half * COLS;
         float m[COLS], l[COLS], tt[COLS];
 #pragma unroll
@@ -396,12 +397,23 @@ __global__ void __launch_bounds__(LP_THREADS) gemm_logprobs_few_kernel(const __g
             }
             __syncwarp();
         }
+        // The lanes' sums of 32 columns joined to a column a lane: at every step a lane gives away half of its columns and takes the
+        // other lane's share of the half it keeps (31 joins a lane, where every column for itself would take 160).
 #pragma unroll
-        for (int j = 0; j < COLS; j++) {
-            if (col0 + j >= g.rows) continue;
-            const RowSums s = joined_lanes({m[j], l[j], tt[j], 0.0f}, 16);
-            if (lane == 0) sums_s[quarter][col0 + j] = make_float4(s.m, s.l, s.t, 0.0f);
+        for (int n = COLS / 2; n > 0; n >>= 1) {
+            const bool upper = lane & n;
+#pragma unroll
+            for (int j = 0; j < n; j++) {
+                const RowSums keep = {upper ? m[j + n] : m[j], upper ? l[j + n] : l[j], upper ? tt[j + n] : tt[j], 0.0f};
+                RowSums come;
+                come.m = __shfl_xor_sync(0xffffffffu, upper ? m[j] : m[j + n], n);
+                come.l = __shfl_xor_sync(0xffffffffu, upper ? l[j] : l[j + n], n);
+                come.t = __shfl_xor_sync(0xffffffffu, upper ? tt[j] : tt[j + n], n);
+                const RowSums both = joined(keep, come);
+                m[j] = both.m, l[j] = both.l, tt[j] = both.t;
+            }
         }
+        sums_s[quarter][col0 + lane] = make_float4(m[0], l[0], tt[0], 0.0f);
     }
     tc::fence_before_sync();
     __syncthreads();
@@ -446,6 +458,12 @@ __global__ void __launch_bounds__(128) logprobs_join_kernel(const float4 *__rest
     }
 }
 
+// Whether few rows against this matrix go to the kernel made for them: the fewer the rows and the larger the matrix, the longer its reading
+// lasts beside what that kernel does at its end. us, that kernel and the one above: 151,936 x 1,024 with 1 row 55 and 84, 33 60 and 74, 64 63 and
+// 65; x 4,096 with 64 203 and 254; 64,000 x 1,024 with 16 31 and 35, 48 35 and 36, 64 36 and 33; 32,000 x 1,024 with 16 18.6 and 21,
+// 48 22.2 and 21.8; 16,000 x 1,024 with 1 12.5 and 15.5, 16 13.5 and 13.6, 33 15.4 and 13.7; 8,000 x 512 with 16 10.7 and 10.1.
+static bool few_wins(int M, int V, int K) { return M <= LP_FEW && (long long)M * 1400000 <= (long long)V * K; }
+
 // Floats of memory for the sums of `rows` rows: 4 a row and pair of CTAs, and the given tokens' logits.
 extern "C" long long abk_gemm_logprobs_floats(int rows) {
     const long long most = rows < LP_MOST_ROWS ? rows : LP_MOST_ROWS;
@@ -460,7 +478,7 @@ extern "C" int abk_gemm_logprobs(const void *x, const void *w, int M, int V, int
     if (floats < abk_gemm_logprobs_floats(M)) ABK_REFUSE("gemm_logprobs: room for %lld floats is too little", floats);
     const int k_blocks = (K + LP_K - 1) / LP_K, pieces = (k_blocks + LP_SEGMENT - 1) / LP_SEGMENT;  // segments as equal as whole blocks allow
     const int segment_blocks = (k_blocks + pieces - 1) / pieces, segments = (k_blocks + segment_blocks - 1) / segment_blocks;
-    if (M <= LP_FEW) {
+    if (few_wins(M, V, K)) {
         const int ctas = abk_sm_count();
         FewLogProbs g;
         const long long waves = (V + (long long)ctas * LP_ROWS - 1) / ((long long)ctas * LP_ROWS);

@@ -363,7 +363,8 @@ extern "C" int abk_token_logprobs(const void *logits, int dtype, long long strid
         ABK_REFUSE("token_logprobs: %d most likely tokens of a vocabulary of %d (at most %d)", top, vocab, LOGPROBS_MAX_TOP);
     const int size = dtype == ABK_F32 ? 4 : 2, piece = 16 / size;
     if ((uintptr_t)logits % size) ABK_REFUSE("token_logprobs: logits that are not aligned to their own size");
-    // CTAs to a row: until the GPU is full (4 to an SM), in slices of at least 4,096 elements, as many as a cluster holds
+    // CTAs to a row: until the GPU is full (4 to an SM; 8: 512 rows of 151,936 with 5 alternatives 79 us, not 71), in slices of at least 4,096
+    // elements, as many as a cluster holds (8 rows with 20 alternatives: one CTA a row 33 us, 16 of them 13)
     const int full = 4 * abk_sm_count();
     int splits = 1;
     while (splits < LOGPROBS_MAX_SPLITS && (long long)n_rows * splits * 2 <= full && vocab / (splits * 2) >= 4096) splits *= 2;

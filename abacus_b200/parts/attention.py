@@ -30,7 +30,9 @@ from .linear import Linear
 # launch less in every layer. ABACUS_DECODE_PREPARES=0 keeps the preparation a kernel of its own (for comparison).
 DECODE_PREPARES = os.environ.get("ABACUS_DECODE_PREPARES", "1") != "0"
 # Tokens a sequence brings up to which a step that goes on with it attends to an 8-bit cache row by row, each row reading all its keys;
-# beyond that the sequences' keys and values are read back into 16-bit pages first, for the prompt kernel.
+# beyond that the sequences' keys and values are read back into 16-bit pages first, for the prompt kernel. us, row by row and read back, 32
+# query and 8 kv heads of 128: 4 sequences behind 4,096 tokens with 4 new ones each 31 and 65, 8 52 and 66, 16 94 and 65, 32 179 and 67;
+# one behind 16,384: 8 50 and 147, 16 89 and 146, 32 167 and 148; 16 behind 512: 4 27 and 40, 8 46 and 41, 16 81 and 41.
 KV8_ROWS_UP_TO = 8
 # The q/k/v product of a long prompt step can do the same in its epilogue (heads of 128): a kernel and a pass over
 # q, k and v less. ABACUS_PRODUCT_PREPARES=0 keeps the preparation a kernel of its own (for comparison).

@@ -175,10 +175,11 @@ def test_refusals(ops):
 
 @pytest.mark.parametrize("m, vocab, k", [(1, 1, 8), (1, 300, 64), (5, 257, 72), (37, 5003, 200), (128, 1024, 128), (129, 999, 64), (256, 4097, 264),
                                          (300, 20011, 1024), (2049, 3001, 136), (2500, 515, 192), (33, 2000, 2048), (70, 3333, 2056), (40, 1500, 4096),
-                                         (16390, 260, 64)])
+                                         (16390, 260, 64), (1, 5000, 1024), (16, 20000, 1160), (17, 37777, 648), (33, 12001, 4096), (50, 30011, 2400),
+                                         (64, 151936, 640), (64, 22003, 4160)])
 def test_logprobs_behind_the_product(ops, m, vocab, k):
     """Row tiles that end anywhere, groups of them, vocabularies that end inside a tile, fewer tiles than pairs of SMs, K that is one
-    segment, two, or ends inside a block; rows beyond m are left alone.
+    segment, two, or ends inside a block; few rows against large matrices, which run on a kernel of their own; rows beyond m are left alone.
 
     A logit is off by K half steps of sum |x w| (the tensor cores cut off instead of rounding: a step of 2^-23 of the running sum for
     every 16 products, counted here as K / 16 + 16 of them); a log probability by twice that of the logits that matter."""
