@@ -473,7 +473,7 @@ __global__ void __launch_bounds__(KV8_THREADS, KV8_CTAS) attention_kv8_kernel(co
 // KV8_FOLD_THREADS * 4 / HD th of the parts, all loads under way together.
 #define KV8_FOLD_THREADS 128
 #define KV8_MAX_GRID 512
-template <int HD> __global__ void __launch_bounds__(KV8_FOLD_THREADS) attention_kv8_fold_kernel(AttnKv8 p, int grid) {
+template <int HD> __global__ void __launch_bounds__(KV8_FOLD_THREADS, 10) attention_kv8_fold_kernel(AttnKv8 p, int grid) {
     constexpr int COLS = HD / 4, GROUPS = KV8_FOLD_THREADS / COLS;
     __shared__ float weight[KV8_MAX_GRID], scratch[33];
     __shared__ float4 sums[GROUPS][COLS];
@@ -510,25 +510,32 @@ template <int HD> __global__ void __launch_bounds__(KV8_FOLD_THREADS) attention_
     const long long size = (long long)most_heads * (HD + 4);
     // of the first CTA it is the second part where the CTA's piece starts with another pair's pages
     auto part = [&](int c) { return p.parts + (2ll * (c0 + c) + (c == 0 && per * c0 < begin)) * size; };
-    float m = -INFINITY, u = -INFINITY, l = 0.0f;
-    for (int c = threadIdx.x; c < n; c += KV8_FOLD_THREADS) {
-        const float4 mlu = *(const float4 *)(part(c) + most_heads * HD + 4 * g);
+    // everything that most pairs need is asked for at once: a thread's first part's numbers and its first four parts' columns
+    const int col = threadIdx.x % COLS, of = threadIdx.x / COLS;
+    float4 x[4];
+    auto columns = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = c + i * GROUPS < n ? *(const float4 *)(part(c + i * GROUPS) + g * HD + 4 * col) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    };
+    auto numbers = [&](int c) { return c < n ? *(const float4 *)(part(c) + most_heads * HD + 4 * g) : make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f); };
+    const float4 mine_mlu = numbers(threadIdx.x);
+    columns(of);
+    float m = mine_mlu.x, u = mine_mlu.z, l = 0.0f;
+    for (int c = threadIdx.x + KV8_FOLD_THREADS; c < n; c += KV8_FOLD_THREADS) {
+        const float4 mlu = numbers(c);
         m = fmaxf(m, mlu.x), u = fmaxf(u, mlu.z);
     }
     m = block_max(m, scratch), u = block_max(u, scratch);
     for (int c = threadIdx.x; c < n; c += KV8_FOLD_THREADS) {
-        const float4 mlu = *(const float4 *)(part(c) + most_heads * HD + 4 * g);
+        const float4 mlu = c == threadIdx.x ? mine_mlu : numbers(c);
         l = fmaf(share(mlu.x, m), mlu.y, l), weight[c] = share(mlu.z, u);
     }
     l = block_sum(l, scratch);  // (a barrier: the weights are there)
-    const int col = threadIdx.x % COLS, of = threadIdx.x / COLS;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int c = of; c < n; c += 8 * GROUPS) {
-        float4 x[8];
+    for (int c = of; c < n; c += 4 * GROUPS) {
+        if (c != of) columns(c);
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = c + i * GROUPS < n ? *(const float4 *)(part(c + i * GROUPS) + g * HD + 4 * col) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
+        for (int i = 0; i < 4; i++) {
             const float w = c + i * GROUPS < n ? weight[c + i * GROUPS] : 0.0f;
             acc.x = fmaf(w, x[i].x, acc.x), acc.y = fmaf(w, x[i].y, acc.y), acc.z = fmaf(w, x[i].z, acc.z), acc.w = fmaf(w, x[i].w, acc.w);
         }
