@@ -324,94 +324,96 @@ __global__ void __launch_bounds__(KV8_THREADS, KV8_CTAS) attention_kv8_kernel(co
                     if (!sees8) sc[nt][2] = sc[nt][3] = -INFINITY;
                 }
             };
+            // The open block, as it came: once a pair, by one warp, ahead of the pages, which may still be on their way.
+            if (pos / KV8_BLOCK >= closed && pos / KV8_PAGE >= first && pos / KV8_PAGE < first + seg.pages && pos % KV8_PAGE / KV8_BLOCK == warp) {
+                const int key0 = pos / KV8_BLOCK * KV8_BLOCK;
+                float sc[NT][4] = {}, f[NT][2];
+                const __nv_bfloat16 *open_k = p.open + ((long long)slot * 2 * p.n_kv_heads + kvh) * (KV8_BLOCK * HD),
+                                    *open_v = open_k + (long long)p.n_kv_heads * (KV8_BLOCK * HD);
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+                    const uint2 k0 = *(const uint2 *)(open_k + i8 * HD + 16 * ks + c4), k8 = *(const uint2 *)(open_k + (i8 + 8) * HD + 16 * ks + c4);
+                    const uint32_t a[4] = {k0.x, k8.x, k0.y, k8.y};
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        const uint2 b = 8 * nt + i8 < heads ? *(const uint2 *)(q + (8 * nt + i8) * HD + 16 * ks) : make_uint2(0, 0);
+                        mma_bf16(sc[nt], a, b.x, b.y);
+                    }
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sc[nt][e] *= p.scale_log2;
+                mask(sc, key0);
+                softmax(sc, f, 1.0f);
+                uint32_t high[NT][2], low[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const float x = sc[nt][2 * i] * f[nt][0], y = sc[nt][2 * i + 1] * f[nt][1];
+                        const uint32_t h = pack_bf16(x, y);
+                        const float2 back = __bfloat1622float2(*(const __nv_bfloat162 *)&h);
+                        high[nt][i] = transposed(h), low[nt][i] = transposed(pack_bf16(x - back.x, y - back.y));
+                    }
+#pragma unroll
+                for (int c = 0; c < KS; c++) {
+                    uint32_t v[4];  // tokens 2 c', 2 c' + 1, 2 c' + 8, 2 c' + 9; a token behind the position may hold anything
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int t = 2 * (lane & 3) + (i & 1) + 8 * (i >> 1);
+                        v[i] = key0 + t <= pos ? *(const uint32_t *)(open_v + t * HD + 16 * c + 2 * i8) : 0u;
+                    }
+                    const uint32_t a[4] = {__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[0], v[1], 0x7632),
+                                           __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[2], v[3], 0x7632)};
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) mma_bf16(o[nt][c], a, high[nt][0], high[nt][1]), mma_bf16(o[nt][c], a, low[nt][0], low[nt][1]);
+                }
+            }
             for (int pg = first; pg < first + seg.pages; pg++) {
                 if (!tc::mbar_wait(&full[s], phase)) {
                     ok = false;
                     break;
                 }
                 const int key0 = pg * KV8_PAGE + KV8_BLOCK * warp;  // this warp's block of the page
-                if (key0 <= pos && key0 + KV8_BLOCK > lo) {
+                if (key0 / KV8_BLOCK < closed && key0 <= pos && key0 + KV8_BLOCK > lo) {
                     float sc[NT][4] = {}, f[NT][2];
-                    if (key0 / KV8_BLOCK < closed) {
-                        const uint32_t k_base = tc::smem_addr(k_s + s * TILE_BYTES), v_base = tc::smem_addr(v_s + s * TILE_BYTES);
-                        const float k_scale = scale_s[s * 2 * KV8_PAGE_BLOCKS + warp], v_scale = scale_s[(s * 2 + 1) * KV8_PAGE_BLOCKS + warp];
+                    const uint32_t k_base = tc::smem_addr(k_s + s * TILE_BYTES), v_base = tc::smem_addr(v_s + s * TILE_BYTES);
+                    const float k_scale = scale_s[s * 2 * KV8_PAGE_BLOCKS + warp], v_scale = scale_s[(s * 2 + 1) * KV8_PAGE_BLOCKS + warp];
 #pragma unroll
-                        for (int ks = 0; ks < KS; ks += 2) {
-                            uint32_t w[4];
-                            ldsm_x4(token_piece<HD>(k_base, KV8_BLOCK * warp + 8 * (j8 & 1) + r8, ks + (j8 >> 1)), w[0], w[1], w[2], w[3]);
+                    for (int ks = 0; ks < KS; ks += 2) {
+                        uint32_t w[4];
+                        ldsm_x4(token_piece<HD>(k_base, KV8_BLOCK * warp + 8 * (j8 & 1) + r8, ks + (j8 >> 1)), w[0], w[1], w[2], w[3]);
 #pragma unroll
-                            for (int i = 0; i < 2; i++) {
-                                uint32_t a[4];
-                                f16_of_word<FORM, false>(w[2 * i], a[0], a[2]), f16_of_word<FORM, false>(w[2 * i + 1], a[1], a[3]);
+                        for (int i = 0; i < 2; i++) {
+                            uint32_t a[4];
+                            f16_of_word<FORM, false>(w[2 * i], a[0], a[2]), f16_of_word<FORM, false>(w[2 * i + 1], a[1], a[3]);
 #pragma unroll
-                                for (int nt = 0; nt < NT; nt++) mma_f16(sc[nt], a, qf[nt][ks + i][0], qf[nt][ks + i][1]);
-                            }
+                            for (int nt = 0; nt < NT; nt++) mma_f16(sc[nt], a, qf[nt][ks + i][0], qf[nt][ks + i][1]);
                         }
+                    }
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
+                    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                            for (int e = 0; e < 4; e++) sc[nt][e] *= unit_of[nt][e & 1] * k_scale;
-                        if (key0 < lo || key0 + KV8_BLOCK - 1 > pos) mask(sc, key0);
-                        softmax(sc, f, v_scale);
-                        uint32_t pf[NT][2];
+                        for (int e = 0; e < 4; e++) sc[nt][e] *= unit_of[nt][e & 1] * k_scale;
+                    if (key0 < lo || key0 + KV8_BLOCK - 1 > pos) mask(sc, key0);
+                    softmax(sc, f, v_scale);
+                    uint32_t pf[NT][2];
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) {
-                            pf[nt][0] = transposed(pack_f16(sc[nt][0] * f[nt][0], sc[nt][1] * f[nt][1]));
-                            pf[nt][1] = transposed(pack_f16(sc[nt][2] * f[nt][0], sc[nt][3] * f[nt][1]));
-                        }
+                    for (int nt = 0; nt < NT; nt++) {
+                        pf[nt][0] = transposed(pack_f16(sc[nt][0] * f[nt][0], sc[nt][1] * f[nt][1]));
+                        pf[nt][1] = transposed(pack_f16(sc[nt][2] * f[nt][0], sc[nt][3] * f[nt][1]));
+                    }
 #pragma unroll
-                        for (int c = 0; c < KS; c += 2) {
-                            uint32_t w[4];
-                            ldsm_x4_t(token_piece<HD>(v_base, KV8_BLOCK * warp + 8 * (j8 & 1) + r8, c + (j8 >> 1)), w[0], w[1], w[2], w[3]);
+                    for (int c = 0; c < KS; c += 2) {
+                        uint32_t w[4];
+                        ldsm_x4_t(token_piece<HD>(v_base, KV8_BLOCK * warp + 8 * (j8 & 1) + r8, c + (j8 >> 1)), w[0], w[1], w[2], w[3]);
 #pragma unroll
-                            for (int i = 0; i < 2; i++) {
-                                uint32_t a[4];
-                                f16_of_word<FORM, true>(w[2 * i], a[0], a[1]), f16_of_word<FORM, true>(w[2 * i + 1], a[2], a[3]);
+                        for (int i = 0; i < 2; i++) {
+                            uint32_t a[4];
+                            f16_of_word<FORM, true>(w[2 * i], a[0], a[1]), f16_of_word<FORM, true>(w[2 * i + 1], a[2], a[3]);
 #pragma unroll
-                                for (int nt = 0; nt < NT; nt++) mma_f16(o[nt][c + i], a, pf[nt][0], pf[nt][1]);
-                            }
-                        }
-                    } else {  // the open block, as it came: once a pair, by one warp
-                        const __nv_bfloat16 *open_k = p.open + ((long long)slot * 2 * p.n_kv_heads + kvh) * (KV8_BLOCK * HD),
-                                            *open_v = open_k + (long long)p.n_kv_heads * (KV8_BLOCK * HD);
-#pragma unroll
-                        for (int ks = 0; ks < KS; ks++) {
-                            const uint2 k0 = *(const uint2 *)(open_k + i8 * HD + 16 * ks + c4), k8 = *(const uint2 *)(open_k + (i8 + 8) * HD + 16 * ks + c4);
-                            const uint32_t a[4] = {k0.x, k8.x, k0.y, k8.y};
-#pragma unroll
-                            for (int nt = 0; nt < NT; nt++) {
-                                const uint2 b = 8 * nt + i8 < heads ? *(const uint2 *)(q + (8 * nt + i8) * HD + 16 * ks) : make_uint2(0, 0);
-                                mma_bf16(sc[nt], a, b.x, b.y);
-                            }
-                        }
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) sc[nt][e] *= p.scale_log2;
-                        mask(sc, key0);
-                        softmax(sc, f, 1.0f);
-                        uint32_t high[NT][2], low[NT][2];
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                            for (int i = 0; i < 2; i++) {
-                                const float x = sc[nt][2 * i] * f[nt][0], y = sc[nt][2 * i + 1] * f[nt][1];
-                                const uint32_t h = pack_bf16(x, y);
-                                const float2 back = __bfloat1622float2(*(const __nv_bfloat162 *)&h);
-                                high[nt][i] = transposed(h), low[nt][i] = transposed(pack_bf16(x - back.x, y - back.y));
-                            }
-#pragma unroll
-                        for (int c = 0; c < KS; c++) {
-                            uint32_t v[4];  // tokens 2 c', 2 c' + 1, 2 c' + 8, 2 c' + 9; a token behind the position may hold anything
-#pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                const int t = 2 * (lane & 3) + (i & 1) + 8 * (i >> 1);
-                                v[i] = key0 + t <= pos ? *(const uint32_t *)(open_v + t * HD + 16 * c + 2 * i8) : 0u;
-                            }
-                            const uint32_t a[4] = {__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[0], v[1], 0x7632),
-                                                   __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[2], v[3], 0x7632)};
-#pragma unroll
-                            for (int nt = 0; nt < NT; nt++) mma_bf16(o[nt][c], a, high[nt][0], high[nt][1]), mma_bf16(o[nt][c], a, low[nt][0], low[nt][1]);
+                            for (int nt = 0; nt < NT; nt++) mma_f16(o[nt][c + i], a, pf[nt][0], pf[nt][1]);
                         }
                     }
                 }
