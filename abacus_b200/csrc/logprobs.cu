@@ -7,7 +7,7 @@
 // probability NaN.
 //
 // A row is read once, by a CTA or, where there are few rows, by a cluster of up to 16 CTAs, a slice each. Every thread keeps a
-// running maximum and the two sums over its elements, 16 at a time, the next 16 on their way; nothing in the walk waits for
+// running maximum and the two sums over its elements, four 16-byte pieces at a time, the next four on their way; nothing in the walk waits for
 // another warp. The most likely tokens: an element is noted, in the warp's own list in shared memory, only where it reaches a bound
 // that at least k elements of the slice reach: every warp leaves its ceil(k / 8)-th largest thread maximum in shared memory as it goes,
 // and of these the one that enough warps reach is the bound (one that is out of date is only lower). A list that fills up is cut to its best k; a
@@ -15,9 +15,9 @@
 // reach the last bound, some tens, are ranked by counting those before each, and once more those of a cluster's CTAs. Elements of -inf are
 // never noted: where a row has fewer than k others, the first of them fill its places.
 //
-// Measured: 512 rows of 151,936 float32 logits with 5 alternatives in 66 us, 4.7 TB/s (53 without); 8 rows with 20 in 12.7 (9.4 without), a
+// Measured: 512 rows of 151,936 float32 logits with 5 alternatives in 66 us, 4.7 TB/s (53 without); 8 rows with 20 in 12.5 to 13.9 (9.4 without), a
 // chain of three turns of loads, bounds, ranks and the cluster's fold; 200 rows of 50,261 bfloat16 logits, a twentieth not -inf, with 64
-// in 26 (10 without): there every turn of 512 elements has some to note.
+// in 24: there every turn of 1,024 elements has some to note.
 #define ABK_DEFINE_ERROR
 #include "common.cuh"
 #include "tc_common.cuh"
@@ -28,6 +28,10 @@
 #define LOGPROBS_THREADS (32 * LOGPROBS_WARPS)
 #define LOGPROBS_MAX_SPLITS 16
 static_assert(LOGPROBS_MAX_SPLITS >= 2 * LOGPROBS_WARPS, "room for all lists");
+// 16-byte pieces a thread takes at a time: 16 elements of float32, 32 of 16-bit types. With two of these for 16-bit types 200 rows of
+// 50,261 with 64 alternatives take 27.7 us, not 24.2; four spill some registers (64 bytes of stores), three (12 bytes)
+// take the same 24.2, and rows without many to note show no difference.
+#define LOGPROBS_PIECES 4
 #define LOGPROBS_NOTED 128  // elements a warp's list has room for beside those of one piece of every lane
 
 struct LogProbs {
@@ -144,7 +148,7 @@ __device__ __forceinline__ void make_room(Noted &noted, Ranked *list, Ranked *sp
 // to stay in registers for this: 512 rows of 151,936 with the 5 most likely take 71 us so, not 66).
 template <typename T> __device__ __forceinline__ Noted note_pieces(const uint4 *src, int j0, int pieces, int body, Noted noted, Ranked *list,
                                                                 Ranked *spare, int top, int lane) {
-    constexpr int N = Piece<T>::N, U = 16 / N;
+    constexpr int N = Piece<T>::N, U = LOGPROBS_PIECES;
     uint4 w[U];
 #pragma unroll
     for (int u = 0; u < U; u++) w[u] = j0 + 32 * u + lane < pieces ? __ldg(src + j0 + 32 * u + lane) : Piece<T>::nothing();
@@ -172,7 +176,7 @@ __device__ __forceinline__ void move_bound(Bounds *b, float of_lane, int top, in
 
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(LOGPROBS_THREADS, sizeof(T) == 4 ? 4 : 3) logprobs_kernel(LogProbs p) {
-    constexpr int N = Piece<T>::N, U = 16 / N, ROOM = LOGPROBS_NOTED + 32 * N;  // elements of a piece, pieces a thread takes at a time
+    constexpr int N = Piece<T>::N, U = LOGPROBS_PIECES, ROOM = LOGPROBS_NOTED + 32 * N;  // elements of a piece, pieces a thread takes at a time
     __shared__ Ranked lists[TOP ? LOGPROBS_WARPS : 1][TOP ? ROOM : 1], best[TOP ? LOGPROBS_MAX_TOP : 1];
     __shared__ Ranked cand[TOP ? LOGPROBS_MAX_SPLITS * LOGPROBS_MAX_TOP : 1];  // in turn: room to sort a list, all lists, the cluster's
     __shared__ Bounds bounds;
@@ -230,13 +234,13 @@ __global__ void __launch_bounds__(LOGPROBS_THREADS, sizeof(T) == 4 ? 4 : 3) logp
     load(warp * U * 32, w);
     bool first = true;
     for (int j0 = warp * U * 32; first || j0 < pieces; j0 += LOGPROBS_THREADS * U) {
-        __align__(8) float v[16];
+        __align__(8) float v[U * N];
 #pragma unroll
         for (int u = 0; u < U; u++) Piece<T>::floats(w[u], v + u * N);
         load(j0 + LOGPROBS_THREADS * U, w);
         float most = v[0];
 #pragma unroll
-        for (int e = 1; e < 16; e++) most = fmaxf(most, v[e]);
+        for (int e = 1; e < U * N; e++) most = fmaxf(most, v[e]);
         if (TOP) {
             if (first) {  // the first bounds
                 leave_bound(&bounds, most, in_warp, warp, lane);
@@ -248,7 +252,7 @@ __global__ void __launch_bounds__(LOGPROBS_THREADS, sizeof(T) == 4 ? 4 : 3) logp
         }
         if (first && warp == 0) loose(lo, body);
         const bool risen = most > m;
-        sum((const float2 *)v, 8, most);
+        sum((const float2 *)v, U * N / 2, most);
         if (TOP && __any_sync(0xffffffffu, most >= noted.cut)) {
             const bool moves = __any_sync(0xffffffffu, most >= noted.cut && risen);  // (else no thread's maximum that counts does)
             noted = note_pieces<T>(src, j0, pieces, body, noted, list, spare, p.top, lane);
