@@ -40,11 +40,11 @@
 #define KV8_MAX_STAGES 16
 #define KV8_THREADS 160
 #define KV8_ROWS 512  // rows of a launch
-// CTAs an SM holds. Three with heads of 64 and up to 8 of them (int8, 32 query and 8 kv heads: 32 rows over 128 to
-// 4,096 tokens 22.4 us, not 25.6; 8 rows over 32,768 55.9, not 69.1; e4m3, 8 rows over 8,448 20.1, not 22.3; one row over 2,176 0.4
-// longer), though 32 to 40 bytes a thread spill. Two with heads of 128, where three take longer (two documents of 131,071 and 100,000
-// tokens 95 us, not 89), and with more than 8 heads of 64, where three were not tried: two tiles hold more registers.
-#define KV8_CTAS(dim, tiles) ((dim) == 64 && (tiles) == 1 ? 3 : 2)
+// CTAs an SM holds. Three with heads of 64 (int8, 8 kv heads, 32 rows over 128 to 4,096 tokens: 4 heads to each 22.4 us, not 25.6, 16 to
+// each 37.7, not 38.2; 8 rows over 32,768: 55.9, not 69.1, and 83.6, not 89.4; e4m3, 8 rows over 8,448: 20.1, not 22.3, and 29.3, not
+// 30.0; one row over 2,176 0.2 to 0.4 longer), though 16 to 40 bytes a thread spill. Two with heads of 128, where three take longer (two
+// documents of 131,071 and 100,000 tokens 95 us, not 89).
+#define KV8_CTAS(dim) ((dim) == 64 ? 3 : 2)
 #define KV8_START 4   // pages that starting a pair costs as much as
 
 struct AttnKv8 {
@@ -134,7 +134,7 @@ struct Kv8Segment {
 };
 
 template <int HD, int FORM, int NT>
-__global__ void __launch_bounds__(KV8_THREADS, KV8_CTAS(HD, NT)) attention_kv8_kernel(const __grid_constant__ CUtensorMap k_map,
+__global__ void __launch_bounds__(KV8_THREADS, KV8_CTAS(HD)) attention_kv8_kernel(const __grid_constant__ CUtensorMap k_map,
                                                                               const __grid_constant__ CUtensorMap v_map, AttnKv8 p) {
     constexpr int TILE_BYTES = KV8_PAGE * HD, KS = HD / 16;
     extern __shared__ uint8_t kv8_raw[];
@@ -557,7 +557,7 @@ template <int HD> __global__ void __launch_bounds__(KV8_FOLD_THREADS, 10) attent
 // Floats of memory for the parts of pairs that several CTAs share.
 extern "C" long long abk_attention_kv8_part_floats(int n_heads, int n_kv_heads, int head_dim) {
     const int group = n_kv_heads > 0 ? n_heads / n_kv_heads : 1;
-    return 2ll * KV8_CTAS(head_dim, group <= 8 ? 1 : 2) * abk_sm_count() * (group < KV8_HEADS ? group : KV8_HEADS) * (head_dim + 4);
+    return 2ll * KV8_CTAS(head_dim) * abk_sm_count() * (group < KV8_HEADS ? group : KV8_HEADS) * (head_dim + 4);
 }
 extern "C" int abk_attention_kv8(const void *q, long long q_row, void *out, int n_rows, int n_heads, float scale, int window,
                                  const int *token_seq, const int *token_pos, const int *seq_slot, const int *seq_pos0,
@@ -571,7 +571,7 @@ extern "C" int abk_attention_kv8(const void *q, long long q_row, void *out, int 
     const int group = n_heads / n_kv_heads, runs = (group + KV8_HEADS - 1) / KV8_HEADS, heads = group < KV8_HEADS ? group : KV8_HEADS;
     if ((((uintptr_t)q | (uintptr_t)out) & 7) || (q_row & 3) || (((uintptr_t)c.scales | (uintptr_t)c.open | (uintptr_t)parts) & 15))
         ABK_REFUSE("attention_kv8: q and out must be 8-byte aligned, scales, open blocks and parts 16-byte aligned");
-    const int ctas = KV8_CTAS(head_dim, heads <= 8 ? 1 : 2), grid = ctas * abk_sm_count();
+    const int ctas = KV8_CTAS(head_dim), grid = ctas * abk_sm_count();
     if (grid > KV8_MAX_GRID) ABK_REFUSE("attention_kv8: %d CTAs are more than the fold has room for", grid);
     if (part_floats < abk_attention_kv8_part_floats(n_heads, n_kv_heads, head_dim))
         ABK_REFUSE("attention_kv8: room for %lld floats of parts is too little", part_floats);
