@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(32 * KV8_WARPS) kv8_write_kernel(Kv8Write p) {
                 const int t = (32 * i + lane) / LPR, c = (32 * i + lane) % LPR, pos = pos0 + t;
                 if (pos >= start && pos < after) *(uint4 *)(open + t * HD + 8 * c) = x[i];
             }
-        } else if (cache_keeps(p.cache, pos0, after)) {
+        } else if (cache_keeps(p.cache, pos0 + KV8_BLOCK - 1, after)) {  // (a place goes to the later block with its last token)
             close_block<HD, FORM>(p, x, slot, head, j, pos0, lane);
         }
         if (!both || b != b0) return;
