@@ -99,8 +99,10 @@ class Engine:
         # the step function in C where the model is made of the library's own parts, else the parts' forward()
         self.cstep = CStep(model, self.cache) if cache is None and CStep.serves(model) else None
         decode_graphs, prompt_graphs = capturable(model)
-        if cache is not None and prompt_graphs:  # a sequence that goes on has its pages counted on the host
-            prompt_graphs = "from_start"
+        if cache is not None and prompt_graphs:
+            # a step that reads an 8-bit cache back has its pages counted on the host: one with a sequence that goes on, and any
+            # prompt step of a layer whose keys are another's
+            prompt_graphs = "from_start" if all(e.source is None for e in model.schedule) else False
         self.graphs = DecodeGraphs(self) if use_graphs and decode_graphs else None
         prompts = use_graphs and prompt_graphs and os.environ.get("ABACUS_PROMPT_GRAPHS", "1") != "0"
         self.prompt_graphs = PromptGraphs(self, from_start_only=prompt_graphs == "from_start") if prompts else None

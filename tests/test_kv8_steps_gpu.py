@@ -1,6 +1,11 @@
 """The 8-bit cache at the steps between whole prompts and single tokens: several new tokens a sequence under windows and rings of pages."""
-import pytest
+import dataclasses
 
+import numpy as np
+import pytest
+import torch
+
+from helpers import make_model_folder
 from test_kv8_gpu import Run, ops  # noqa: F401  (ops is a fixture)
 
 pytestmark = pytest.mark.gpu
@@ -25,3 +30,36 @@ def test_several_tokens_under_a_window(ops, window, form, dim, ring):  # noqa: F
         qkv = run.rows(most + 1).cuda()
         with pytest.raises(ops.KernelRefused, match="ring"):
             ops.attention_kv8(qkv, qkv.new_zeros((most + 1, 6 * dim)), 6, 2, dim, 0.125, window, batch, run.kv, run.ws)
+
+
+def model_of(folder, schedule=None):
+    """The bfloat16 model of a folder, with its layers in another order."""
+    from abacus_b200.config import load_config
+    from abacus_b200.models import Model
+    from abacus_b200.weights import load_folder
+    arch, cfg = load_config(folder)
+    spec = cfg.to_spec() if schedule is None else dataclasses.replace(cfg.to_spec(), schedule=schedule)
+    tensors = load_folder(folder, lambda names: arch.tensor_names(spec, names))
+    return Model(spec, arch.layout(spec), tensors, torch.bfloat16, torch.device("cuda", 0))
+
+
+def test_prompts_of_a_layer_that_reads_anothers_cache_again_and_again(tmp_path):
+    """Prompt steps of one shape, the lengths and slots others each time: an engine that captures steps gives what one without graphs
+    gives (the pages that the second layer reads back are this step's, not an earlier one's)."""
+    from abacus_b200.config import ScheduleEntry
+    from abacus_b200.engine import Engine
+    model = model_of(make_model_folder(tmp_path, "D"), (ScheduleEntry(0), ScheduleEntry(1, source=0), ScheduleEntry(1)))
+    engines = [Engine(model, max_tokens=64 * 20, use_graphs=graphs, cache="int8") for graphs in (True, False)]
+    rng = np.random.default_rng(3)
+    for lengths in ((100, 150), (140, 110), (90, 160), (155, 95), (150, 100)):
+        prompts = [rng.integers(0, 515, n).tolist() for n in lengths]
+        got = []
+        for e in engines:
+            slots = [e.open() for _ in prompts]
+            logits = e.step([(s, p, [len(p) - 1]) for s, p in zip(slots, prompts)]).clone()
+            logits = torch.cat([logits, e.step([(s, [7], [0]) for s in slots])])
+            for s in slots[::-1]:
+                e.close(s)
+            e.check_status()
+            got.append(logits)
+        assert torch.equal(*got), lengths
