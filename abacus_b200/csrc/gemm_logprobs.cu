@@ -11,7 +11,7 @@
 // accumulator of its own, and the reading threads add them up, in registers, while the tensor cores are on the next one.
 // A second kernel joins the pairs' sums, a warp a row. Measured: 2,048 rows of 1,024 against 151,936 in 515 us, 1,240 TFLOP/s (cuBLAS
 // sustains 1,377 under the power cap); 4,999 rows of 4,096 in 5,300, three segments, 1,174 TFLOP/s (5,280 in two,
-// 4,850 to 5,000 in one). The eight warps that read need 5.5 instructions and one exponential a logit:
+// 4,850 to 5,000 in one). The eight warps that read need 6.5 instructions and one exponential a logit:
 // at K = 1,024 half of the time that the tensor cores take for it.
 //
 // Few rows (up to LP_FEW, few_wins): w is all there is to read, and a tile of 256 rows of x of which a few are there costs the tensor cores as much
@@ -205,22 +205,35 @@ __global__ void __launch_bounds__(LP_THREADS) gemm_logprobs_kernel(const __grid_
 #pragma unroll
                             for (int j = 0; j < 32; j++) v[j] += sum[c0 + j];
                         }
-                        if (col0 + c0 + 32 > g.vocab) {  // the last tile: columns behind the vocabulary weigh nothing
+                        const bool edge = col0 + c0 + 32 > g.vocab;
+                        if (edge) {  // columns behind the vocabulary, until they are left out below: the first one again
 #pragma unroll
-                            for (int j = 0; j < 32; j++)
-                                if (col0 + c0 + j >= g.vocab) v[j] = LOGPROBS_FAR;
+                            for (int j = 1; j < 32; j++)
+                                if (col0 + c0 + j >= g.vocab) v[j] = v[0];
                         }
                         if (here) {
 #pragma unroll
                             for (int j = 0; j < 32; j++)
                                 if (wanted == c0 + j && col0 + c0 + j < g.vocab) g.given[p] = v[j];
                         }
-                        float most = v[0];
+                        float most = v[0], least = v[0];
 #pragma unroll
-                        for (int j = 1; j < 32; j++) most = fmaxf(most, v[j]);
+                        for (int j = 1; j < 32; j++) most = fmaxf(most, v[j]), least = fminf(least, v[j]);
                         if (most > m) {
                             const float d = fmaxf(m - most, LOGPROBS_FAR), e = ex2(d * 1.4426950408889634f);
                             tt = mul2(make_float2(e, e), fma2(l, make_float2(d, d), tt)), l = mul2(make_float2(e, e), l), m = most;
+                        }
+                        // The end of the vocabulary, or a distance that float32 does not hold (0 times it would be NaN): one by one,
+                        // with the same roundings (the warp's other rows come this way too).
+                        if (__any_sync(0xffffffffu, edge || least - m < LOGPROBS_FAR)) {
+#pragma unroll
+                            for (int j = 0; j < 32; j++) {
+                                const float d = v[j] - m, e = ex2(d * 1.4426950408889634f);
+                                if (col0 + c0 + j >= g.vocab) continue;
+                                float &l1 = j & 1 ? l.y : l.x, &t1 = j & 1 ? tt.y : tt.x;
+                                l1 += v[j] == -INFINITY ? __int_as_float(0x7fffffff) : e, t1 = fmaf(e, fmaxf(d, LOGPROBS_FAR), t1);
+                            }
+                            return;
                         }
                         const float2 down = make_float2(-m, -m), unit = make_float2(1.4426950408889634f, 1.4426950408889634f);
 #pragma unroll
@@ -389,10 +402,10 @@ __global__ void __launch_bounds__(LP_THREADS) gemm_logprobs_few_kernel(const __g
 #pragma unroll
                 for (int j = 0; j < COLS; j++) {
                     if (col0 + j >= g.rows) continue;
-                    const float v = sum[j], n = fmaxf(m[j], v), dm = m[j] - n, dv = v - n;
+                    const float v = sum[j], n = fmaxf(m[j], v), dm = fmaxf(m[j] - n, LOGPROBS_FAR), dv = v - n;
                     const float a = ex2(dm * 1.4426950408889634f), e = ex2(dv * 1.4426950408889634f);
-                    tt[j] = fmaf(a, fmaf(l[j], dm, tt[j]), e * dv);
-                    l[j] = fmaf(l[j], a, e), m[j] = n;
+                    tt[j] = fmaf(a, fmaf(l[j], dm, tt[j]), e * fmaxf(dv, LOGPROBS_FAR));
+                    l[j] = v == -INFINITY ? __int_as_float(0x7fffffff) : fmaf(l[j], a, e), m[j] = n;
                     if (token_s[col0 + j] == token) g.given[col0 + j] = v;
                 }
             }
