@@ -128,6 +128,14 @@ __device__ __forceinline__ float heads_sum(float v) {
 // What a part with exponent `from` is multiplied by where the common exponent is `to` (a part without keys: nothing).
 __device__ __forceinline__ float share(float from, float to) { return from == -INFINITY ? 0.0f : exp2f(from - to); }
 
+// A barrier over the four warps that compute, which tells all of them whether any brings true.
+__device__ __forceinline__ bool any_of_the_four_warps(bool x) {
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(any) : "r"((uint32_t)x) : "memory");
+    return any;
+}
+
 // A run of pages of one pair, in one CTA.
 struct Kv8Segment {
     int row, pair, page, pages, units;  // row of the launch; the run's first page among the row's, how many (maybe none), its units
@@ -374,10 +382,8 @@ __global__ void __launch_bounds__(KV8_THREADS, KV8_CTAS(HD)) attention_kv8_kerne
                 }
             }
             for (int pg = first; pg < first + seg.pages; pg++) {
-                if (!tc::mbar_wait(&full[s], phase)) {
-                    ok = false;
-                    break;
-                }
+                ok = __all_sync(0xffffffffu, tc::mbar_wait(&full[s], phase));
+                if (!ok) break;
                 const int key0 = pg * KV8_PAGE + KV8_BLOCK * warp;  // this warp's block of the page
                 if (key0 / KV8_BLOCK < closed && key0 <= pos && key0 + KV8_BLOCK > lo) {
                     float sc[NT][4] = {}, f[NT][2];
@@ -440,7 +446,7 @@ __global__ void __launch_bounds__(KV8_THREADS, KV8_CTAS(HD)) attention_kv8_kerne
                     }
                 }
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
+            ok = !any_of_the_four_warps(!ok);  // all stop behind this run or none: every barrier is passed by all of them
             const bool whole = seg.pages == first_unit[seg.row + 1] - first_unit[seg.row] - KV8_START;
             float *part = p.parts + (2 * (long long)blockIdx.x + (done > 0)) * most_heads * (HD + 4);
             done++;
