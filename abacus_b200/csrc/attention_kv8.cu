@@ -156,25 +156,27 @@ __global__ void __launch_bounds__(KV8_THREADS, KV8_CTAS(HD)) attention_kv8_kerne
     __shared__ int first_unit[KV8_ROWS + 1];  // of a pair of the rows before a row
     __shared__ int4 row_info[KV8_ROWS];       // position, slot, blocks in 8 bits, first visible key
     __shared__ int fresh_page[KV8_ROWS];      // the first page that the step itself writes to
-    __shared__ int failed;
+    __shared__ int failed, bad_s;  // a wait ran out; pages and slots that are not there (said to the host at the end: not before pdl_wait())
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        failed = 0;
+        failed = 0, bad_s = 0;
         for (int s = 0; s < stages; s++) tc::mbar_init(&full[s], 1), tc::mbar_init(&empty[s], 4);
         tc::mbar_init_fence();
         tc::tma_prefetch_map(&k_map), tc::tma_prefetch_map(&v_map);
     }
     // Before pdl_wait() only what kernels further back than the one just before this wrote is read: the step's index arrays and
     // the page table, and (by the copy warp) the pages that the step's own tokens, which that kernel may still be writing, are not in.
+    int bad = 0;
     for (int r = threadIdx.x; r < p.n_rows; r += KV8_THREADS) {
         const int seq = p.token_seq[p.first_row + r], pos = p.token_pos[p.first_row + r];
         const int lo = p.window > 0 && pos - p.window + 1 > 0 ? pos - p.window + 1 : 0;
         first_unit[r + 1] = seq < 0 ? 0 : units_of(pos, lo);
         fresh_page[r] = seq < 0 ? 0 : p.seq_pos0[seq] / KV8_PAGE;
-        row_info[r] = seq < 0 ? make_int4(0, 0, 0, 0) : make_int4(pos, kv8_slot(p.seq_slot[seq], p.n_slots, p.status), p.seq_len_after[seq] / KV8_BLOCK, lo);
+        row_info[r] = seq < 0 ? make_int4(0, 0, 0, 0) : make_int4(pos, kv8_slot(p.seq_slot[seq], p.n_slots, bad), p.seq_len_after[seq] / KV8_BLOCK, lo);
     }
     __syncthreads();
+    if (bad) atomicOr(&bad_s, bad), bad = 0;
     if (warp == 0) {
         int before = 0;
         if (lane == 0) first_unit[0] = 0;
@@ -221,7 +223,7 @@ __global__ void __launch_bounds__(KV8_THREADS, KV8_CTAS(HD)) attention_kv8_kerne
             const int kvh = seg.pair / p.runs, first = info.w / KV8_PAGE + seg.page;
             for (int base = 0; base < seg.pages && go; base += 32) {
                 int page_lane = 0;  // every lane looks up one of the next 32 pages
-                if (base + lane < seg.pages) page_lane = kv8_page(p.cache, p.n_pages, info.y, (first + base + lane) * KV8_PAGE, p.status);
+                if (base + lane < seg.pages) page_lane = kv8_page(p.cache, p.n_pages, info.y, (first + base + lane) * KV8_PAGE, bad);
                 const int n = min(32, seg.pages - base);
                 for (int i = 0; i < n && go; i++, issued++) {
                     const long long tile = (long long)__shfl_sync(0xffffffffu, page_lane, i) * p.n_kv_heads + kvh;
@@ -243,6 +245,7 @@ __global__ void __launch_bounds__(KV8_THREADS, KV8_CTAS(HD)) attention_kv8_kerne
             }
             unit += seg.units;
         }
+        if (bad) atomicOr(&bad_s, bad);
         pdl_wait();
         if (!go && lane == 0) {  // let the copies in flight land before the CTA's memory goes away
             failed = 1;
@@ -476,7 +479,7 @@ __global__ void __launch_bounds__(KV8_THREADS, KV8_CTAS(HD)) attention_kv8_kerne
         if (!ok) failed = 1;
     }
     __syncthreads();
-    if (failed && threadIdx.x == 0) atomicOr(p.status + 2, 1);
+    if ((failed | bad_s) && threadIdx.x == 0) atomicOr(p.status + 2, (failed ? 1 : 0) | bad_s);
 }
 
 // The pairs that several CTAs have parts of, folded in the order of the keys, a CTA a head; zeros for rows that are padding. `grid`:

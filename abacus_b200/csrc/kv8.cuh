@@ -77,22 +77,34 @@ template <int FORM> __device__ __forceinline__ void kv8_unpack(uint32_t w, float
     }
 }
 
-// The page of a position, 0 where the table names one that is not among the pool's n_pages (and a status bit says so: nothing
-// outside the pool is touched).
+// The page of a position, 0 where the table names one that is not among the pool's n_pages (and a bit of `bad`, or of the status, says
+// so: nothing outside the pool is touched).
 #define KV8_BAD_PAGE 2
 #define KV8_BAD_SLOT 4
-__device__ __forceinline__ int kv8_page(const PagedCache &c, int n_pages, int slot, int pos, int *status) {
+__device__ __forceinline__ int kv8_page(const PagedCache &c, int n_pages, int slot, int pos, int &bad) {
     const int page = cache_page(c, slot, pos);
     if ((unsigned)page < (unsigned)n_pages) return page;
-    atomicOr(status + 2, KV8_BAD_PAGE);
+    bad |= KV8_BAD_PAGE;
     return 0;
 }
+__device__ __forceinline__ int kv8_page(const PagedCache &c, int n_pages, int slot, int pos, int *status) {
+    int bad = 0;
+    const int page = kv8_page(c, n_pages, slot, pos, bad);
+    if (bad) atomicOr(status + 2, bad);
+    return page;
+}
 
-// The slot, 0 where it is not one of the cache's n_slots (a status bit says so).
-__device__ __forceinline__ int kv8_slot(int slot, int n_slots, int *status) {
+// The slot, 0 where it is not one of the cache's n_slots (a bit says so).
+__device__ __forceinline__ int kv8_slot(int slot, int n_slots, int &bad) {
     if ((unsigned)slot < (unsigned)n_slots) return slot;
-    atomicOr(status + 2, KV8_BAD_SLOT);
+    bad |= KV8_BAD_SLOT;
     return 0;
+}
+__device__ __forceinline__ int kv8_slot(int slot, int n_slots, int *status) {
+    int bad = 0;
+    slot = kv8_slot(slot, n_slots, bad);
+    if (bad) atomicOr(status + 2, bad);
+    return slot;
 }
 
 // The largest i in [0, n) with below(values[i], i), -1 if there is none; below is true up to some place and false from there on.

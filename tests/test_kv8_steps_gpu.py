@@ -63,3 +63,30 @@ def test_prompts_of_a_layer_that_reads_anothers_cache_again_and_again(tmp_path):
             e.check_status()
             got.append(logits)
         assert torch.equal(*got), lengths
+
+
+def test_what_is_not_there_is_reported_after_the_launch_before(ops):  # noqa: F811
+    """The status bits of a bad page or slot come when the launch before has ended, so one that sets the status to zero does not take
+    them away; rows of a good slot are as they were."""
+    from abacus_b200.engine.batch import Sequence, StepBatch
+    run = Run(2, 1, 64, "int8", slots=3, pages=6)
+    a, b = run.open(), run.open()
+    run.write(ops, [(a, 70), (b, 30)], run.rows(100))
+    qkv = run.rows(2).cuda()
+    status = ops.kernel_status(qkv.device)
+    out, good = torch.zeros((2, 128), dtype=torch.bfloat16, device="cuda"), torch.zeros((2, 128), dtype=torch.bfloat16, device="cuda")
+    batch = StepBatch(2, 2, 1, "cuda").fill([Sequence(b, [0], 29, []), Sequence(a, [0], 69, [])], exact=True)
+    ops.attention_kv8(qkv, good, 2, 1, 64, 0.125, None, batch, run.kv, run.ws)
+    lost = torch.zeros(1 << 22, dtype=torch.int32, device="cuda")
+    for slot, bad_page, bit in ((7, False, 4), (-1, False, 4), (a, True, 2)):
+        batch = StepBatch(2, 2, 1, "cuda").fill([Sequence(b, [0], 29, []), Sequence(slot, [0], 69, [])], exact=True)
+        table = run.kv.page_table.clone()
+        if bad_page:
+            run.kv.page_table[a, 0] = 1000
+        for _ in range(20):
+            lost.zero_()  # (a launch of a while)
+            status.zero_()
+            ops.attention_kv8(qkv, out, 2, 1, 64, 0.125, None, batch, run.kv, run.ws)
+            assert status.tolist()[2] == bit and torch.equal(out[0], good[0])
+        run.kv.page_table.copy_(table)
+    status.zero_()
