@@ -372,11 +372,11 @@ __global__ void __launch_bounds__(KV8_THREADS, KV8_CTAS(HD)) attention_kv8_kerne
                     }
 #pragma unroll
                 for (int c = 0; c < KS; c++) {
-                    uint32_t v[4];  // tokens 2 c', 2 c' + 1, 2 c' + 8, 2 c' + 9; a token behind the position may hold anything
+                    uint32_t v[4];  // tokens 2 c', 2 c' + 1, 2 c' + 8, 2 c' + 9; one that the row does not see may hold anything
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int t = 2 * (lane & 3) + (i & 1) + 8 * (i >> 1);
-                        v[i] = key0 + t <= pos ? *(const uint32_t *)(open_v + t * HD + 16 * c + 2 * i8) : 0u;
+                        v[i] = key0 + t <= pos && key0 + t >= lo ? *(const uint32_t *)(open_v + t * HD + 16 * c + 2 * i8) : 0u;
                     }
                     const uint32_t a[4] = {__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[0], v[1], 0x7632),
                                            __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[2], v[3], 0x7632)};

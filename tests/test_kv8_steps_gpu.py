@@ -90,3 +90,21 @@ def test_what_is_not_there_is_reported_after_the_launch_before(ops):  # noqa: F8
             assert status.tolist()[2] == bit and torch.equal(out[0], good[0])
         run.kv.page_table.copy_(table)
     status.zero_()
+
+
+@pytest.mark.parametrize("ring", [True, False])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_open_tokens_before_the_window_may_hold_anything(ops, ring, bad):  # noqa: F811
+    """Keys and values that are not finite, in a sequence's open block but before a row's window: nothing of them reaches the row."""
+    run = Run(4, 2, 64, "int8", slots=2, pages=6, window=5 if ring else None, max_context=200)
+    run.window = 5
+    a, b = run.open(), run.open()
+    spoilt = run.rows(23)
+    spoilt[:4, 4 * 64:], spoilt[22, 4 * 64:] = bad, bad  # tokens 0 to 3 of a, token 18 of b
+    run.write(ops, [(a, 4), (b, 19)], spoilt)
+    run.write(ops, [(a, 4), (b, 4)], run.rows(8))
+    for slot in (a, b):  # (the formula takes them as zeros, which no row sees either)
+        run.brought[slot] = [torch.nan_to_num(x, 0.0, 0.0, 0.0) for x in run.brought[slot]]
+    for _ in range(3):
+        qkv = run.rows(2)
+        run.attend(ops, run.write(ops, [(a, 1), (b, 1)], qkv), qkv)
