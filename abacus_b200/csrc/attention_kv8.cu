@@ -59,6 +59,7 @@ struct AttnKv8 {
     const float *scales;
     const __nv_bfloat16 *open;
     int n_pages, n_slots, *status, stages;
+    int early;               // this step's kv8_write has been launched: what came before it is there
     int n_rows, pairs;       // rows of the launch; pairs of a row: n_kv_heads * runs
     int first_row;           // of the step, of this launch
     float *parts;            // [2 * grid][heads of a pair][HD + 4]
@@ -165,8 +166,13 @@ __global__ void __launch_bounds__(KV8_THREADS, KV8_CTAS(HD)) attention_kv8_kerne
         tc::mbar_init_fence();
         tc::tma_prefetch_map(&k_map), tc::tma_prefetch_map(&v_map);
     }
-    // Before pdl_wait() only what kernels further back than the one just before this wrote is read: the step's index arrays and
-    // the page table, and (by the copy warp) the pages that the step's own tokens, which that kernel may still be writing, are not in.
+    // Where kv8_write of this very step has been launched, the launch just before this one is that or a later one: what came before kv8_write
+    // is there, and is read before pdl_wait(): the step's index arrays and the page table, and (by the copy warp) the pages before
+    // those that the step's own tokens are in. Under a ring such a page may be one that kv8_write is putting blocks into at that moment; it
+    // puts one only where no row sees any token of the block that was there (the step's rows and the window fit the ring, as
+    // the launcher's caller checks), so what is torn belongs to blocks that are behind no row's first key and are never looked at. Otherwise
+    // all of it waits for the launch before, whatever that is.
+    if (!p.early) pdl_wait();
     int bad = 0;
     for (int r = threadIdx.x; r < p.n_rows; r += KV8_THREADS) {
         const int seq = p.token_seq[p.first_row + r], pos = p.token_pos[p.first_row + r];
@@ -216,7 +222,7 @@ __global__ void __launch_bounds__(KV8_THREADS, KV8_CTAS(HD)) attention_kv8_kerne
 
     if (warp == 4) {
         int issued = 0;
-        bool go = true, waited = false;
+        bool go = true, waited = !p.early;
         for (long long unit = begin; unit < end && go;) {
             const Kv8Segment seg = segment_at(unit);
             const int4 info = row_info[seg.row];
@@ -570,7 +576,8 @@ extern "C" long long abk_attention_kv8_part_floats(int n_heads, int n_kv_heads, 
 }
 extern "C" int abk_attention_kv8(const void *q, long long q_row, void *out, int n_rows, int n_heads, float scale, int window,
                                  const int *token_seq, const int *token_pos, const int *seq_slot, const int *seq_pos0,
-                                 const int *seq_len_after, const Kv8Cache *cache, float *parts, long long part_floats, void *stream) {
+                                 const int *seq_len_after, const Kv8Cache *cache, float *parts, long long part_floats, int early,
+                                 void *stream) {
     const Kv8Cache &c = *cache;
     const int head_dim = c.head_dim, n_kv_heads = c.n_kv_heads, form = c.form;
     if (n_rows <= 0) return 0;
@@ -594,7 +601,7 @@ extern "C" int abk_attention_kv8(const void *q, long long q_row, void *out, int 
     p.scale_log2 = scale * 1.4426950408889634f, p.window = window, p.token_seq = token_seq, p.token_pos = token_pos;
     p.seq_slot = seq_slot, p.seq_pos0 = seq_pos0, p.seq_len_after = seq_len_after, p.cache.page_table = c.page_table, p.cache.table_width = c.table_width;
     p.cache.ring_pages = c.ring_pages, p.cache.tokens_per_page = KV8_PAGE, p.scales = c.scales, p.open = (const __nv_bfloat16 *)c.open;
-    p.n_pages = c.n_pages, p.n_slots = c.n_slots, p.status = c.status, p.runs = runs, p.pairs = n_kv_heads * runs, p.parts = parts;
+    p.n_pages = c.n_pages, p.n_slots = c.n_slots, p.status = c.status, p.runs = runs, p.pairs = n_kv_heads * runs, p.parts = parts, p.early = early;
     void (*kernel)(CUtensorMap, CUtensorMap, AttnKv8) = nullptr;
     auto of_dim = [&](auto hd, auto tiles) {
         constexpr int HD = decltype(hd)::value, NT = decltype(tiles)::value;

@@ -95,6 +95,7 @@ class StepBatch:
         self.is_decode = False
         self.any_continuation = False
         self.scoring = None  # a step that scores: where its numbers go (engine.engine.Scoring)
+        self.kv8_written = None  # the 8-bit cache that this step's keys and values went to last (ops.kv8_write)
         self._sent, self._sent_on = None, set()
 
     def fill(self, sequences, pad_logits=False, exact=False):
@@ -167,6 +168,7 @@ class StepBatch:
         self.max_position = int(lens_after.max()) - 1 if n_seqs else 0
         self.max_len_after = self.max_position + 1
         self.any_continuation = n_seqs > 0 and max(starts) > 0
+        self.kv8_written = None
         self._send()
         return self
 
@@ -193,6 +195,7 @@ class StepBatch:
         left as they are on the device. The host's view follows."""
         from ..kernels import ops
         ops.advance_decode(self)
+        self.kv8_written = None
         for s in self.sequences:
             s.start += 1
         self.max_position += 1

@@ -625,6 +625,7 @@ def kv8_write(qkv, n_heads, n_kv_heads, head_dim, batch, cache, row=None, prepar
     assert qkv.dtype == torch.bfloat16 and qkv.is_contiguous() and width == row >= heads_size and n >= batch.n_rows
     record = _kv8_record("kv8_write", batch, cache, n_kv_heads, head_dim)
     _here("kv8_write", cache.k)
+    batch.kv8_written = cache  # (until the batch is filled anew or moves on)
     if prepare is not None:
         cos = prepare["cos"]
         if not batch.is_decode:
@@ -666,7 +667,9 @@ def attention_kv8(qkv, out, n_heads, n_kv_heads, head_dim, scale, window, batch,
     """Causal grouped-query attention of the step's rows (src/model.c:197-211) over an 8-bit cache that holds the step's own keys
     and values too (kv8_write comes first): each row sees the keys up to its position, within `window` of it if given. Any
     number of new tokens a sequence; meant for one or a few (each row reads its keys itself). q is read from qkv's q columns.
-    ws: a Workspace for the parts of rows that several CTAs share. A block with a value that is not finite is NaN in all that see it."""
+    ws: a Workspace for the parts of rows that several CTAs share. A block with a value that is not finite is NaN in all that see it.
+    Behind kv8_write of this very step (the same filled batch, the same cache) the kernel reads the step's index arrays, the page table and earlier
+    tokens' pages while kv8_write still runs; nothing launched since then may write those. Otherwise it waits for the launch before."""
     _here("attention_kv8", qkv, out, batch.token_seq)
     lib = load_module("attention_kv8")
     n, row = batch.n_rows, (n_heads + 2 * n_kv_heads) * head_dim
@@ -681,10 +684,10 @@ def attention_kv8(qkv, out, n_heads, n_kv_heads, head_dim, scale, window, batch,
     floats = _kv8_part_floats(n_heads, n_kv_heads, head_dim, cache.device_index)
     parts = ws.get("attention_kv8_parts", (floats,), torch.float32)
     _here("attention_kv8", parts, cache.k)
-    fn = _typed(lib.abk_attention_kv8, "plpiifippppppplp")
+    fn = _typed(lib.abk_attention_kv8, "plpiifippppppplip")
     _check(lib, fn(qkv.data_ptr(), row, out.data_ptr(), n, n_heads, scale, window or 0, batch.token_seq.data_ptr(), batch.token_pos.data_ptr(),
-                   batch.seq_slot.data_ptr(), batch.seq_pos0.data_ptr(), batch.seq_len_after.data_ptr(), record, parts.data_ptr(), floats, _raw_stream()),
-           "attention_kv8", kernels=2 * -(-n // 512))
+                   batch.seq_slot.data_ptr(), batch.seq_pos0.data_ptr(), batch.seq_len_after.data_ptr(), record, parts.data_ptr(), floats,
+                   1 if batch.kv8_written is cache else 0, _raw_stream()), "attention_kv8", kernels=2 * -(-n // 512))
 
 
 def attention(qkv, out, n_heads, n_kv_heads, head_dim, scale, window, batch, cache, from_step=False, ws=None, lists=None,

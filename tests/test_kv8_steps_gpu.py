@@ -108,3 +108,34 @@ def test_open_tokens_before_the_window_may_hold_anything(ops, ring, bad):  # noq
     for _ in range(3):
         qkv = run.rows(2)
         run.attend(ops, run.write(ops, [(a, 1), (b, 1)], qkv), qkv)
+
+
+@pytest.mark.parametrize("form", ["int8", "e4m3"])
+def test_attention_right_behind_a_write_of_another_step(ops, form):  # noqa: F811
+    """Rows that attend to what a larger step's kv8_write has just put into the cache: the last tokens of a long prompt as a step of their
+    own, and a decode step moved on by the device. Such calls wait for the launch before (the same step's kv8_write lets them read ahead)."""
+    from abacus_b200.engine.batch import Sequence, StepBatch
+    run = Run(8, 2, 128, form, slots=6, pages=400, max_context=1 << 13)
+    for new in (4, 1):
+        slots = [run.open() for _ in range(3)]
+        lengths = [8000, 5003, 7001]
+        qkv = run.rows(sum(lengths))
+        tail = StepBatch(3 * new, 3, 1, "cuda").fill([Sequence(s, [0] * new, n - new, []) for s, n in zip(slots, lengths)], exact=True)
+        ends = np.cumsum(lengths)
+        rows = torch.cat([qkv[e - new:e] for e in ends])
+        on_gpu, out, whole = rows.cuda(), torch.zeros((3 * new, 8 * 128), dtype=torch.bfloat16, device="cuda"), qkv.cuda()
+        batch = run.batch(list(zip(slots, lengths)))
+        torch.cuda.synchronize()
+        ops.kv8_write(whole, 8, 2, 128, batch, run.kv)
+        ops.attention_kv8(on_gpu, out, 8, 2, 128, 128 ** -0.5, None, tail, run.kv, run.ws)
+        assert batch.kv8_written is run.kv and tail.kv8_written is None
+        torch.cuda.synchronize()
+        again = torch.zeros_like(out)
+        ops.attention_kv8(on_gpu, again, 8, 2, 128, 128 ** -0.5, None, tail, run.kv, run.ws)
+        assert torch.equal(out, again)
+        for s in slots:
+            run.cache.close_slot(s)
+    one = StepBatch(1, 1, 1, "cuda").fill([Sequence(run.open(), [0], 0, [])], exact=True)
+    run.cache.reserve(one.sequences[0].slot, 8)
+    ops.kv8_write(rows[:1].cuda(), 8, 2, 128, one, run.kv)
+    assert one.kv8_written is run.kv and one.advance_on_device().kv8_written is None
