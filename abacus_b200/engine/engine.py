@@ -15,6 +15,7 @@ import torch
 
 from ..cache import TOKENS_PER_PAGE, SequenceCache
 from ..config.registry import load_config
+from ..kernels.ops import KernelRefused
 from ..models.model import Model
 from ..weights.loader import load_folder
 from ..weights.safetensors_io import folder_shapes
@@ -108,6 +109,10 @@ class Engine:
         self.prompt_graphs = PromptGraphs(self, from_start_only=prompt_graphs == "from_start") if prompts else None
         self._step_batch = None
         self._graph_memory = None
+        # an 8-bit cache's layers that take several tokens of a sequence only at its start, or never (keys of another entry's ring)
+        windowed = [e for e in model.schedule if cache is not None and model.blocks[e.layer].mixer.spec.window is not None]
+        self._several_at_start_only = bool(windowed)
+        self._single_only = any(e.source is not None for e in windowed)
 
     @staticmethod
     def _check_kv8(model, form):
@@ -161,6 +166,9 @@ class Engine:
                 bad = tokens[(tokens < 0) | (tokens >= self.vocab)]
                 raise StepError(f"slot {slot}: token {int(bad[0])} is outside the vocabulary of {self.vocab}")
             seqs.append(Sequence(slot, tokens, self.cache.length[slot], [int(w) for w in want]))
+        if self._several_at_start_only and any(len(s.tokens) > 1 and (s.start > 0 or self._single_only) for s in seqs):
+            # (before anything is written: an 8-bit cache's open blocks would keep what the layers before put there)
+            raise KernelRefused("windowed attention takes several tokens of a sequence only at its start, and only with keys of its own")
         self.cache.reserve_all([(s.slot, s.start + len(s.tokens)) for s in seqs])
         return seqs
 

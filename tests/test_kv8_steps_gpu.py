@@ -139,3 +139,36 @@ def test_attention_right_behind_a_write_of_another_step(ops, form):  # noqa: F81
     run.cache.reserve(one.sequences[0].slot, 8)
     ops.kv8_write(rows[:1].cuda(), 8, 2, 128, one, run.kv)
     assert one.kv8_written is run.kv and one.advance_on_device().kv8_written is None
+
+
+def windowed_folder(tmp_path):
+    """A model folder of three layers of heads of 64, the second windowed."""
+    import os
+    from abacus_b200.config import Qwen3Config
+    from abacus_b200.weights import write_random_model
+    raw = dict(hidden_size=128, intermediate_size=160, num_hidden_layers=3, num_attention_heads=4, num_key_value_heads=2, head_dim=64,
+               vocab_size=300, max_position_embeddings=512, rope_theta=10000.0, rms_norm_eps=1e-6, tie_word_embeddings=True,
+               layer_types=["full_attention", "sliding_attention", "full_attention"], sliding_window=40, use_sliding_window=True,
+               architectures=["Qwen3ForCausalLM"], model_type="qwen3")
+    return write_random_model(os.path.join(str(tmp_path), "w"), Qwen3Config.from_dict(raw), seed=4)
+
+
+def test_a_refused_step_leaves_the_cache_as_it_was(tmp_path, ops):  # noqa: F811
+    """Several tokens that go on with a windowed sequence are refused before the layers in front have written: the sequence goes on as if
+    nobody had asked (the refused tokens would have closed its open block and begun another)."""
+    import abacus_b200
+    lm = abacus_b200.LM(windowed_folder(tmp_path), max_tokens=64 * 12, cache="int8")
+    rng = np.random.default_rng(2)
+    tokens, engine, got = rng.integers(0, 300, 60).tolist(), lm.engine, []
+    for asks in (False, True):
+        slot = engine.open()
+        rows = [engine.step([(slot, tokens[:13], [12])]).clone()]
+        if asks:
+            with pytest.raises(ops.KernelRefused, match="windowed"):
+                engine.step([(slot, tokens[:5], [4])])
+            with pytest.raises(ops.KernelRefused, match="windowed"):
+                engine.score([(slot, tokens[:5], [4])], [1])
+        rows += [engine.step([(slot, [t], [0])]).clone() for t in tokens[13:]]
+        got.append(torch.cat(rows))
+        engine.close(slot)
+    assert torch.equal(*got)
