@@ -17,6 +17,7 @@ from ..cache import TOKENS_PER_PAGE, SequenceCache
 from ..config.registry import load_config
 from ..kernels.ops import KernelRefused
 from ..models.model import Model
+from ..parts.attention import KV8_ROWS_UP_TO
 from ..weights.loader import load_folder
 from ..weights.safetensors_io import folder_shapes
 from .batch import Sequence, StepBatch
@@ -62,6 +63,10 @@ class Scoring:
     top_logprobs: torch.Tensor = None  # float32 [rows, k]
     done: bool = False        # the model's frame has seen to it
 
+
+# Tokens whose keys and values a pass over portions reads back from an 8-bit cache at a time (of one sequence, if it holds more): 0.5 GB a
+# layer with 8 kv heads of 128.
+READ_BACK_TOKENS = 1 << 17
 
 _ONE_TOKEN, _WANT_IT = np.zeros(1, dtype=np.int64), [0]
 
@@ -111,6 +116,7 @@ class Engine:
         self._graph_memory = None
         # an 8-bit cache's layers that take several tokens of a sequence only at its start, or never (keys of another entry's ring)
         windowed = [e for e in model.schedule if cache is not None and model.blocks[e.layer].mixer.spec.window is not None]
+        self._borrows = any(e.source is not None for e in model.schedule)
         self._several_at_start_only = bool(windowed)
         self._single_only = any(e.source is not None for e in windowed)
 
@@ -176,20 +182,78 @@ class Engine:
         """Run one step; returns float32 logits [wanted rows, vocab] on the device, in the order of
         the entries and of each entry's `want`."""
         seqs = self.plan(entries)
+        ways = self._ways(seqs)
+        if len(ways) == 1:
+            logits, self.last_batch = self._run(seqs)
+            self._advance(seqs)
+            return logits
+        rows, out = self._rows(seqs), None
+        for way in ways:
+            part = [seqs[i] for i in way]
+            logits, _ = self._run(part)
+            self._advance(part)
+            out = logits.new_empty((rows[-1], logits.shape[1])) if out is None else out
+            self._put(out, logits, way, rows)
+        self._fill_whole(seqs)
+        return out
+
+    def _run(self, seqs):
+        """One forward pass over the sequences of a step: (logits, its StepBatch)."""
         if self.graphs is not None and self.graphs.takes(seqs):  # a plain decode step: replay its graph
             graph = self.graphs.get(seqs)
-            logits = graph.run(seqs)
-            self.last_batch = graph.batch
-        elif self.prompt_graphs is not None and self.prompt_graphs.takes(seqs):  # a shape of prompts seen before
-            logits, self.last_batch = self.prompt_graphs.run(seqs)
-        else:
-            batch = self._room_for(sum(len(s.tokens) for s in seqs), len(seqs), sum(len(s.want) for s in seqs))
-            batch.fill(seqs, exact=True)
-            logits = self.forward(batch)
-            self.last_batch = batch
+            return graph.run(seqs), graph.batch
+        if self.prompt_graphs is not None and self.prompt_graphs.takes(seqs):  # a shape of prompts seen before
+            return self.prompt_graphs.run(seqs)
+        batch = self._room_for(sum(len(s.tokens) for s in seqs), len(seqs), sum(len(s.want) for s in seqs))
+        batch.fill(seqs, exact=True)
+        return self.forward(batch), batch
+
+    def _advance(self, seqs):
         for s in seqs:
             self.cache.advance(s.slot, len(s.tokens))
-        return logits
+
+    def _ways(self, seqs):
+        """The places of a step's sequences by the forward passes they go through. One pass, but with an 8-bit cache: there whole prompts
+        attend to their own keys as they came, sequences that bring a few tokens row by row to what the cache holds, and longer
+        portions to pages read back into 16 bits (parts/attention.py: forward_kv8). Each way has a pass of its own, so that a
+        sequence's numbers do not depend on what else is in the step; portions come READ_BACK_TOKENS of context at a time, so that their
+        pages in 16 bits stay a small share of what the cache holds."""
+        if self.cache.form is None or all(len(s.tokens) == 1 for s in seqs):
+            return [list(range(len(seqs)))]
+        from_start = all(s.start == 0 for s in seqs)
+        ways, portions, held = {}, [[]], 0
+        for i, s in enumerate(seqs):
+            n = len(s.tokens)
+            few = n <= KV8_ROWS_UP_TO
+            if s.start == 0 and (n > 1 or from_start):
+                # (only a layer whose keys are another's reads the cache for a whole prompt, by either way)
+                ways.setdefault(("whole", few and self._borrows), []).append(i)
+            elif few:
+                ways.setdefault("few", []).append(i)
+            else:
+                if portions[-1] and held + s.start + n > READ_BACK_TOKENS:
+                    portions.append([])
+                    held = 0
+                portions[-1].append(i)
+                held += s.start + n
+        return [way for way in [*ways.values(), *portions] if way]
+
+    @staticmethod
+    def _rows(seqs):
+        """The wanted rows in front of each sequence's own, and of all."""
+        return np.concatenate([[0], np.cumsum([len(s.want) for s in seqs])]).tolist()
+
+    @staticmethod
+    def _put(out, part, way, rows):
+        """What a pass gave for the sequences at the places `way` of a step, to their rows of `out`."""
+        index = [r for i in way for r in range(rows[i], rows[i + 1])]
+        if index:
+            out.index_copy_(0, torch.tensor(index, device=out.device), part)
+
+    def _fill_whole(self, seqs):
+        """last_batch for a step that ran in several passes: all of its sequences, in their order."""
+        self.last_batch = self._room_for(sum(len(s.tokens) for s in seqs), len(seqs), sum(len(s.want) for s in seqs))
+        self.last_batch.fill(seqs, exact=True)
 
     def score(self, entries, tokens, top=0):
         """A step (see step) that gives, for every wanted row, the log probability of the given token, the entropy and the `top` most
@@ -202,12 +266,35 @@ class Engine:
             raise StepError(f"{top} most likely tokens: 0 to {min(64, self.vocab)} can be had")
         seqs = self.plan(entries)
         device = self.model.ctx.device
-        batch = self._room_for(sum(len(s.tokens) for s in seqs), len(seqs), rows)
-        batch.fill(seqs, exact=True)
-        number = lambda *shape: torch.empty(shape, dtype=torch.float32, device=device)
         given = torch.tensor(list(tokens), dtype=torch.int32).to(device)
-        batch.scoring = Scoring(given, number(rows), number(rows), torch.empty((rows, top), dtype=torch.int32, device=device) if top else None,
-                                number(rows, top) if top else None)
+        ways = self._ways(seqs)
+        if len(ways) == 1:
+            scoring = self._run_scoring(seqs, given, top)
+        else:
+            rows, scoring = self._rows(seqs), self._scoring(given, top)
+            for way in ways:
+                part = [seqs[i] for i in way]
+                index = torch.tensor([r for i in way for r in range(rows[i], rows[i + 1])], dtype=torch.int64, device=device)
+                got = self._run_scoring(part, given[index], top)
+                for name in ("logprob", "entropy", "top_ids", "top_logprobs"):
+                    if getattr(got, name) is not None:
+                        self._put(getattr(scoring, name), getattr(got, name), way, rows)
+            self._fill_whole(seqs)
+        return scoring.logprob, scoring.entropy, scoring.top_ids, scoring.top_logprobs
+
+    @staticmethod
+    def _scoring(given, top):
+        """Room for the numbers of a step that scores the tokens `given`."""
+        rows, device = given.numel(), given.device
+        number = lambda *shape: torch.empty(shape, dtype=torch.float32, device=device)
+        return Scoring(given, number(rows), number(rows), torch.empty((rows, top), dtype=torch.int32, device=device) if top else None,
+                       number(rows, top) if top else None)
+
+    def _run_scoring(self, seqs, given, top):
+        """One forward pass that scores."""
+        batch = self._room_for(sum(len(s.tokens) for s in seqs), len(seqs), given.numel())
+        batch.fill(seqs, exact=True)
+        batch.scoring = self._scoring(given, top)
         try:
             self.model.forward(batch, self.cache)
             scoring = batch.scoring
@@ -216,9 +303,8 @@ class Engine:
         if not scoring.done:
             raise StepError(f"the model's frame {self.model.spec.frame!r} makes logits of its own and cannot score")
         self.last_batch = batch
-        for s in seqs:
-            self.cache.advance(s.slot, len(s.tokens))
-        return scoring.logprob, scoring.entropy, scoring.top_ids, scoring.top_logprobs
+        self._advance(seqs)
+        return scoring
 
     def forward(self, batch):
         """The model's forward pass over a filled step: in one call to C where that serves the model."""

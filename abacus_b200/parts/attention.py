@@ -183,8 +183,9 @@ class Attention:
             self.cos, self.sin = self.position.tables(max_positions, device)
 
     def forward_kv8(self, xn, out, batch, cache, ws):
-        """The same over an 8-bit cache: whole prompts attend to their own keys as they came, everything else to what the cache
-        holds (cache/kv8.py)."""
+        """The same over an 8-bit cache: a step of whole prompts attends to its own keys as they came, every other to what the cache
+        holds (cache/kv8.py), its own whole blocks in 8 bits too. The engine gives whole prompts, sequences that bring a few tokens and
+        longer portions a pass each (Engine._ways)."""
         s, n, writes = self.spec, batch.n_rows, cache.owns_storage
         if self.general or self.ctx.dtype != torch.bfloat16:
             raise ops.KernelRefused("an 8-bit cache serves plain attention in bfloat16")

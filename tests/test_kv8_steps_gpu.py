@@ -172,3 +172,41 @@ def test_a_refused_step_leaves_the_cache_as_it_was(tmp_path, ops):  # noqa: F811
         got.append(torch.cat(rows))
         engine.close(slot)
     assert torch.equal(*got)
+
+
+@pytest.mark.parametrize("borrows", [False, True])
+@pytest.mark.parametrize("form", ["int8", "e4m3"])
+def test_a_sequence_goes_the_same_way_whatever_is_beside_it(tmp_path, monkeypatch, form, borrows):
+    """A whole prompt, a short one, a portion, a few tokens and a single one in one step give the bits that they give in steps of their own
+    (a prompt attends to its keys as they came beside a sequence that goes on, too), logits and scores; portions that are more context than is read
+    back at a time go one after the other; last_batch holds the step's sequences."""
+    from abacus_b200.config import ScheduleEntry
+    from abacus_b200.engine import Engine, engine as module
+    monkeypatch.setattr(module, "READ_BACK_TOKENS", 150)
+    schedule = (ScheduleEntry(0), ScheduleEntry(1, source=0), ScheduleEntry(1)) if borrows else None
+    model = model_of(make_model_folder(tmp_path, "D"), schedule)
+    rng = np.random.default_rng(5)
+    before, news = [40, 0, 90, 77, 70], [30, 50, 20, 3, 25]
+    if borrows:
+        before, news = before + [0], news + [6]
+    texts = [rng.integers(0, 515, b + n).tolist() for b, n in zip(before, news)]
+    for score in (False, True):
+        got = []
+        for together in (True, False):
+            engine = Engine(model, max_tokens=64 * 20, use_graphs=False, cache=form)
+            slots = [engine.open() for _ in texts]
+            for slot, text, n in zip(slots, texts, before):
+                if n:
+                    engine.step([(slot, text[:n], [])])
+            entries = [(slot, text[n:], [0, len(text) - n - 1] if n != 77 else [1]) for slot, text, n in zip(slots, texts, before)]
+            steps = [entries] if together else [[e] for e in entries]
+            if score:
+                parts = [engine.score(step, [int(t) for _, text, want in step for t in text[:len(want)]], top=3) for step in steps]
+                got.append([torch.cat([p[i] for p in parts]) for i in range(4)])
+            else:
+                got.append([torch.cat([engine.step(step).clone() for step in steps])])
+            if together:
+                assert [s.slot for s in engine.last_batch.sequences] == slots and engine.last_batch.n_rows == sum(news)
+            assert [engine.length(s) for s in slots] == [len(t) for t in texts]
+            engine.check_status()
+        assert all(torch.equal(x, y) for x, y in zip(*got))
