@@ -15,6 +15,8 @@ import os
 import time
 from dataclasses import dataclass
 
+import torch
+
 from .engine import Engine, load_model
 from .engine.generate import Generator, plan_batches, Request
 from .sampling import Sampler
@@ -85,33 +87,44 @@ class LM:
             return [self.tokenizer.decode(r.output) for r in requests]
         return [r.output for r in requests]
 
-
-    def score(self, texts, top=0, raw=True):
+    def score(self, texts, top=0, raw=True, from_cache=False):
         """A Score for each text (token-id lists, or strings, which raw=False wraps as generate does): the log probability of every
         token after the first, and with top > 0 the `top` most likely tokens in its place. Texts go through in batches that
-        fit the cache, and leave nothing there."""
+        fit the cache, and leave nothing there.
+        from_cache: with an 8-bit cache a whole text attends to its own keys as they came, like a prompt, so that its score is the 16-bit
+        model's. With from_cache=True every token attends to keys and values as the cache holds them, and the score shows what the
+        8 bits cost: the first token goes in a step of its own and the others go on with it, one by one where a layer is windowed."""
         as_text = bool(texts) and isinstance(texts[0], str)
         ids = [self.encode(t, raw) for t in texts] if as_text else [[int(t) for t in text] for text in texts]
-        cache = self.engine.cache
+        engine, cache = self.engine, self.engine.cache
         scores = [None] * len(ids)
         requests = [Request(i, tokens, 0) for i, tokens in enumerate(ids)]
-        for batch in plan_batches(requests, self.engine.cache_tokens, cache.max_slots, self.engine.max_context):
-            slots = []
+        for batch in plan_batches(requests, engine.cache_tokens, cache.max_slots, engine.max_context):
+            longest = max(len(r.prompt) for r in batch)
+            cuts = [0, longest] if not from_cache or cache.form is None else [0, 1, longest] if engine.takes_portions else list(range(longest + 1))
+            of_row, numbers, slots = [], [], []  # the place in the batch of each row of numbers
             try:
                 for r in batch:
-                    slots.append(self.engine.open())
-                entries = [(slot, r.prompt, list(range(len(r.prompt) - 1))) for slot, r in zip(slots, batch)]
-                logprob, entropy, top_ids, top_logprobs = self.engine.score(entries, [t for r in batch for t in r.prompt[1:]], top)
-                logprob, entropy = logprob.tolist(), entropy.tolist()
-                best = [list(zip(i, v)) for i, v in zip(top_ids.tolist(), top_logprobs.tolist())] if top else None
+                    slots.append(engine.open())
+                for lo, hi in zip(cuts, cuts[1:]):
+                    here = [(i, r, min(hi, len(r.prompt) - 1)) for i, r in enumerate(batch) if len(r.prompt) > lo]
+                    if here:
+                        entries = [(slots[i], r.prompt[lo:hi], list(range(end - lo))) for i, r, end in here]
+                        numbers.append(engine.score(entries, [t for _, r, end in here for t in r.prompt[lo + 1:end + 1]], top))
+                        of_row += [i for i, _, end in here for _ in range(lo, end)]
+                logprob, entropy = (torch.cat([n[i] for n in numbers]).tolist() for i in (0, 1))
+                best = [torch.cat([n[i] for n in numbers]).tolist() for i in (2, 3)] if top else None
             finally:
                 for slot in slots:
-                    self.engine.close(slot)
-            at = 0
-            for r in batch:
-                n = len(r.prompt) - 1
-                scores[r.index] = Score(r.prompt, logprob[at:at + n], entropy[at:at + n], best[at:at + n] if top else None)
-                at += n
+                    engine.close(slot)
+            made = [Score(r.prompt, [], [], [] if top else None) for r in batch]
+            for row, i in enumerate(of_row):
+                made[i].logprobs.append(logprob[row])
+                made[i].entropies.append(entropy[row])
+                if top:
+                    made[i].top.append(list(zip(best[0][row], best[1][row])))
+            for r, s in zip(batch, made):
+                scores[r.index] = s
         self.engine.check_status()
         return scores
 

@@ -26,7 +26,7 @@ USAGE = """usage: abacus MODEL [options]
   --fp32           run everything in true 32-bit floating point (default: bfloat16)
   --top-k K        sample among the K most likely tokens (default 20, at most 64; 0: all tokens)
   --batch B        with --bench: B sequences at once (default 1)
-  --score TEXT     print how likely the text is (JSON); with --ids: the ids instead, TEXT may be empty
+  --score TEXT     print how likely the text is (JSON), with --kv8 as read from that cache; with --ids: the ids instead, TEXT may be empty
   --kv8 FORM       keep keys and values in 8 bits, int8 or e4m3 (plain attention, bfloat16)
   -t N, --q4       abacus's CPU threads and 4-bit weights: not built here
 """
@@ -187,7 +187,7 @@ def main(argv=None):
         if o.ids is None and lm.tokenizer is None:
             sys.stderr.write("abacus: this model folder has no tokenizer.json; use --ids\n")
             return 1
-        s = lm.score([o.ids if o.ids is not None else lm.encode(o.score, raw=True)])[0]
+        s = lm.score([o.ids if o.ids is not None else lm.encode(o.score, raw=True)], from_cache=o.kv8 is not None)[0]
         n = max(len(s.logprobs), 1)
         print(json.dumps({"tokens": len(s.tokens), "logprob": round(s.total, 4), "perplexity": round(math.exp(-s.total / n), 4),
                           "mean_entropy": round(sum(s.entropies) / n, 4)}))

@@ -114,10 +114,10 @@ class Engine:
         self.prompt_graphs = PromptGraphs(self, from_start_only=prompt_graphs == "from_start") if prompts else None
         self._step_batch = None
         self._graph_memory = None
-        # an 8-bit cache's layers that take several tokens of a sequence only at its start, or never (keys of another entry's ring)
+        # the windowed layers of an 8-bit cache take several tokens of a sequence only at its start, or never (keys of another entry's ring)
         windowed = [e for e in model.schedule if cache is not None and model.blocks[e.layer].mixer.spec.window is not None]
         self._borrows = any(e.source is not None for e in model.schedule)
-        self._several_at_start_only = bool(windowed)
+        self.takes_portions = not windowed
         self._single_only = any(e.source is not None for e in windowed)
 
     @staticmethod
@@ -172,7 +172,7 @@ class Engine:
                 bad = tokens[(tokens < 0) | (tokens >= self.vocab)]
                 raise StepError(f"slot {slot}: token {int(bad[0])} is outside the vocabulary of {self.vocab}")
             seqs.append(Sequence(slot, tokens, self.cache.length[slot], [int(w) for w in want]))
-        if self._several_at_start_only and any(len(s.tokens) > 1 and (s.start > 0 or self._single_only) for s in seqs):
+        if not self.takes_portions and any(len(s.tokens) > 1 and (s.start > 0 or self._single_only) for s in seqs):
             # (before anything is written: an 8-bit cache's open blocks would keep what the layers before put there)
             raise KernelRefused("windowed attention takes several tokens of a sequence only at its start, and only with keys of its own")
         self.cache.reserve_all([(s.slot, s.start + len(s.tokens)) for s in seqs])

@@ -210,3 +210,41 @@ def test_a_sequence_goes_the_same_way_whatever_is_beside_it(tmp_path, monkeypatc
             assert [engine.length(s) for s in slots] == [len(t) for t in texts]
             engine.check_status()
         assert all(torch.equal(x, y) for x, y in zip(*got))
+
+
+@pytest.mark.parametrize("form", ["int8", "e4m3"])
+@pytest.mark.parametrize("windowed", [False, True])
+def test_a_score_reads_the_8_bit_cache(tmp_path, form, windowed):
+    """LM.score(from_cache=True): the numbers of texts whose tokens go on with their first one (single tokens where a layer is windowed), which
+    are not those of whole texts, the default's. Texts of one token, of two, unequal ones. A 16-bit cache has one kind of score."""
+    import abacus_b200
+    folder = windowed_folder(tmp_path) if windowed else make_model_folder(tmp_path, "D")
+    lm = abacus_b200.LM(folder, max_tokens=64 * 20, cache=form)
+    rng = np.random.default_rng(8)
+    texts = [rng.integers(0, 300, n).tolist() for n in (1, 2, 75, 40)]
+    engine = lm.engine
+
+    def by_hand(cuts):
+        slots, rows = [engine.open() for _ in texts], [[] for _ in texts]
+        for lo, hi in zip(cuts, cuts[1:]):
+            here = [i for i, t in enumerate(texts) if len(t) > lo]
+            wants = [list(range(min(hi, len(texts[i]) - 1) - lo)) for i in here]
+            got = engine.score([(slots[i], texts[i][lo:hi], w) for i, w in zip(here, wants)],
+                               [texts[i][lo + 1 + p] for i, w in zip(here, wants) for p in w], top=2)
+            at = 0
+            for i, w in zip(here, wants):
+                rows[i] += zip(*(x[at:at + len(w)].tolist() for x in got))
+                at += len(w)
+        for s in slots:
+            engine.close(s)
+        return rows
+
+    for from_cache, cuts in ((False, (0, 75)), (True, range(76) if windowed else (0, 1, 75))):
+        scores = lm.score(texts, top=2, from_cache=from_cache)
+        for s, text, rows in zip(scores, texts, by_hand(list(cuts))):
+            assert s.tokens == text and len(s.logprobs) == len(s.entropies) == len(s.top) == len(text) - 1
+            assert [(p, h, [i for i, _ in t], [v for _, v in t]) for p, h, t in zip(s.logprobs, s.entropies, s.top)] == rows
+    assert lm.score(texts)[2].logprobs == lm.score(texts, from_cache=False)[2].logprobs != lm.score(texts, from_cache=True)[2].logprobs
+    assert lm.engine.cache.free_pages == lm.engine.cache.n_pages
+    plain = abacus_b200.LM(folder, max_tokens=64 * 20)
+    assert plain.score(texts, from_cache=True)[2].logprobs == plain.score(texts)[2].logprobs
