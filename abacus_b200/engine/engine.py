@@ -61,7 +61,6 @@ class Scoring:
     entropy: torch.Tensor     # float32
     top_ids: torch.Tensor = None       # int32 [rows, k], or None
     top_logprobs: torch.Tensor = None  # float32 [rows, k]
-    done: bool = False        # the model's frame has seen to it
 
 
 # Tokens whose keys and values a pass over portions reads back from an 8-bit cache at a time (of one sequence, if it holds more): 0.5 GB a
@@ -264,6 +263,8 @@ class Engine:
             raise StepError(f"{len(tokens)} tokens to score at {rows} wanted places")
         if not 0 <= top <= min(64, self.vocab):
             raise StepError(f"{top} most likely tokens: 0 to {min(64, self.vocab)} can be had")
+        if not getattr(self.model.frame.logits, "scores", False):  # (before a recurrent state has moved on)
+            raise StepError(f"the model's frame {self.model.spec.frame!r} makes logits of its own and cannot score")
         seqs = self.plan(entries)
         device = self.model.ctx.device
         given = torch.tensor(list(tokens), dtype=torch.int32).to(device)
@@ -300,8 +301,6 @@ class Engine:
             scoring = batch.scoring
         finally:
             batch.scoring = None
-        if not scoring.done:
-            raise StepError(f"the model's frame {self.model.spec.frame!r} makes logits of its own and cannot score")
         self.last_batch = batch
         self._advance(seqs)
         return scoring

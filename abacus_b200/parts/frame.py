@@ -11,7 +11,8 @@ A frame has
   bind(params, ctx)
   embed(batch, ws, status) -> x           float32 [rows, hidden], the residual stream
   logits(x, y, batch, ws) -> float32 [batch.n_logit_rows, vocab], or nothing of them for a step that scores (batch.scoring):
-                                          `end` does either behind the frame's last norm
+                                          `end` does either behind the frame's last norm, and a logits() that ends there
+                                          is marked @scores
   step_weights() -> tensors a step reads once whatever its size
 """
 import torch
@@ -20,6 +21,12 @@ from ..kernels import ops
 from .base import FRAMES, NORMS, to_device
 from .linear import Linear
 from .position import Sinusoids
+
+
+def scores(logits):
+    """Marks a frame's logits() that leaves log probabilities where a step scores (a subclass's own logits() is marked anew)."""
+    logits.scores = True
+    return logits
 
 
 LOGIT_ROWS = 512  # rows whose logits a step that scores keeps at a time, where it needs them
@@ -34,7 +41,6 @@ def end(frame, batch, ws, norm):
         out = ws.get("logits", (max(r, 1), frame.vocab), torch.float32)[:r]
     else:
         out = ws.get("logits", (1, frame.vocab), torch.float32)[:0]
-        scoring.done = True
     if not r:
         return out
     xn = ws.get("xn_final", (r, frame.hidden), frame.ctx.dtype)
@@ -86,6 +92,7 @@ class PlainFrame:
         ops.embed(batch.tokens, self.table, x, status)
         return x
 
+    @scores
     def logits(self, x, y, batch, ws):
         return end(self, batch, ws, lambda xn, rows, r: self.final_norm.forward(x, y, xn, rows=rows, n_rows=r))
 
@@ -137,6 +144,7 @@ class PairsFrame:
             ops.remember_tokens(batch, remembered)
         return x
 
+    @scores
     def logits(self, x, pending, batch, ws):
         from .streams import read_streams
         return end(self, batch, ws, lambda xn, rows, r: read_streams(x, pending, self.ones, self.final_norm, xn, rows=rows, n_rows=r))
@@ -188,6 +196,7 @@ class PositionsFrame:
             raise ValueError("the schedule joins the embedding again, but the frame does not keep it")
         ops.rejoin(x, self.kept, batch.n_rows)
 
+    @scores
     def logits(self, x, pending, batch, ws):
         from .streams import read_streams
         return end(self, batch, ws, lambda xn, rows, r: read_streams(x, pending, self.ones, self.final_norm, xn, rows=rows, n_rows=r))
@@ -252,6 +261,7 @@ class LoopInputFrame:
         ops.add_vector(x, self.loop_step[t], n)
         return None
 
+    @scores
     def logits(self, x, pending, batch, ws):
         from .streams import read_streams
         return end(self, batch, ws, lambda xn, rows, r: read_streams(x, pending, self.ones, self.final_norm, xn, rows=rows, n_rows=r))
@@ -265,6 +275,7 @@ class NormedEndFrame(PlainFrame):
         super().__init__(spec)
         self.options = spec.frame_spec
 
+    @scores
     def logits(self, x, pending, batch, ws):
         return end(self, batch, ws, lambda xn, rows, r: self.final_norm.forward_normed(x, pending, xn, rows=rows, n_rows=r))
 
