@@ -20,6 +20,7 @@ from dataclasses import dataclass, field
 import torch
 
 from ..cache.kv import TOKENS_PER_PAGE
+from ..kernels import ops
 
 
 @dataclass
@@ -113,6 +114,11 @@ class Generator:
         loop prints each piece as it comes, src/main.c:177-180). logprobs: None, or how many most likely tokens a request keeps beside each of
         its own and its log probability."""
         self.engine, self.sampler, self.stop_tokens, self.on_token = engine, sampler, tuple(stop_tokens), on_token
+        if logprobs is not None:
+            most = min(ops.LOGPROBS_MAX_TOP, getattr(engine, "vocab", ops.LOGPROBS_MAX_TOP))
+            if logprobs != int(logprobs) or not 0 <= logprobs <= most:
+                raise ValueError(f"logprobs={logprobs}: 0 to {most} most likely tokens can be had beside each one")
+            logprobs = int(logprobs)
         self.logprobs = logprobs
         self.stats = {"prefill_steps": 0, "decode_steps": 0, "batches": 0}
         self.rng = None
@@ -136,39 +142,43 @@ class Generator:
         return all(r.max_new_tokens > 0 and len(r.output) + 1 < r.max_new_tokens
                    and len(r.prompt) + len(r.output) + 1 < max_context for r in rows)
 
-    def _read_beside(self, drawn):
-        """Start copying `drawn` (int32 on the device) to the host on a stream of its own, ordered after what the
+    def _read_beside(self, *tensors):
+        """Start copying `tensors` (int32 or float32 on the device) to the host on a stream of its own, ordered after what the
         current stream holds now but not after what is launched on it later. Returns a function that waits for
-        the copy and gives the list."""
-        if drawn.device.type != "cuda":
-            return drawn.tolist
+        the copies and gives them as lists."""
+        device = tensors[0].device
+        if device.type != "cuda":
+            return lambda: [t.tolist() for t in tensors]
         if getattr(self, "_copy_stream", None) is None:
-            self._copy_stream = torch.cuda.Stream(drawn.device)
-            self._landing = torch.empty(4096, dtype=torch.int32).pin_memory()
-        n = drawn.numel()
-        if n > self._landing.numel():
-            return drawn.tolist
-        self._copy_stream.wait_stream(torch.cuda.current_stream(drawn.device))
+            self._copy_stream, self._landing = torch.cuda.Stream(device), None
+        ends = [0]
+        for t in tensors:
+            ends.append(ends[-1] + t.numel())
+        if self._landing is None or self._landing.numel() < ends[-1]:
+            self._landing = torch.empty(max(4096, 2 * ends[-1]), dtype=torch.int32).pin_memory()
+        self._copy_stream.wait_stream(torch.cuda.current_stream(device))
+        landed = [self._landing[a:b].view(t.dtype).view(t.shape) for t, a, b in zip(tensors, ends, ends[1:])]
         with torch.cuda.stream(self._copy_stream):
-            self._landing[:n].copy_(drawn, non_blocking=True)
+            for t, to in zip(tensors, landed):
+                to.copy_(t, non_blocking=True)
             done = torch.cuda.Event()
             done.record()
-        drawn.record_stream(self._copy_stream)
+        for t in tensors:
+            t.record_stream(self._copy_stream)
 
         def read():
             done.synchronize()
-            return self._landing[:n].tolist()
+            return [t.tolist() for t in landed]
         return read
 
     def _score(self, logits, drawn):
-        """The drawn tokens' log probabilities and the most likely tokens (launched at once: a step that runs ahead takes the logits'
-        place). Returns a function that gives them, [(log probability, [(token, log probability)])] by row."""
-        from ..kernels import ops
+        """The drawn tokens' log probabilities, and the most likely tokens with theirs, by row (launched at once: a step that runs ahead
+        takes the logits' place)."""
         n, k, device = drawn.numel(), self.logprobs, logits.device
         logprob = torch.empty(n, dtype=torch.float32, device=device)
         ids, values = torch.empty((n, k), dtype=torch.int32, device=device), torch.empty((n, k), dtype=torch.float32, device=device)
         ops.token_logprobs(logits, drawn, logprob, top_ids=ids if k else None, top_logprobs=values if k else None, n_rows=n)
-        return lambda: [(p, list(zip(i, v))) for p, i, v in zip(logprob.tolist(), ids.tolist(), values.tolist())]
+        return logprob, ids, values
 
     def run_batch(self, batch):
         engine = self.engine
@@ -188,24 +198,24 @@ class Generator:
             while True:
                 rows = list(live.live)
                 drawn = self.sampler.sample(logits, self.rng, index=index)
-                scored = self._score(logits, drawn) if self.logprobs is not None else None
+                wanted = (drawn, *self._score(logits, drawn)) if self.logprobs is not None else (drawn,)
                 ahead = None
                 if self._may_run_ahead(rows, engine, live.max_context):
-                    read = self._read_beside(drawn)
+                    read = self._read_beside(*wanted)
                     ahead = engine.step_ahead([r.slot for r in rows], drawn)
-                    sampled = read() if ahead is not None else drawn.tolist()
+                    sampled, *scored = read()
                 else:
-                    sampled = drawn.tolist()
+                    sampled, *scored = [t.tolist() for t in wanted]
                 now = time.perf_counter()  # the tokens are on the host
                 self.stats.setdefault("t_first_token", now)
                 self.stats["t_end"] = now
                 kept = [len(r.output) for r in rows]
                 finished, entries = live.take(sampled)
-                if scored is not None:
-                    for r, n, (logprob, top) in zip(rows, kept, scored()):
+                if scored:
+                    for r, n, logprob, ids, values in zip(rows, kept, *scored):
                         if len(r.output) > n:
                             r.logprobs.append(logprob)
-                            r.top.append(top)
+                            r.top.append(list(zip(ids, values)))
                 if self.on_token is not None:
                     for r, n in zip(rows, kept):
                         for token in r.output[n:]:

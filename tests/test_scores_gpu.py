@@ -31,3 +31,54 @@ def test_a_frame_that_cannot_score_is_refused_before_anything_moves(tmp_path):
     assert engine.length(slot) == 7 and before
     assert all(torch.equal(x, y) for x, y in zip(before, engine.cache.save_states([slot])[1]))
     assert engine.score([(slot, [1], [0])], [2])[0].isfinite().all()
+
+
+@pytest.mark.parametrize("logprobs", [None, 0, 5])
+def test_tokens_and_their_log_probabilities_do_not_wait_for_the_step_that_runs_ahead(logprobs):
+    """An engine whose step ahead takes the GPU a tenth of a second: on_token has each token, with its log probability and the most likely
+    ones, while that step is still running."""
+    from abacus_b200.engine.generate import Generator
+    from abacus_b200.sampling import Sampler
+
+    class Engine:
+        max_context, vocab = 64, 50
+
+        class cache:
+            n_pages, max_slots = 4, 2
+
+        ended = None
+
+        def open(self):
+            return 0
+
+        def close(self, slot):
+            pass
+
+        def logits(self, last):
+            out = torch.zeros((1, 50), device="cuda")
+            out[:, (last + 1) % 50].fill_(9.0)
+            self.last, self.last_batch = last + 1, type("B", (), {"seq_slot": torch.zeros(1, dtype=torch.int32, device="cuda")})()
+            return out
+
+        def step(self, entries):
+            return self.logits(entries[0][1][-1])
+
+        def step_ahead(self, slots, tokens):
+            torch.cuda._sleep(200_000_000)  # (cycles)
+            out = self.logits(self.last)
+            self.ended = torch.cuda.Event()
+            self.ended.record()
+            return out
+
+    engine, seen = Engine(), []
+    gen = Generator(engine, Sampler("cuda", temperature=0.0), logprobs=logprobs,
+                    on_token=lambda r, token: seen.append((token, len(r.logprobs), engine.ended is not None and not engine.ended.query())))
+    gen.generate([[1, 2]], max_new_tokens=2)  # (loads the kernels)
+    seen.clear()
+    engine.ended = None
+    r = gen.generate([[1, 2]], max_new_tokens=5)[0]
+    assert r.output == [3, 4, 5, 6, 7]
+    has = 0 if logprobs is None else 1
+    assert seen == [(3 + i, has * (i + 1), i < 4) for i in range(5)]
+    if logprobs:
+        assert all(top[0][0] == token and top[0][1] == p and len(top) == logprobs for token, p, top in zip(r.output, r.logprobs, r.top))
