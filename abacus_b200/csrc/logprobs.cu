@@ -10,14 +10,17 @@
 // running maximum and the two sums over its elements, four 16-byte pieces at a time, the next four on their way; nothing in the walk waits for
 // another warp. The most likely tokens: an element is noted, in the warp's own list in shared memory, only where it reaches a bound
 // that at least k elements of the slice reach: every warp leaves its ceil(k / 8)-th largest thread maximum in shared memory as it goes,
-// and of these the one that enough warps reach is the bound (one that is out of date is only lower). A list that fills up is cut to its best k; a
+// and of these the one that enough warps reach is the bound (one that is out of date is only lower). Where fewer warps have elements (a short
+// slice, a mask that leaves one range of tokens) each leaves more. A list that fills up is cut to its best k; a
 // warp meets its elements by rising index, so from then on an equal of the k-th need not be noted. At the end the elements that
 // reach the last bound, some tens, are ranked by counting those before each, and once more those of a cluster's CTAs. Elements of -inf are
 // never noted: where a row has fewer than k others, the first of them fill its places.
 //
-// Measured: 512 rows of 151,936 float32 logits with 5 alternatives in 66 us, 4.7 TB/s (53 without); 8 rows with 20 in 12.5 to 13.9 (9.4 without), a
+// Measured: 512 rows of 151,936 float32 logits with 5 alternatives in 61 us, 5.1 TB/s (50 without); 8 rows with 20 in 12.5 to 13.9 (9.4 without), a
 // chain of three turns of loads, bounds, ranks and the cluster's fold; 200 rows of 50,261 bfloat16 logits, a twentieth not -inf, with 64
-// in 24: there every turn of 1,024 elements has some to note.
+// in 24: there every turn of 1,024 elements has some to note. Short slices and ranges, with 1, 20 and 64 alternatives: 32 rows of 65,536 bfloat16 logits
+// 14, 18.5 and 26, 600 rows of 6,000 9, 12 and 16, 500 rows of 1,500 float32 ones 6, 8 and 13.5, 64 rows of 151,936 with 1,000 neighbours
+// left 13, 16 and 20 (float32) and 18, 21 and 33 (bfloat16). Most of a row's elements as alternatives are ranked the long way: 600 rows of 500 with 64 98.
 #define ABK_DEFINE_ERROR
 #include "common.cuh"
 #include "tc_common.cuh"
@@ -32,6 +35,7 @@ static_assert(LOGPROBS_MAX_SPLITS >= 2 * LOGPROBS_WARPS, "room for all lists");
 // 50,261 with 64 alternatives take 27.7 us, not 24.2; four spill some registers (64 bytes of stores), three (12 bytes)
 // take the same 24.2, and rows without many to note show no difference.
 #define LOGPROBS_PIECES 4
+#define LOGPROBS_LOWEST (-3.402823466e38f)
 #define LOGPROBS_NOTED 128  // elements a warp's list has room for beside those of one piece of every lane
 
 struct LogProbs {
@@ -95,33 +99,45 @@ __device__ __noinline__ int cut_to_best(Ranked *list, Ranked *spare, int n, int 
     return n;
 }
 
-// What the warps of a CTA know of the most likely elements, in shared memory.
+// What the warps of a CTA know of the most likely elements, in shared memory. At level L k elements of the slice are looked for in
+// LOGPROBS_WARPS >> L warps, ceil(k / that many) in each: level 0 where all warps have elements, the others where a slice is short
+// or a mask leaves one range of tokens.
+#define LOGPROBS_LEVELS 4
+static_assert(LOGPROBS_WARPS >> (LOGPROBS_LEVELS - 1) == 1 && LOGPROBS_LEVELS * LOGPROBS_WARPS == 32, "a lane a level and warp");
 struct Bounds {
-    volatile float of_warp[LOGPROBS_WARPS];  // what ceil(k / 8) of a warp's elements reach
-    volatile float common;                   // what k elements of the slice reach, as of some moment
+    volatile float of_warp[LOGPROBS_LEVELS][LOGPROBS_WARPS];  // what that many of a warp's elements reach
+    volatile float common;                                    // what k elements of the slice reach, as of some moment
 };
-// A warp's bound: the in_warp-th largest of its lanes' numbers.
-__device__ __forceinline__ void leave_bound(Bounds *b, float of_lane, int in_warp, int warp, int lane) {
-    float x = -INFINITY;
-    for (int r = 0; r < in_warp; r++) {
-        x = largest_of_lanes(of_lane);
-        const unsigned holders = __ballot_sync(0xffffffffu, of_lane == x);
-        if (lane == __ffs(holders) - 1) of_lane = -INFINITY;  // one of them is taken out
-    }
-    if (lane == 0) b->of_warp[warp] = x;
+// Elements a warp at a level: ceil(top / warps)
+__device__ __forceinline__ int in_warp_at(int top, int level) {
+    const int shift = LOGPROBS_LEVELS - 1 - level;
+    return (top + (1 << shift) - 1) >> shift;
 }
-// What k elements of the slice reach: ceil(k / in_warp) warps have in_warp of them that reach it. The bounds of this moment or earlier
-// ones, either will do.
-__device__ __forceinline__ float common_bound(const Bounds *bounds, int top, int in_warp, int lane) {
-    const float b = bounds->of_warp[lane & (LOGPROBS_WARPS - 1)];
+// A warp's bounds at the first levels: the in_warp_at()-th largest of its lanes' numbers (none where it has fewer lanes).
+__device__ __forceinline__ void leave_bounds(Bounds *b, float of_lane, int top, int levels, int warp, int lane) {
+    float x = -INFINITY;
+    for (int level = 0, r = 0; level < levels; level++) {
+        const int in_warp = in_warp_at(top, level);
+        if (in_warp > 32) return;
+        for (; r < in_warp; r++) {
+            x = largest_of_lanes(of_lane);
+            const unsigned holders = __ballot_sync(0xffffffffu, of_lane == x);
+            if (lane == __ffs(holders) - 1) of_lane = -INFINITY;  // one of them is taken out
+        }
+        if (lane == 0) b->of_warp[level][warp] = x;
+    }
+}
+// What k elements of the slice reach: at its level a lane's warp is the `need`-th that has in_warp_at() of them that reach it. The bounds
+// of this moment or earlier ones, either will do.
+__device__ __forceinline__ float common_bound(const Bounds *bounds, int need, int lane) {
+    const float b = (&bounds->of_warp[0][0])[lane];
     int above = 0;  // (equals in the order of the warps)
 #pragma unroll
     for (int w = 0; w < LOGPROBS_WARPS; w++) {
-        const float o = __shfl_sync(0xffffffffu, b, w);
+        const float o = __shfl_sync(0xffffffffu, b, w, LOGPROBS_WARPS);
         above += o > b || (o == b && w < (lane & (LOGPROBS_WARPS - 1)));
     }
-    const unsigned at = __ballot_sync(0xffffffffu, above == (top + in_warp - 1) / in_warp - 1);
-    return __shfl_sync(0xffffffffu, b, __ffs(at) - 1);
+    return largest_of_lanes(above == need - 1 ? b : -INFINITY);
 }
 // A warp's list: n elements, and what an element has to reach to be noted.
 struct Noted {
@@ -144,14 +160,14 @@ __device__ __forceinline__ void make_room(Noted &noted, Ranked *list, Ranked *sp
     noted.n = cut_to_best(list, spare, noted.n, top, lane);
     if (noted.n == top) noted.cut = fmaxf(noted.cut, next_up(list[noted.n - 1].v));
 }
-// The elements of a warp's 32 * U pieces from j0 on that reach the cut, read again behind their sums (the walk's own copies would have
+// The elements of a warp's 32 * U pieces (32 of every LOGPROBS_THREADS, from j0 on) that reach the cut, read again behind their sums (the walk's own copies would have
 // to stay in registers for this: 512 rows of 151,936 with the 5 most likely take 71 us so, not 66).
 template <typename T> __device__ __forceinline__ Noted note_pieces(const uint4 *src, int j0, int pieces, int body, Noted noted, Ranked *list,
                                                                 Ranked *spare, int top, int lane) {
     constexpr int N = Piece<T>::N, U = LOGPROBS_PIECES;
     uint4 w[U];
 #pragma unroll
-    for (int u = 0; u < U; u++) w[u] = j0 + 32 * u + lane < pieces ? __ldg(src + j0 + 32 * u + lane) : Piece<T>::nothing();
+    for (int u = 0; u < U; u++) w[u] = j0 + LOGPROBS_THREADS * u + lane < pieces ? __ldg(src + j0 + LOGPROBS_THREADS * u + lane) : Piece<T>::nothing();
 #pragma unroll
     for (int u = 0; u < U; u++) {
         float v[N];
@@ -162,16 +178,17 @@ template <typename T> __device__ __forceinline__ Noted note_pieces(const uint4 *
         if (!__any_sync(0xffffffffu, of_piece >= noted.cut)) continue;
         make_room(noted, list, spare, top, lane);
 #pragma unroll
-        for (int e = 0; e < N; e++) note(noted, list, v[e], body + (j0 + 32 * u + lane) * N + e, j0 + 32 * u + lane < pieces, lane);
+        for (int e = 0; e < N; e++) note(noted, list, v[e], body + (j0 + LOGPROBS_THREADS * u + lane) * N + e, j0 + LOGPROBS_THREADS * u + lane < pieces, lane);
     }
     return noted;
 }
-// The bound moves with a thread's maximum that counts.
-__device__ __forceinline__ void move_bound(Bounds *b, float of_lane, int top, int in_warp, int warp, int lane) {
-    leave_bound(b, of_lane, in_warp, warp, lane);
+// The bound moves with a thread's maximum that counts; returns it.
+__device__ __forceinline__ float move_bound(Bounds *b, float of_lane, int top, int levels, int need, int warp, int lane) {
+    leave_bounds(b, of_lane, top, levels, warp, lane);
     __syncwarp();
-    const float x = common_bound(b, top, in_warp, lane);
+    const float x = common_bound(b, need, lane);
     if (lane == 0) b->common = x;
+    return x;
 }
 
 template <typename T, bool TOP>
@@ -185,6 +202,7 @@ __global__ void __launch_bounds__(LOGPROBS_THREADS, sizeof(T) == 4 ? 4 : 3) logp
     const int split = (int)tc::cluster_rank(), splits = (int)tc::cluster_size(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int row = blockIdx.y;
     if (threadIdx.x == 0) count = 0, bounds.common = -INFINITY;
+    if (TOP && lane < LOGPROBS_LEVELS) bounds.of_warp[lane][warp] = -INFINITY;
     pdl_wait();
     const T *x = (const T *)p.logits + row * p.stride;
     // slices start on a 16-byte boundary of memory; slice 0 also takes the elements before the first one
@@ -197,7 +215,7 @@ __global__ void __launch_bounds__(LOGPROBS_THREADS, sizeof(T) == 4 ? 4 : 3) logp
         const int token = p.tokens[row];
         if (token >= 0 && token < p.vocab) given = to_float(x[token]);
     }
-    float m = -3.402823466e38f;
+    float m = LOGPROBS_LOWEST;
     float2 l = make_float2(0.0f, 0.0f), t = l;  // of the elements at even places and at odd ones
     auto sum = [&](const float2 *v, int pairs, float most) {
         if (most > m) {
@@ -212,8 +230,10 @@ __global__ void __launch_bounds__(LOGPROBS_THREADS, sizeof(T) == 4 ? 4 : 3) logp
         }
     };
     Ranked *list = lists[TOP ? warp : 0], *spare = cand + (TOP ? warp * LOGPROBS_MAX_TOP : 0);
-    Noted noted = {0, -3.402823466e38f};
-    const int in_warp = (p.top + LOGPROBS_WARPS - 1) / LOGPROBS_WARPS;
+    Noted noted = {0, LOGPROBS_LOWEST};
+    // levels that a bound of the first turn needs: as many warps as it has have a piece a lane
+    const int filled = min(pieces, LOGPROBS_THREADS) / 32, levels = filled >= 8 ? 1 : filled >= 4 ? 2 : filled >= 2 ? 3 : 4;
+    const int in_warp = TOP ? in_warp_at(p.top, lane >> 3) : 1, need = (p.top + in_warp - 1) / in_warp;  // of the lane's level
     auto loose = [&](int from, int to) {  // elements outside the pieces, a lane each
         const int at = from + lane;
         const float v = at < to ? to_float(x[at]) : -INFINITY;
@@ -221,19 +241,23 @@ __global__ void __launch_bounds__(LOGPROBS_THREADS, sizeof(T) == 4 ? 4 : 3) logp
         if (at < to) sum(&alone, 1, v);
         if (TOP) make_room(noted, list, spare, p.top, lane), note(noted, list, v, at, at < to, lane);
     };
+    // With most likely tokens a thread's pieces lie LOGPROBS_THREADS apart: all warps have some of a short slice, and of a range of tokens that a
+    // mask leaves. Without, a warp's lie side by side.
+    constexpr int APART = TOP ? LOGPROBS_THREADS : 32;
     auto load = [&](int j0, uint4 *w) {
-        if (j0 + 32 * U <= pieces) {
+        if (j0 + APART * (U - 1) + 32 <= pieces) {
 #pragma unroll
-            for (int u = 0; u < U; u++) w[u] = __ldcs(src + j0 + 32 * u + lane);
+            for (int u = 0; u < U; u++) w[u] = __ldcs(src + j0 + APART * u + lane);
         } else {
 #pragma unroll
-            for (int u = 0; u < U; u++) w[u] = j0 + 32 * u + lane < pieces ? __ldcs(src + j0 + 32 * u + lane) : Piece<T>::nothing();
+            for (int u = 0; u < U; u++) w[u] = j0 + APART * u + lane < pieces ? __ldcs(src + j0 + APART * u + lane) : Piece<T>::nothing();
         }
     };
     uint4 w[U];
-    load(warp * U * 32, w);
+    const int from = warp * (TOP ? 32 : U * 32);  // of a turn's pieces
+    load(from, w);
     bool first = true;
-    for (int j0 = warp * U * 32; first || j0 < pieces; j0 += LOGPROBS_THREADS * U) {
+    for (int j0 = from; first || j0 < pieces; j0 += LOGPROBS_THREADS * U) {
         __align__(8) float v[U * N];
 #pragma unroll
         for (int u = 0; u < U; u++) Piece<T>::floats(w[u], v + u * N);
@@ -243,9 +267,9 @@ __global__ void __launch_bounds__(LOGPROBS_THREADS, sizeof(T) == 4 ? 4 : 3) logp
         for (int e = 1; e < U * N; e++) most = fmaxf(most, v[e]);
         if (TOP) {
             if (first) {  // the first bounds
-                leave_bound(&bounds, most, in_warp, warp, lane);
+                leave_bounds(&bounds, most, p.top, levels, warp, lane);
                 __syncthreads();
-                noted.cut = fmaxf(noted.cut, common_bound(&bounds, p.top, in_warp, lane));
+                noted.cut = fmaxf(noted.cut, common_bound(&bounds, need, lane));
             } else {
                 noted.cut = fmaxf(noted.cut, bounds.common);
             }
@@ -255,8 +279,9 @@ __global__ void __launch_bounds__(LOGPROBS_THREADS, sizeof(T) == 4 ? 4 : 3) logp
         sum((const float2 *)v, U * N / 2, most);
         if (TOP && __any_sync(0xffffffffu, most >= noted.cut)) {
             const bool moves = __any_sync(0xffffffffu, most >= noted.cut && risen);  // (else no thread's maximum that counts does)
+            const bool none = noted.cut == LOGPROBS_LOWEST;  // no bound yet: what few warps have may give one
+            if (none || (!first && moves)) noted.cut = fmaxf(noted.cut, move_bound(&bounds, m, p.top, none ? LOGPROBS_LEVELS : levels, need, warp, lane));
             noted = note_pieces<T>(src, j0, pieces, body, noted, list, spare, p.top, lane);
-            if (!first && moves) move_bound(&bounds, m, p.top, in_warp, warp, lane);
         }
         first = false;
     }
@@ -266,7 +291,7 @@ __global__ void __launch_bounds__(LOGPROBS_THREADS, sizeof(T) == 4 ? 4 : 3) logp
     if (TOP) make_room(noted, list, spare, p.top, lane);
     __syncthreads();
     if (TOP) {
-        const float b = common_bound(&bounds, p.top, in_warp, lane);
+        const float b = common_bound(&bounds, need, lane);
         for (int i = lane; i < noted.n; i += 32)
             if (list[i].v >= b) cand[atomicAdd(&count, 1)] = list[i];
     }
