@@ -15,7 +15,9 @@
 // floats with the query heads as the 8 columns (two tiles of them from 9 heads on): scores are keys x heads, the
 // output columns x heads, so nothing is spent on heads that are not there beyond the eighth. An 8-bit number is a float16 number exactly,
 // and q is one too once each head's row is brought below 1 by a power of two (what of a head lies 2^-14 below its largest
-// element keeps an absolute error of 2^-25 of that). The softmax weights are p_j s_b 2^-u in float16, 2^-11 off at most, u
+// element keeps an absolute error of 2^-25 of that). The softmax weights are p_j s_b 2^-u in float16: 2^-11 off at most down
+// to 2^-14 of the largest contribution, below that to within 2^-25 of it (N keys that are all below 2^-25 of it are lost, N 2^-25 of the
+// output at most; the sums that it is divided by are float32 and have them), u
 // chosen per head so that the largest ever seen is about 1: a block of small values with large weights counts as precisely
 // as one of large values. Scores, maximum, sum and output are float32. The open block's keys and values go through the same products
 // in bfloat16, its weights as two bfloat16 parts.

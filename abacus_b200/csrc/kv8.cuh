@@ -27,8 +27,9 @@ template <int FORM> __host__ __device__ constexpr float kv8_top() { return FORM 
 
 // Eight bfloat16 values in 8 bits each; `by` and `inverse` as kv8_steps makes them of the block's largest magnitude.
 // 127 x / most comes as x times a reciprocal, up to 2^-22 off, and is then rounded to 18 bits: where it is halfway between two steps it
-// is exactly that again (8 bits), and where it is not it is 2^-15 or more away (127 x and an odd number times most are whole
-// numbers of 15 bits, at least 1 apart; 448 x likewise). So the rounding to a step is that of the exact quotient, ties to even. A
+// is exactly that again (8 bits), and where it is not it is 2^-16 or more away, relative to itself (2 * 127 x and an odd number times most are
+// whole numbers of 16 bits, at least 1 apart; 254 and 255 come closest, 126.50196; 448 x with fewer bits), which is more than the 2^-18
+// that the rounding moves it. So the rounding to a step is that of the exact quotient, ties to even. A
 // division takes three times as long.
 struct Kv8Steps {
     float by, inverse;

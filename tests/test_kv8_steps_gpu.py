@@ -248,3 +248,20 @@ def test_a_score_reads_the_8_bit_cache(tmp_path, form, windowed):
     assert lm.engine.cache.free_pages == lm.engine.cache.n_pages
     plain = abacus_b200.LM(folder, max_tokens=64 * 20)
     assert plain.score(texts, from_cache=True)[2].logprobs == plain.score(texts)[2].logprobs
+
+
+@pytest.mark.parametrize("form", ["int8", "e4m3"])
+def test_every_quotient_of_two_mantissas(ops, form):  # noqa: F811
+    """Blocks whose largest number has every mantissa M of 8 bits, with every other mantissa at eight sizes below it, of both signs: each
+    is rounded as the exact quotient is (254 / 255 comes within 2^-16 of a tie, 127 x 2^-s / 255 and others are ties)."""
+    run = Run(1, 1, 64, form, slots=1, pages=40)
+    a = run.open()
+    qkv = torch.zeros((128 * 16, 3 * 64))
+    x = torch.arange(128, 256).float()[:, None] * 2.0 ** -torch.arange(8).float()  # [mantissas, sizes]
+    for i, m in enumerate(range(128, 256)):
+        block = torch.where(x <= m, x, torch.zeros(())).reshape(-1) * (1 - 2 * (torch.arange(1024) % 3 == 0).float())
+        block[0] = m
+        qkv[16 * i:16 * i + 16, 64:] = block.view(16, 64).repeat(1, 2)
+    qkv = qkv.to(torch.bfloat16)
+    assert (qkv[127 * 16:, 64:].float().abs() == 254).any() and float(qkv.abs().max()) == 255
+    run.check(ops, run.write(ops, [(a, 128 * 16)], qkv))
