@@ -7,11 +7,12 @@
 // every pairs-th tile of the line. A thread that reads the accumulator has one row and 128 of a tile's columns; the sums of the
 // group's rows wait in shared memory for the row's next tile, and at the group's end every pair leaves its own for every row.
 // The tensor cores' own sums are cut off, not rounded, at every step of 16 products: over K = 4,096 that leaves log probabilities
-// 1.6e-6 off (against 4e-7 over 1,024), relative to their size. So a long K is multiplied in segments of up to 1,536, each into an
-// accumulator of its own, and the reading threads add them up, in registers, while the tensor cores are on the next one.
-// A second kernel joins the pairs' sums, a warp a row. Measured: 2,048 rows of 1,024 against 151,936 in 515 us, 1,240 TFLOP/s (cuBLAS
-// sustains 1,377 under the power cap); 4,999 rows of 4,096 in 5,300, three segments, 1,174 TFLOP/s (5,280 in two,
-// 4,850 to 5,000 in one). The eight warps that read need 6.5 instructions and one exponential a logit:
+// 1.6e-6 off (against 4e-7 over 1,024), relative to their size, and the entropies of few rows twice as much. So a long K is multiplied in segments
+// of up to 1,024, each into an accumulator of its own, and the reading threads add them up, in registers, while the tensor cores are on the
+// next one. Of 3,000 drawn products of 1 to 4,500 rows 3 had an output more than 1e-6 off; with segments of up to 1,536 30, with 768
+// one, but then K = 1,024 takes two: 2,048 rows 613 us, not 516.
+// A second kernel joins the pairs' sums, a warp a row. Measured: 2,048 rows of 1,024 against 151,936 in 516 us, 1,235 TFLOP/s (cuBLAS
+// sustains 1,377 under the power cap); 4,999 rows of 4,096 in 5,140, four segments, 1,210 TFLOP/s (5,020 in three). The eight warps that read need 6.5 instructions and one exponential a logit:
 // at K = 1,024 half of the time that the tensor cores take for it.
 //
 // Few rows (up to LP_FEW, few_wins): w is all there is to read, and a tile of 256 rows of x of which a few are there costs the tensor cores as much
@@ -31,7 +32,7 @@
 #define LP_STAGES 6
 #define LP_GROUP 8
 #define LP_THREADS 320   // one warp that loads, one that multiplies, eight that read
-#define LP_SEGMENT 24    // blocks of K to a segment at most
+#define LP_SEGMENT 16    // blocks of K to a segment at most
 #define LP_MOST_ROWS 16384  // rows of a launch
 
 struct GemmLogProbs {

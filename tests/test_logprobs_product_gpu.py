@@ -60,7 +60,7 @@ def test_no_token_is_missing_or_counted_twice(ops, m, vocab, k):  # noqa: F811
 def test_a_long_k_is_added_up_in_segments(ops, m, vocab, k):  # noqa: F811
     """One token's logit is a sum S of a first product of 32 and many small ones, the others' are zero: the log probability of another is -S
     (beside e^-S V, which is taken in too). The tensor cores cut off a step of 2^-23 of the running sum at most for every 16 products:
-    in a first segment of 1,536 that is 96 such steps of S at most, in the others, whose sums are small, less than one together, and four
+    in a first segment of 1,024 that is 64 such steps of S at most, in the others, whose sums are small, less than one together, and eight
     roundings more for adding up. In one segment of 8,192 or more the small products lose half a step of S for each 16 on average."""
     g = torch.Generator().manual_seed(k)
     x, w = torch.ones((m, k), dtype=torch.bfloat16), torch.zeros((vocab, k), dtype=torch.bfloat16)
@@ -69,4 +69,4 @@ def test_a_long_k_is_added_up_in_segments(ops, m, vocab, k):  # noqa: F811
     s = float(w[5].double().sum())
     logprob, _ = product(ops, x.cuda(), w.cuda(), [vocab - 1 - r % 2 for r in range(m)])
     want = -s - math.log1p((vocab - 1) * math.exp(-s))
-    assert ((logprob - want).abs() <= s * 2.0 ** -23 * (96 + 1 + 4)).all(), float((logprob - want).abs().max()) / s * 2.0 ** 23
+    assert ((logprob - want).abs() <= s * 2.0 ** -23 * (64 + 1 + 8)).all(), float((logprob - want).abs().max()) / s * 2.0 ** 23
