@@ -89,7 +89,8 @@ def capturable(model):
 class Engine:
     def __init__(self, model, max_tokens, max_slots=None, max_context=None, use_graphs=True, cache=None):
         """cache: "int8" or "e4m3" keeps keys and values in 8 bits with scales (cache/kv8.py; models whose mixers are all plain attention
-        in bfloat16, heads of 64 or 128): half the bytes a token. None: in the model's type."""
+        in bfloat16, heads of 64 or 128): half the bytes a token, and an open block of 16 tokens in bfloat16 a slot beside them (a quarter
+        of a 16-bit page; with a slot a page, the default, 0.75 of the 16-bit cache in all: give max_slots). None: in the model's type."""
         self.model = model
         if cache is not None:
             self._check_kv8(model, cache)

@@ -1,4 +1,6 @@
 """Scoring at its edges: frames that cannot score, and generation that keeps log probabilities beside a step that runs ahead."""
+import math
+
 import pytest
 import torch
 
@@ -114,3 +116,22 @@ def test_the_bound_on_candidates_holds_for_short_slices_and_ranges(dtype, rows, 
     want = torch.sort(x.float(), dim=1, descending=True, stable=True).indices[:, :20]
     assert torch.equal(top[20][0].long(), want) and torch.equal(top[1][0].long(), want[:, :1])
     assert fastest[20] <= 3 * fastest[1], fastest
+
+
+def test_more_rows_than_a_launch_takes():
+    """Rows in launches of 32,768: the last ones too, and nothing behind them."""
+    from abacus_b200.kernels import ops
+    n, vocab = 65600, 131
+    x = (torch.randn((n + 1, vocab), generator=torch.Generator().manual_seed(2)) * 3.0).cuda()
+    tokens = (torch.arange(n + 1, device="cuda") % vocab).to(torch.int32)
+    logprob, entropy, values = (torch.full(s, 7.0, device="cuda") for s in ((n + 1,), (n + 1,), (n + 1, 3)))
+    ids = torch.full((n + 1, 3), 9, dtype=torch.int32, device="cuda")
+    ops.token_logprobs(x, tokens, logprob, entropy=entropy, top_ids=ids, top_logprobs=values, n_rows=n)
+    logp = torch.log_softmax(x[:n].double(), dim=1)
+    order = torch.sort(x[:n], dim=1, descending=True, stable=True).indices[:, :3]
+    off = 2.0 ** -24 * 60  # (sums of 131 terms, each 2^-22 and 2^-23 of its distance off, as test_logprobs_gpu.compare counts them, and a logarithm)
+    for got, want in ((logprob, logp.gather(1, tokens[:n].long()[:, None])[:, 0]), (values, logp.gather(1, order)),
+                      (entropy, -(logp.exp() * logp).sum(dim=1))):
+        assert ((got[:n].double() - want).abs() <= off * (2 + math.log(vocab)) + 2.0 ** -22 * want.abs()).all()
+        assert (got[n] == 7.0).all()
+    assert torch.equal(ids[:n].long(), order) and (ids[n] == 9).all()
