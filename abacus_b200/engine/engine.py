@@ -63,8 +63,8 @@ class Scoring:
     top_logprobs: torch.Tensor = None  # float32 [rows, k]
 
 
-# Tokens whose keys and values a pass over portions reads back from an 8-bit cache at a time (of one sequence, if it holds more): 0.5 GB a
-# layer with 8 kv heads of 128.
+# Tokens whose keys and values a pass over portions reads back from an 8-bit cache at a time (of one sequence, if it holds more): 0.5 GB with
+# 8 kv heads of 128, which all layers use one after the other.
 READ_BACK_TOKENS = 1 << 17
 
 _ONE_TOKEN, _WANT_IT = np.zeros(1, dtype=np.int64), [0]
@@ -236,7 +236,13 @@ class Engine:
                     held = 0
                 portions[-1].append(i)
                 held += s.start + n
-        return [way for way in [*ways.values(), *portions] if way]
+        ways = [way for way in [*ways.values(), *portions] if way]
+        if len(ways) > 1:  # (a wanted place that is not there is refused before any pass runs)
+            for s in seqs:
+                for place in s.want:
+                    if not 0 <= place < len(s.tokens):
+                        raise StepError(f"wanted place {place} is outside the {len(s.tokens)} tokens given")
+        return ways
 
     @staticmethod
     def _rows(seqs):

@@ -265,3 +265,32 @@ def test_every_quotient_of_two_mantissas(ops, form):  # noqa: F811
     qkv = qkv.to(torch.bfloat16)
     assert (qkv[127 * 16:, 64:].float().abs() == 254).any() and float(qkv.abs().max()) == 255
     run.check(ops, run.write(ops, [(a, 128 * 16)], qkv))
+
+
+def test_a_mixed_step_of_a_windowed_model_and_one_that_asks_for_what_is_not_there(tmp_path):
+    """Whole prompts and single tokens of a windowed model in one step give the bits of steps apart; a wanted place beyond a sequence's
+    tokens is refused with no sequence moved, whichever pass it would have been in."""
+    from abacus_b200.engine import Engine
+    model = model_of(windowed_folder(tmp_path))
+    rng = np.random.default_rng(6)
+    first, second, third = (rng.integers(0, 300, n).tolist() for n in (61, 83, 9))
+    got = []
+    for together in (True, False):
+        engine = Engine(model, max_tokens=64 * 12, use_graphs=False, cache="e4m3")
+        a, b, c = (engine.open() for _ in range(3))
+        engine.step([(a, first, []), (c, third, [])])
+        entries = [(a, [5], [0]), (b, second, [3, 82])]
+        if together:
+            for bad in (1, -1):
+                with pytest.raises(ValueError, match="wanted place"):
+                    engine.step([(a, [5], [0]), (b, second, [bad * 83])])
+                with pytest.raises(ValueError, match="wanted place"):
+                    engine.step([(a, [5], [bad]), (b, second, [0])])
+            assert [engine.length(s) for s in (a, b, c)] == [61, 0, 9]
+        steps = [entries] if together else [[e] for e in entries]
+        rows = [engine.step(step).clone() for step in steps]
+        rows.append(engine.step([(a, [7], [0])]).clone())
+        rows.append(engine.step([(b, [8], [0])]).clone())
+        got.append(torch.cat(rows))
+        engine.check_status()
+    assert torch.equal(*got)
